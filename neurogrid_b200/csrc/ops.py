@@ -9,6 +9,7 @@ step, H = model width.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 from typing import Optional, Tuple
 
@@ -18,7 +19,8 @@ from . import build
 
 _c_int, _c_float, _c_void_p, _c_ll = ctypes.c_int, ctypes.c_float, ctypes.c_void_p, ctypes.c_longlong
 
-_ERR = {1: "a size the kernel does not take", 2: "the launch failed", 3: "a dtype the kernel does not take"}
+_ERR = {1: "a size the kernel does not take", 2: "the launch failed", 3: "a dtype the kernel does not take",
+        6: "a page number is outside its pool, is written twice, or is both read and written"}
 
 
 class KernelError(RuntimeError):
@@ -428,6 +430,187 @@ def attn_decode_prep_bf16(qkv: torch.Tensor, q_weight: Optional[torch.Tensor], k
              _ptr(cu_q), _ptr(ctx_before), _ptr(out), _ptr(scratch), n, n_entries, n_heads, n_kv, hd, page_size, num_pages,
              int(window or 0), float(scale), int(n_splits), int(max_ctx), _slopes(slopes, n_heads), _stream()),
            "attn_decode_prep_bf16")
+
+
+# ----------------------------------------------------------------------------- a cache in 8 bits
+Q8_KINDS = {torch.float8_e4m3fn: 0, torch.int8: 1}
+
+
+def _q8_cache(what: str, k_pages, v_pages, k_scales, v_scales, table):
+    """(kind, pages, KV heads, page, head size, block) of a cache in 8 bits, after its checks."""
+    kind = Q8_KINDS.get(k_pages.dtype)
+    if kind is None or v_pages.dtype != k_pages.dtype:
+        raise KernelError(f"{what}: pages in 8 bits are float8_e4m3fn or int8 (keys and values alike), got {k_pages.dtype} and {v_pages.dtype}")
+    if k_pages.dim() != 4 or v_pages.shape != k_pages.shape:
+        raise KernelError(f"{what}: pages are [pages, KV heads, page, head], keys and values alike")
+    num_pages, n_kv, page_size, hd = k_pages.shape
+    if k_scales.shape != v_scales.shape or k_scales.dim() != 3 or tuple(k_scales.shape[:2]) != (num_pages, n_kv) \
+            or k_scales.shape[2] < 1 or page_size % k_scales.shape[2]:
+        raise KernelError(f"{what}: scales are [pages, KV heads, page / block], keys' and values' alike")
+    _f32(k_scales, "key scales"), _f32(v_scales, "value scales"), _i32(table, "table")
+    block = page_size // k_scales.shape[2]
+    if page_size & (page_size - 1) or block & (block - 1) or block < 8:
+        raise KernelError(f"{what}: pages and blocks are powers of two, blocks of at least 8 tokens; got {page_size} and {block}")
+    if hd % 16 or table.dim() != 2:
+        raise KernelError(f"{what}: head sizes are multiples of 16 and the table is [entries, pages]")
+    return kind, num_pages, n_kv, page_size, hd, block
+
+
+def _one_device(what: str, *tensors) -> None:
+    """The launch goes to the current device's stream: what it reads and writes has to be there."""
+    if not torch.cuda.is_available():
+        return                                                # (each tensor's own check says what is wrong)
+    here = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.is_cuda and t.device.index != here:
+            raise KernelError(f"{what}: a tensor is on {t.device}, the current device is cuda:{here}")
+
+
+def cache_write_q8(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, k_scales: torch.Tensor,
+                   v_scales: torch.Tensor, table: torch.Tensor, row_entry: torch.Tensor, cu_q: torch.Tensor,
+                   ctx_before: torch.Tensor, status: torch.Tensor) -> None:
+    """New keys and values k, v [N, nKV * hd] (bfloat16 or float32; each may be a block of columns of a wider buffer) into pages of codes
+    [P, nKV, page, hd], float8_e4m3fn or int8, whose scales [P, nKV, page / block] float32 are powers of two: a code c stands
+    for c * scale.  Entry e's new rows are cu_q[e] .. cu_q[e+1]-1, behind ``ctx_before[e]`` tokens; ``row_entry`` [N] names each row's
+    entry (-1: a padding row, written nowhere).
+
+    A block's scale is the least of 2^-100 .. 2^100 with which the largest finite value of its new tokens is within 448 (e4m3) or 127
+    (int8), and at least its old one where tokens of the entry are already in it; if it grows, their codes are rounded to the new
+    scale.  Codes are rounded to nearest, ties to even; infinities become the largest code, NaN stays NaN in e4m3 and becomes 0 in
+    int8.  Places of a page that no row goes to stay as they were.  A page that is not in the table sets the bad-page bit."""
+    what = "cache_write_q8"
+    kind, num_pages, n_kv, page_size, hd, block = _q8_cache(what, k_pages, v_pages, k_scales, v_scales, table)
+    if k.dim() != 2 or k.shape != v.shape or k.shape[1] != n_kv * hd or k.dtype != v.dtype:
+        raise KernelError(f"{what}: keys {tuple(k.shape)} and values {tuple(v.shape)} do not fit the pages")
+    act = _act_flag(k, "keys")
+    _i32(row_entry, "row_entry"), _i32(cu_q, "cu_q"), _i32(ctx_before, "ctx_before"), _i32(status, "status")
+    n_entries = ctx_before.numel()
+    if row_entry.numel() != k.shape[0] or cu_q.numel() != n_entries + 1 or table.shape[0] < n_entries:
+        raise KernelError(f"{what}: the batch description does not fit {k.shape[0]} rows of {n_entries} entries")
+    _one_device(what, k, v, k_pages, v_pages, k_scales, v_scales, table, row_entry, cu_q, ctx_before, status)
+    f = _fn("cache_q8", "ng_cache_write_q8", [_c_void_p] * 2 + [_c_ll] * 2 + [_c_void_p] * 5 + [_c_int] + [_c_void_p] * 3 + [_c_int] * 9
+            + [_c_void_p] * 2)
+    _check(f(k.data_ptr(), v.data_ptr(), _column_block(k, "keys"), _column_block(v, "values"), _ptr(k_pages), _ptr(v_pages),
+             _ptr(k_scales), _ptr(v_scales), _ptr(table), table.shape[1], _ptr(row_entry), _ptr(cu_q), _ptr(ctx_before), k.shape[0],
+             n_entries, n_kv, hd, page_size, block, num_pages, kind, act, _ptr(status), _stream()), what)
+
+
+def copy_pages(pools, src, dst) -> None:
+    """pool[:, dst[i]] = pool[:, src[i]] for every tensor of ``pools``, each [layers, pages, ...] and contiguous (keys, values and
+    scales of a group of layers go in one launch).  ``src`` and ``dst`` are page numbers on the host: sequences, numpy arrays or CPU
+    tensors.  No page may be written twice, or be read as well as written; a page may be read several times.  The numbers are checked
+    before anything is launched, and travel with the launch: nothing has to be kept for it (a captured graph repeats the same copies)."""
+    import numpy as np
+    what = "copy_pages"
+    if any(isinstance(x, torch.Tensor) and x.is_cuda for x in (src, dst)):
+        raise KernelError(f"{what}: page numbers are host values")
+    a, b = np.asarray(src), np.asarray(dst)
+    if a.size == 0 and b.size == 0:
+        return
+    if a.ndim != 1 or a.shape != b.shape or a.dtype.kind not in "iu" or b.dtype.kind not in "iu":
+        raise KernelError(f"{what}: src and dst are whole numbers, as many of one as of the other")
+    if a.dtype != np.int32 or b.dtype != np.int32:
+        if min(a.min(), b.min()) < 0 or max(a.max(), b.max()) > 0x7fffffff:
+            raise KernelError(f"{what}: {_ERR[6]}")
+    a, b = np.ascontiguousarray(a, dtype=np.int32), np.ascontiguousarray(b, dtype=np.int32)
+    pools = [t for t in pools if t is not None]
+    for t in pools:
+        if t.dim() < 2 or t.shape[1] != pools[0].shape[1]:
+            raise KernelError(f"{what}: pools are [layers, pages, ...] with the same pages")
+        _ptr(t, "a pool")
+    _one_device(what, *pools)
+    pools = [t for t in pools if t.shape[0] and t.numel()]
+    f = _fn("cache_q8", "ng_copy_pages", [_c_void_p] * 4 + [_c_int] + [_c_void_p] * 2 + [_c_int, _c_void_p])
+    for i in range(0, len(pools), 8):
+        part = pools[i:i + 8]
+        n = len(part)
+        base = (ctypes.c_void_p * n)(*[t.data_ptr() for t in part])
+        layers, pages = (ctypes.c_int * n)(*[t.shape[0] for t in part]), (ctypes.c_int * n)(*[t.shape[1] for t in part])
+        size = (ctypes.c_longlong * n)(*[t.stride(1) * t.element_size() if t.shape[1] > 1 else t[0].numel() * t.element_size() for t in part])
+        _check(f(base, layers, pages, size, n, a.ctypes.data, b.ctypes.data, a.size, _stream()), what)
+
+
+def attn_q8_scratch_floats(n_rows: int, n_heads: int, head_dim: int, n_splits: int) -> int:
+    """float32 values the attention over a cache in 8 bits needs when it cuts the keys into ``n_splits`` runs."""
+    return n_rows * n_heads * n_splits * (head_dim + 4) if n_splits > 1 else 0
+
+
+@functools.lru_cache(maxsize=None)
+def _sm_count(device) -> int:
+    return torch.cuda.get_device_properties(device).multi_processor_count
+
+
+def attn_decode_q8_splits(n_single: int, n_heads: int, n_kv_heads: int, head_dim: int, max_ctx: int, window: Optional[int], device) -> int:
+    """Runs ``attn_decode_q8`` should cut the keys into."""
+    span = min(window, max_ctx) if window else max_ctx
+    pairs = max(1, n_single * n_kv_heads * -(-n_heads // n_kv_heads // 16))
+    want = max(-(-4 * _sm_count(device) // pairs), -(-span // 4096))
+    return max(1, min(want, span // 256))
+
+
+def attn_prefill_q8_splits(q_lens, n_heads: int, n_kv_heads: int, head_dim: int, max_ctx: int, window: Optional[int], device) -> int:
+    """Runs ``attn_prefill_q8`` should cut the keys into: where its blocks (128 rows of a KV head's query heads) leave SMs idle and see
+    keys enough to share."""
+    group = n_heads // n_kv_heads
+    blocks = sum(-(-n * group // 128) for n in q_lens) * n_kv_heads
+    span = min(window + max(q_lens), max_ctx) if window else max_ctx
+    return max(1, min(_sm_count(device) // max(1, blocks), span // 512, 65535 // max(1, len(q_lens))))
+
+
+def _q8_attention(what, q, out, scratch, cache, cu_q, ctx_before, n_entries, n_heads, n_splits):
+    kind, num_pages, n_kv, page_size, hd, block = _q8_cache(what, *cache)
+    if q.dtype != torch.bfloat16 or out.dtype != torch.bfloat16:
+        raise KernelError(f"{what} takes bfloat16 queries")
+    if hd > 256:
+        raise KernelError(f"{what}: head size {hd} is above 256")
+    if q.dim() != 2 or q.shape[1] != n_heads * hd or out.shape != q.shape or n_heads % n_kv:
+        raise KernelError(f"{what}: shapes do not fit")
+    if n_splits < 1:
+        raise KernelError(f"{what}: {n_splits} runs")
+    need = attn_q8_scratch_floats(q.shape[0], n_heads, hd, n_splits)
+    if need and (scratch is None or scratch.numel() < need or scratch.dtype != torch.float32):
+        raise KernelError(f"{what} needs {need} float32 values of scratch")
+    _i32(cu_q, "cu_q"), _i32(ctx_before, "ctx_before")
+    if cu_q.numel() < n_entries + 1 or ctx_before.numel() < n_entries or cache[4].shape[0] < n_entries:
+        raise KernelError(f"{what}: the batch description does not fit {n_entries} entries")
+    _one_device(what, q, out, scratch if need else None, *cache, cu_q, ctx_before)
+    return kind, num_pages, n_kv, page_size, hd, block
+
+
+def attn_decode_q8(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, k_scales: torch.Tensor, v_scales: torch.Tensor,
+                   table: torch.Tensor, cu_q: torch.Tensor, ctx_before: torch.Tensor, out: torch.Tensor, scratch: Optional[torch.Tensor],
+                   n_entries: int, n_heads: int, window: Optional[int], scale: float, n_splits: int, max_ctx: int,
+                   slopes: Optional[torch.Tensor] = None) -> None:
+    """``attn_decode_bf16`` over a cache in 8 bits (``cache_write_q8``): split-context attention of the entries that bring one token, any
+    number of query heads a KV head.  The rows of other entries stay as they were.  ``n_splits`` (``attn_decode_q8_splits``) runs of
+    the keys; ``scratch`` holds ``attn_q8_scratch_floats`` float32 values when there is more than one."""
+    cache = (k_pages, v_pages, k_scales, v_scales, table)
+    kind, num_pages, n_kv, page_size, hd, block = _q8_attention("attn_decode_q8", q, out, scratch, cache, cu_q, ctx_before, n_entries,
+                                                                n_heads, n_splits)
+    f = _fn("attention_q8", "ng_attn_decode_q8", [_c_void_p] * 6 + [_c_int] + [_c_void_p] * 4 + [_c_int] * 10
+            + [_c_float, _c_int, _c_int, _c_void_p, _c_void_p], {"NG_HEAD_DIM": hd})
+    _check(f(_ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(k_scales), _ptr(v_scales), _ptr(table), table.shape[1], _ptr(cu_q),
+             _ptr(ctx_before), _ptr(out), _ptr(scratch) if n_splits > 1 else None, q.shape[0], n_entries, n_heads, n_kv, hd, page_size,
+             block, num_pages, kind, int(window or 0), float(scale), int(n_splits), int(max_ctx), _slopes(slopes, n_heads), _stream()),
+           "attn_decode_q8")
+
+
+def attn_prefill_q8(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, k_scales: torch.Tensor, v_scales: torch.Tensor,
+                    table: torch.Tensor, cu_q: torch.Tensor, ctx_before: torch.Tensor, out: torch.Tensor, n_entries: int, max_q: int,
+                    n_heads: int, window: Optional[int], scale: float, skip_single: bool, slopes: Optional[torch.Tensor] = None,
+                    scratch: Optional[torch.Tensor] = None, n_splits: int = 1) -> None:
+    """Flash attention of the step's portions over a cache in 8 bits (``cache_write_q8``); their own keys are read from the cache too.
+    Entries of one token are left to ``attn_decode_q8`` when ``skip_single``.  ``n_splits`` (``attn_prefill_q8_splits``) runs of every
+    block's keys, merged through ``scratch`` (``attn_q8_scratch_floats``)."""
+    cache = (k_pages, v_pages, k_scales, v_scales, table)
+    kind, num_pages, n_kv, page_size, hd, block = _q8_attention("attn_prefill_q8", q, out, scratch, cache, cu_q, ctx_before, n_entries,
+                                                                n_heads, n_splits)
+    f = _fn("attention_q8", "ng_attn_prefill_q8", [_c_void_p] * 6 + [_c_int] + [_c_void_p] * 4 + [_c_int] * 11
+            + [_c_float, _c_int, _c_int, _c_void_p, _c_void_p], {"NG_HEAD_DIM": hd})
+    _check(f(_ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(k_scales), _ptr(v_scales), _ptr(table), table.shape[1], _ptr(cu_q),
+             _ptr(ctx_before), _ptr(out), _ptr(scratch) if n_splits > 1 else None, q.shape[0], n_entries, int(max_q), n_heads, n_kv, hd,
+             page_size, block, num_pages, kind, int(window or 0), float(scale), int(bool(skip_single)), int(n_splits),
+             _slopes(slopes, n_heads), _stream()), "attn_prefill_q8")
 
 
 # ----------------------------------------------------------------------------- attention with float32 weights
