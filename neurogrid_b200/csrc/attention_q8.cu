@@ -61,173 +61,234 @@ struct Cache {
 };
 
 // ===================================================================================== single tokens
-// A block owns one (entry, 16 or fewer query heads of one KV head, run of the keys).  Its four warps take groups of 16 * SUB keys in
-// turn, each on its own (no barrier until the end): the heads are the rows of one MMA tile, the contraction index of q.c and the output
-// dimension are permuted so that a lane reads contiguous bytes, and K and V come from memory into the registers they are used
-// from, the next group's requested before this group is computed.  Nothing passes through shared memory but the four warps' results.
+// A segment is an entry's keys for up to 8 NT query heads of one KV head.  The block's four warps take groups of GROUP keys in turn, each on
+// its own (no barrier until the end of a piece).  Keys are the rows of the first product's tiles and dimensions those of the second's,
+// S^T = K Q^T and O^T = V^T P^T, so that up to eight heads fill a tile's columns: half the products, exponentials and
+// accumulators of heads as rows (16 of them, of which eight stay empty).  The contraction index of the first and the row index of the second are
+// permuted so that a lane reads contiguous bytes.  K and V come from memory into the registers they are used from, the next group's requested
+// before this group is computed and the page numbers a group earlier still; nothing passes through shared memory but the four warps' results.
 //
-// Bound by the codes' bytes.  A lane's words of V hold four keys' codes of one dimension apart; two byte permutations a pair of
-// words put a pair of keys beside each other, as the MMA wants them.
+// Bound by the codes' bytes and by the issue of instructions.  A lane's words of V hold one key's codes each; a byte permutation puts a pair of
+// keys beside each other, as the MMA wants them, and a movmatrix turns a tile of weights from keys x heads to heads x keys.
+//
+// Who does what: with one run, a block has a segment.  With more, the launch has as many blocks as the GPU holds at once and every block finds, from
+// the entries' lengths on the device, its equal share of the turns of all segments laid end to end: pieces of one segment or several.  A piece that
+// is a whole segment writes its output rows; others write records for the merge, the piece's number within the segment as the run's.  So
+// batches of unequal lengths, and segments a little more than the blocks, fill the GPU evenly.
 #define DC_WARPS 4
 #define DC_THREADS (DC_WARPS * 32)
 constexpr int W = HD % 64 == 0 ? 16 : HD % 32 == 0 ? 8 : 4;        // bytes of a key that a lane takes at once (of a value row: half of it)
 constexpr int NC = HD / (4 * W);                                    // such pieces a row has for it
-constexpr int SUB = HD <= 64 ? 2 : 1;                               // 16-key tiles a group has
+constexpr int VW = (W / 2 + 3) / 4;                                 // words that hold a value row's piece
+constexpr int SUB = HD <= 128 ? 2 : 1;                              // 16-key tiles a group has
 constexpr int GROUP = 16 * SUB;
+constexpr int DC_NT_MAX = HD <= 64 ? 2 : 1;                         // 8 heads wide; more heads are blocks of their own
 
+// GRAN (8 or 16): keys that certainly lie in one page and one block; a unit is so many
+template <int GRAN>
 struct DcGroup {
+    static constexpr int UNITS = 16 / GRAN;
     uint32_t k[SUB][2][NC * W / 4];          // keys g and 8 + g of the tile
-    uint32_t v[SUB][4][NC * ((W / 2 + 3) / 4)];       // keys 2t, 2t+1, 8+2t, 8+2t+1
-    float ks[SUB][2], vs[SUB][2];            // of the tile's halves
+    uint32_t v[SUB][4][NC * VW];             // keys 2t, 2t+1, 8+2t, 8+2t+1
+    float ks[SUB][UNITS], vs[SUB][UNITS];
+    uint32_t missing;                        // a bit for each unit whose page is not there
+};
+template <int GRAN>
+struct DcPages { int id[SUB][16 / GRAN]; };
+// where a lane's pieces of a page's keys and values begin (the pointers of page 0), and what a page is long
+struct DcBase {
+    const unsigned char *k, *v;
+    const float *ks, *vs;
+    int page_bytes, page_scales, slot_mask, bl_log2;
 };
 
-// Keys key0 .. key0 + GROUP - 1 of the block's run.  Halves (8 keys: one page, one block) that have no key of the run, and pages
-// that are not there, give zeros.
-__device__ __forceinline__ void dc_load(DcGroup& r, const Cache& c, const int* trow, int key0, int k_end, int kvh) {
-    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    int page[SUB][2];
+template <int GRAN>
+__device__ __forceinline__ void dc_pages(DcPages<GRAN>& p, const Cache& c, const int* trow, int key0, int k_end) {
 #pragma unroll
     for (int s = 0; s < SUB; ++s)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int key = key0 + 16 * s + 8 * h;
-            page[s][h] = key < k_end && (key >> c.ps_log2) < c.table_stride ? trow[key >> c.ps_log2] : -1;
+        for (int u = 0; u < 16 / GRAN; ++u) {
+            const int key = key0 + 16 * s + GRAN * u, i = key >> c.ps_log2;
+            p.id[s][u] = key < k_end && i < c.table_stride ? trow[i] : -1;
         }
+}
+// Keys key0 .. key0 + GROUP - 1 of the block's run.  Of a page that is not there, or a unit behind the run, page 0 is read: the group's keys
+// are then looked at one by one.
+template <int GRAN>
+__device__ __forceinline__ void dc_load(DcGroup<GRAN>& r, const DcBase& b, const DcPages<GRAN>& p, int key0, int num_pages) {
+    r.missing = 0;
 #pragma unroll
     for (int s = 0; s < SUB; ++s)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int slot = (key0 + 16 * s + 8 * h) & ((1 << c.ps_log2) - 1);
-            const bool ok = page[s][h] >= 0 && page[s][h] < c.num_pages;
-            const size_t slab = (size_t)(ok ? page[s][h] : 0) * c.nKV + kvh;
-            const size_t at = ((slab << c.ps_log2) + slot) * HD;
-            const size_t sc = (slab << (c.ps_log2 - c.bl_log2)) + (slot >> c.bl_log2);
-            r.ks[s][h] = ok ? c.ks[sc] : 1.f;
-            r.vs[s][h] = ok ? c.vs[sc] : 1.f;
-#pragma unroll
-            for (int n = 0; n < NC; ++n) {
-#pragma unroll
-                for (int i = 0; i < W / 4; ++i) r.k[s][h][n * (W / 4) + i] = 0;
-                if (ok) ld_codes<W>(&r.k[s][h][n * (W / 4)], c.k + at + (size_t)g * HD + n * 4 * W + t * W);
+        for (int u = 0; u < 16 / GRAN; ++u) {
+            int id = p.id[s][u];
+            if ((unsigned)id >= (unsigned)num_pages) {
+                id = 0;
+                r.missing |= 1u << (s * (16 / GRAN) + u);
             }
-            constexpr int VW = (W / 2 + 3) / 4;
+            const int slot = (key0 + 16 * s + GRAN * u) & b.slot_mask;
+            const long long at = (long long)id * b.page_bytes + slot * HD;
+            const long long sc = (long long)id * b.page_scales + (slot >> b.bl_log2);
+            r.ks[s][u] = b.ks[sc];
+            r.vs[s][u] = b.vs[sc];
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
+            for (int h = 0; h < GRAN / 8; ++h) {
+                const int half = GRAN == 8 ? u : h;
 #pragma unroll
-                for (int n = 0; n < NC; ++n) {
+                for (int n = 0; n < NC; ++n) ld_codes<W>(&r.k[s][half][n * (W / 4)], b.k + at + h * 8 * HD + n * 4 * W);
 #pragma unroll
-                    for (int i = 0; i < VW; ++i) r.v[s][2 * h + j][n * VW + i] = 0;
-                    if (ok) ld_codes<W / 2>(&r.v[s][2 * h + j][n * VW], c.v + at + (size_t)(2 * t + j) * HD + n * 4 * W + g * (W / 2));
-                }
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int n = 0; n < NC; ++n) ld_codes<W / 2>(&r.v[s][2 * half + j][n * VW], b.v + at + (h * 8 + j) * HD + n * 4 * W);
+            }
         }
 }
 
+// Of the heads 2t and 2t+1 (and, for the second tile of heads, 8 + those): accumulators, reference point, sum.
+template <int NT>
 struct DcState {
-    float o[HD / 8][4], m_lo, m_hi, l_lo, l_hi;
+    float o[NT][HD / 16][4], m[NT][2], l[NT][2];
+    uint32_t seen;                           // a bit for each tile of heads: a key has been met
 };
+__device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
 
-// One group into the warp's state.  f_lo, f_hi: what the raw products of the lane's two rows are multiplied by (base 2).
-template <int KIND>
-__device__ __forceinline__ void dc_compute(DcState& st, const DcGroup& r, const uint32_t (&qa)[HD / 16][4], int key0, int key_lo, int k_end,
-                                           int pos, float f_lo, float f_hi, float slope_lo, float slope_hi) {
-    const int t = threadIdx.x & 3;
-    float sc[SUB][2][4];
+// One group into the warp's state.  f: what the raw products of the lane's heads are multiplied by (base 2).
+template <int KIND, int NT, int GRAN>
+__device__ __forceinline__ void dc_compute(DcState<NT>& st, DcGroup<GRAN>& r, const uint32_t (&qb)[NT][HD / 16][2], int key0, int key_lo,
+                                           int k_end, int pos, const float (&f)[NT][2], const float (&slope)[NT][2], bool biased) {
+    const int g = (threadIdx.x & 31) >> 2, t = threadIdx.x & 3;
+    constexpr int UNITS = 16 / GRAN;
+    float sc[NT][SUB][4];
 #pragma unroll
     for (int s = 0; s < SUB; ++s)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            sc[s][h][0] = sc[s][h][1] = sc[s][h][2] = sc[s][h][3] = 0.f;
+        for (int n = 0; n < NT; ++n) sc[n][s][0] = sc[n][s][1] = sc[n][s][2] = sc[n][s][3] = 0.f;
 #pragma unroll
-            for (int i = 0; i < HD / 16; ++i) {
-                uint32_t b0, b1;
-                q8_to_half<KIND>(r.k[s][h][i], b0, b1);
-                mma_f16(sc[s][h], qa[i], b0, b1);
-            }
+    for (int s = 0; s < SUB; ++s)
+#pragma unroll
+        for (int i = 0; i < HD / 16; ++i) {
+            uint32_t a[4];
+            q8_to_half<KIND>(r.k[s][0][i], a[0], a[2]);
+            q8_to_half<KIND>(r.k[s][1][i], a[1], a[3]);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma_f16(sc[n][s], a, qb[n][i][0], qb[n][i][1]);
         }
-    const bool whole = key0 >= key_lo && key0 + GROUP <= k_end;
-    float mx_lo = -INFINITY, mx_hi = -INFINITY;
+    const bool whole = key0 >= key_lo && key0 + GROUP <= k_end && r.missing == 0;
+    if (!whole)                                                      // scales of units that no key is seen of may be NaN
 #pragma unroll
-    for (int s = 0; s < SUB; ++s)
+        for (int s = 0; s < SUB; ++s)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const float a = f_lo * r.ks[s][h], b = f_hi * r.ks[s][h], lg = q8_log2(r.vs[s][h]);
+            for (int u = 0; u < UNITS; ++u) {
+                const int key = key0 + 16 * s + GRAN * u;
+                if (key >= k_end || key + GRAN <= key_lo || (r.missing >> (s * UNITS + u) & 1)) r.ks[s][u] = r.vs[s][u] = 1.f;
+            }
+    // z less the reference point as it stands: what 2^ is taken of, unless the point has to move
+    float mx[NT][2];
+    bool up = false;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        mx[n][0] = mx[n][1] = -INFINITY;
+#pragma unroll
+        for (int s = 0; s < SUB; ++s)
+#pragma unroll
+            for (int u = 0; u < UNITS; ++u) {
+                const float lg = q8_log2(r.vs[s][u]);
+#pragma unroll
+                for (int j = 0; j < 4 / UNITS; ++j) {                // of a unit: [half of the tile,] head
+                    const int c = UNITS == 1 ? j : 2 * u + j;
+                    sc[n][s][c] = fmaf(sc[n][s][c], f[n][j & 1] * r.ks[s][u], lg - st.m[n][j & 1]);
+                }
+            }
+        if (biased || !whole)
+#pragma unroll
+            for (int s = 0; s < SUB; ++s)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int key = key0 + 16 * s + 8 * (j >> 1) + g;
+                    const bool seen = whole || (key >= key_lo && key < k_end && !(r.missing >> (s * UNITS + (j >> 1) * (UNITS - 1)) & 1));
+                    sc[n][s][j] = seen ? fmaf(-slope[n][j & 1], (float)(pos - key), sc[n][s][j]) : -INFINITY;
+                }
+#pragma unroll
+        for (int s = 0; s < SUB; ++s)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) mx[n][j & 1] = fmaxf(mx[n][j & 1], sc[n][s][j]);
+        up |= fmaxf(mx[n][0], mx[n][1]) > 8.f || !(st.seen >> n & 1);
+    }
+    // the reference point follows the maximum lazily: weights may reach 2^8 before the sums are rescaled.  It starts at 0 and moves to a head's
+    // first maximum, up or down, with sums that are zero.
+    if (__any_sync(0xffffffffu, up)) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            bool any = true;
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                const int key = key0 + 16 * s + 8 * h + 2 * t + j;
-                const bool ok = whole || (key >= key_lo && key < k_end);
-                const float away = (float)(pos - key);
-                sc[s][h][j] = ok ? fmaf(-slope_lo, away, fmaf(sc[s][h][j], a, lg)) : -INFINITY;
-                sc[s][h][2 + j] = ok ? fmaf(-slope_hi, away, fmaf(sc[s][h][2 + j], b, lg)) : -INFINITY;
-                mx_lo = fmaxf(mx_lo, sc[s][h][j]);
-                mx_hi = fmaxf(mx_hi, sc[s][h][2 + j]);
+                float x = mx[n][j];
+#pragma unroll
+                for (int o = 4; o <= 16; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+                const bool first = !(st.seen >> n & 1);
+                const float by = x == -INFINITY ? 0.f : first ? x : fmaxf(x, 0.f), c = ex2(-by);
+                any = any && x != -INFINITY;
+                st.m[n][j] += by;
+                st.l[n][j] *= first ? 1.f : c;
+#pragma unroll
+                for (int i = 0; i < HD / 16; ++i)
+                    if (!first) { st.o[n][i][j] *= c; st.o[n][i][2 + j] *= c; }
+#pragma unroll
+                for (int s = 0; s < SUB; ++s) { sc[n][s][j] -= by; sc[n][s][2 + j] -= by; }
             }
+            if (__any_sync(0xffffffffu, any)) st.seen |= 1u << n;     // (a key is seen by all heads or by none)
         }
-    // the reference point follows the maximum lazily: weights may reach 2^8 before the sums are rescaled
-    if (__any_sync(0xffffffffu, mx_lo > st.m_lo + 8.f || mx_hi > st.m_hi + 8.f || st.m_lo == -INFINITY || st.m_hi == -INFINITY)) {
-#pragma unroll
-        for (int x = 1; x <= 2; x <<= 1) {
-            mx_lo = fmaxf(mx_lo, __shfl_xor_sync(0xffffffffu, mx_lo, x));
-            mx_hi = fmaxf(mx_hi, __shfl_xor_sync(0xffffffffu, mx_hi, x));
-        }
-        const float n_lo = fmaxf(st.m_lo, mx_lo), n_hi = fmaxf(st.m_hi, mx_hi);
-        const float c_lo = n_lo == -INFINITY ? 1.f : ex2(st.m_lo - n_lo), c_hi = n_hi == -INFINITY ? 1.f : ex2(st.m_hi - n_hi);
-        st.m_lo = n_lo;
-        st.m_hi = n_hi;
-        st.l_lo *= c_lo;
-        st.l_hi *= c_hi;
-#pragma unroll
-        for (int i = 0; i < HD / 8; ++i) { st.o[i][0] *= c_lo; st.o[i][1] *= c_lo; st.o[i][2] *= c_hi; st.o[i][3] *= c_hi; }
     }
-    const float ref_lo = st.m_lo == -INFINITY ? 0.f : st.m_lo, ref_hi = st.m_hi == -INFINITY ? 0.f : st.m_hi;
+    uint32_t pb[NT][SUB][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int s = 0; s < SUB; ++s) {
+            float p[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) p[j] = ex2(sc[n][s][j]);
+            if constexpr (UNITS == 1) {
+                const float inv = q8_recip(r.vs[s][0]);
+                st.l[n][0] = fmaf(p[0] + p[2], inv, st.l[n][0]);
+                st.l[n][1] = fmaf(p[1] + p[3], inv, st.l[n][1]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) st.l[n][j & 1] = fmaf(p[j], q8_recip(r.vs[s][j >> 1]), st.l[n][j & 1]);
+            }
+            pb[n][s][0] = movmatrix(pack_f16(p[0], p[1]));
+            pb[n][s][1] = movmatrix(pack_f16(p[2], p[3]));
+        }
+    }
 #pragma unroll
     for (int s = 0; s < SUB; ++s) {
-        uint32_t pa[4];
+        if (!whole)                                                  // a key that no row sees has a weight of 0, but its codes may be NaN
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const float p0 = ex2(sc[s][h][0] - ref_lo), p1 = ex2(sc[s][h][1] - ref_lo);
-            const float p2 = ex2(sc[s][h][2] - ref_hi), p3 = ex2(sc[s][h][3] - ref_hi);
-            const float inv = q8_recip(r.vs[s][h]);
-            st.l_lo = fmaf(p0 + p1, inv, st.l_lo);
-            st.l_hi = fmaf(p2 + p3, inv, st.l_hi);
-            pa[2 * h] = pack_f16(p0, p1);
-            pa[2 * h + 1] = pack_f16(p2, p3);
-        }
-        uint32_t v[4][sizeof(r.v[0][0]) / 4];
+            for (int j = 0; j < 4; ++j) {
+                const int key = key0 + 16 * s + 8 * (j >> 1) + 2 * t + (j & 1);
+                if (key < key_lo || key >= k_end || (r.missing >> (s * UNITS + (j >> 1) * (UNITS - 1)) & 1))
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            // a key that no row sees has a weight of 0, but its codes may be NaN
-            const int key = key0 + 16 * s + 8 * (j >> 1) + 2 * t + (j & 1);
-            const bool ok = whole || (key >= key_lo && key < k_end);
-#pragma unroll
-            for (int i = 0; i < (int)(sizeof(r.v[0][0]) / 4); ++i) v[j][i] = ok ? r.v[s][j][i] : 0u;
-        }
-        if constexpr (W >= 8) {
-#pragma unroll
-            for (int i = 0; i < HD / 32; ++i) {                     // a word: four dimensions
-                uint32_t b0[4], b1[4];
-                q8_to_half<KIND>(__byte_perm(v[0][i], v[1][i], 0x5140), b0[0], b0[1]);
-                q8_to_half<KIND>(__byte_perm(v[0][i], v[1][i], 0x7362), b0[2], b0[3]);
-                q8_to_half<KIND>(__byte_perm(v[2][i], v[3][i], 0x5140), b1[0], b1[1]);
-                q8_to_half<KIND>(__byte_perm(v[2][i], v[3][i], 0x7362), b1[2], b1[3]);
-#pragma unroll
-                for (int d = 0; d < 4; ++d) mma_f16(st.o[4 * i + d], pa, b0[d], b1[d]);
+                    for (int i = 0; i < NC * VW; ++i) r.v[s][j][i] = 0u;
             }
-        } else {
 #pragma unroll
-            for (int i = 0; i < NC; ++i) {                          // two dimensions in a word's lower half
-                uint32_t b0[2], b1[2];
-                q8_to_half<KIND>(__byte_perm(v[0][i], v[1][i], 0x5140), b0[0], b0[1]);
-                q8_to_half<KIND>(__byte_perm(v[2][i], v[3][i], 0x5140), b1[0], b1[1]);
+        for (int i = 0; i < NC * VW; ++i)                            // a word: four dimensions (two where W is 4), two tiles (one)
 #pragma unroll
-                for (int d = 0; d < 2; ++d) mma_f16(st.o[2 * i + d], pa, b0[d], b1[d]);
+            for (int d = 0; d < (W >= 8 ? 2 : 1); ++d) {
+                uint32_t a[4];
+                q8_to_half<KIND>(__byte_perm(r.v[s][0][i], r.v[s][1][i], d ? 0x7362 : 0x5140), a[0], a[1]);
+                q8_to_half<KIND>(__byte_perm(r.v[s][2][i], r.v[s][3][i], d ? 0x7362 : 0x5140), a[2], a[3]);
+#pragma unroll
+                for (int n = 0; n < NT; ++n) mma_f16(st.o[n][W >= 8 ? 2 * i + d : i], a, pb[n][s][0], pb[n][s][1]);
             }
-        }
     }
 }
-// the head's dimension of column n (0..7) of MMA tile i
-__device__ __forceinline__ int dc_dim(int i, int n) {
+// the dimension that rows g (upper 0) and g + 8 (upper 1) of tile i of O^T are
+__device__ __forceinline__ int dc_dim(int i, int g, int upper) {
     constexpr int PER = W / 2;                                       // dimensions a lane group has of a piece
-    return (i / PER) * 8 * PER + n * PER + i % PER;
+    return (2 * i / PER) * 8 * PER + g * PER + 2 * i % PER + upper;
 }
 
 struct DcArgs {
@@ -237,119 +298,176 @@ struct DcArgs {
     bf16* out;
     float* scratch;
     const float* slopes;
-    int n_rows, nH, chunks, window, n_splits, keys_per_split;
+    int n_rows, n_entries, nH, chunks, window, n_splits;
     float scale;
 };
+constexpr int TURN = DC_WARPS * GROUP;                               // keys of a turn of the four warps
+// turns of an entry's segments (0: not a single token, or a row that the buffers do not hold)
+__device__ __forceinline__ int dc_turns(const DcArgs& a, int e) {
+    const int row = a.cu_q[e], pos = a.ctx_before[e];
+    if (a.cu_q[e + 1] - row != 1 || row < 0 || row >= a.n_rows || pos < 0) return 0;
+    const int lo = a.window > 0 ? max(0, pos - a.window + 1) & ~(GROUP - 1) : 0;
+    return (pos - lo) / TURN + 1;
+}
 
-template <int KIND>
-__global__ void __launch_bounds__(DC_THREADS, HD <= 64 ? 4 : HD <= 128 ? 3 : 2)
-attn_decode_q8_kernel(const DcArgs a) {
-    extern __shared__ float red_s[];                                 // [warp][head][REC]
-    ng_pdl_trigger();
-    const int e = blockIdx.y, kvh = blockIdx.x / a.chunks, split = blockIdx.z;
-    const int row = a.cu_q[e], n_here = a.cu_q[e + 1] - row, pos = a.ctx_before[e];
-    ng_pdl_wait();
-    if (n_here != 1 || row < 0 || row >= a.n_rows || pos < 0) return;
-    const int G = a.nH / a.c.nKV, h0 = (blockIdx.x - kvh * a.chunks) * 16, heads = min(16, G - h0);
+// A team is a block for each segment of an entry; its blocks have the same share of the keys, so that the heads of a page, which lie side by side in
+// memory, are read at about the same time.  The team's share: turns [first, last) of all entries laid end to end, of which entry e's begin at
+// `before`.  Every warp finds it for itself, 32 entries at a time.  Few entries: they count as whole multiples of the share, so that no team has
+// pieces of two.
+struct DcShare { int first, last, each, before, e; bool even; };
+__device__ __forceinline__ int dc_length(const DcShare& sh, int turns) { return sh.even ? (turns + sh.each - 1) / sh.each * sh.each : turns; }
+__device__ __forceinline__ DcShare dc_share(const DcArgs& a, int team, int teams) {
+    const int lane = threadIdx.x & 31;
+    int total = 0, most = 0, live = 0;
+    for (int e0 = 0; e0 < a.n_entries; e0 += 32) {
+        const int n = e0 + lane < a.n_entries ? dc_turns(a, e0 + lane) : 0;
+        total += __reduce_add_sync(0xffffffffu, n);
+        most = max(most, __reduce_max_sync(0xffffffffu, n));
+        live += __popc(__ballot_sync(0xffffffffu, n > 0));
+    }
+    DcShare sh;
+    sh.even = 4 * live <= teams;
+    // none so small that an entry has more pieces than there are records for
+    sh.each = max(sh.even ? (total + teams - live - 1) / max(1, teams - live) : (total + teams - 1) / teams,
+                  (most + a.n_splits - 2) / (a.n_splits - 1));
+    sh.each = max(sh.each, 1);
+    sh.first = sh.last = sh.before = sh.e = 0;
+    const long long want = (long long)sh.each * team;
+    int before = 0;
+    for (int e0 = 0; e0 < a.n_entries; e0 += 32) {
+        const int n = e0 + lane < a.n_entries ? dc_length(sh, dc_turns(a, e0 + lane)) : 0;
+        int upto = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += x;
+        }
+        const uint32_t in = __ballot_sync(0xffffffffu, want < before + upto);
+        if (in) {
+            const int l = __ffs(in) - 1;
+            sh.before = before + __shfl_sync(0xffffffffu, upto - n, l);
+            sh.e = e0 + l;
+            sh.first = (int)want;
+            sh.last = sh.first + sh.each;                            // (the caller stops behind the last entry)
+            break;
+        }
+        before += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    return sh;
+}
+
+template <int KIND, int NT, int GRAN>
+__device__ __forceinline__ void dc_piece(const DcArgs& a, float* red_s, int e, int segment, int turn0, int turn1, int run, int runs) {
+    const int row = a.cu_q[e], pos = a.ctx_before[e], kvh = segment / a.chunks;
+    const int G = a.nH / a.c.nKV, h0 = (segment - kvh * a.chunks) * 8 * NT, heads = min(8 * NT, G - h0);
     const int head0 = kvh * G + h0;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int key_lo = a.window > 0 ? max(0, pos - a.window + 1) : 0;
-    const int k_begin = (key_lo & ~(GROUP - 1)) + split * a.keys_per_split;
-    // the last run takes what is left: a caller's bound on the keys that is too low costs time, not keys
-    const int k_end = split == a.n_splits - 1 ? pos + 1 : min(pos + 1, k_begin + a.keys_per_split);
+    const int k_begin = (key_lo & ~(GROUP - 1)) + turn0 * TURN, k_end = min(pos + 1, k_begin + (turn1 - turn0) * TURN);
     const int* trow = a.c.table + (size_t)e * a.c.table_stride;
+    constexpr int STEP = TURN;
 
-    DcGroup cur, nxt;
+    DcGroup<GRAN> cur, nxt;
+    DcPages<GRAN> pages;
+    DcBase base;
+    base.page_scales = a.c.nKV << (a.c.ps_log2 - a.c.bl_log2);
+    base.page_bytes = (a.c.nKV << a.c.ps_log2) * HD;
+    base.k = a.c.k + (kvh << a.c.ps_log2) * HD + g * HD + t * W;
+    base.v = a.c.v + (kvh << a.c.ps_log2) * HD + 2 * t * HD + g * (W / 2);
+    base.ks = a.c.ks + (kvh << (a.c.ps_log2 - a.c.bl_log2));
+    base.vs = a.c.vs + (kvh << (a.c.ps_log2 - a.c.bl_log2));
+    base.slot_mask = (1 << a.c.ps_log2) - 1;
+    base.bl_log2 = a.c.bl_log2;
     int key0 = k_begin + warp * GROUP;
-    if (key0 < k_end) dc_load(cur, a.c, trow, key0, k_end, kvh);
-
-    // rows of the MMA tile: the block's heads (rows beyond them are zero), each divided by a power of two
-    uint32_t qa[HD / 16][4];
-    float f_lo, f_hi, slope_lo = 0.f, slope_hi = 0.f;
-    {
-        const bf16* q = ng_after_wait(a.q) + ((size_t)row * a.nH + head0) * HD;
-        uint2 lo[HD / 16], hi[HD / 16];
-        float top_lo = 0.f, top_hi = 0.f;
-        auto top_of = [](uint2 w, float top) {
-            const uint32_t x[4] = {w.x << 16, w.x & 0xffff0000u, w.y << 16, w.y & 0xffff0000u};
+    if (key0 < k_end) {
+        dc_pages(pages, a.c, trow, key0, k_end);
+        dc_load(cur, base, pages, key0, a.c.num_pages);
+        dc_pages(pages, a.c, trow, key0 + STEP, k_end);
+    }
+    // columns of the MMA tiles: the block's heads (beyond them: zeros), each divided by a power of two
+    uint32_t qb[NT][HD / 16][2];
+    float f[NT][2], slope[NT][2];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float v = fabsf(__uint_as_float(x[i]));
-                top = v < INFINITY ? fmaxf(top, v) : top;
-            }
-            return top;
-        };
+    for (int n = 0; n < NT; ++n) {
+        const int h = 8 * n + g;
+        const bf16* q = ng_after_wait(a.q) + ((size_t)row * a.nH + head0 + h) * HD;
+        uint2 w[HD / 16];
+        float top = 0.f;
 #pragma unroll
         for (int i = 0; i < HD / 16; ++i) {
             const int d = (i / (W / 4)) * 4 * W + t * W + (i % (W / 4)) * 4;
-            lo[i] = g < heads ? *reinterpret_cast<const uint2*>(q + (size_t)g * HD + d) : make_uint2(0u, 0u);
-            hi[i] = g + 8 < heads ? *reinterpret_cast<const uint2*>(q + (size_t)(g + 8) * HD + d) : make_uint2(0u, 0u);
-            top_lo = top_of(lo[i], top_lo);
-            top_hi = top_of(hi[i], top_hi);
-        }
+            w[i] = h < heads ? *reinterpret_cast<const uint2*>(q + d) : make_uint2(0u, 0u);
+            const uint32_t x[4] = {w[i].x << 16, w[i].x & 0xffff0000u, w[i].y << 16, w[i].y & 0xffff0000u};
 #pragma unroll
-        for (int x = 1; x <= 2; x <<= 1) {
-            top_lo = fmaxf(top_lo, __shfl_xor_sync(0xffffffffu, top_lo, x));
-            top_hi = fmaxf(top_hi, __shfl_xor_sync(0xffffffffu, top_hi, x));
+            for (int j = 0; j < 4; ++j) {
+                const float v = fabsf(__uint_as_float(x[j]));
+                top = v < INFINITY ? fmaxf(top, v) : top;
+            }
         }
-        const int e_lo = q_exponent(top_lo), e_hi = q_exponent(top_hi);
-        const float d_lo = pow2_any(-e_lo), d_hi = pow2_any(-e_hi);
-        f_lo = a.scale * LOG2E * pow2_any(e_lo);
-        f_hi = a.scale * LOG2E * pow2_any(e_hi);
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const int ex = q_exponent(top);
+        const float div = pow2_any(-ex), mul = a.scale * LOG2E * pow2_any(ex);
+        const float sl = a.slopes && h < heads ? a.slopes[head0 + h] * LOG2E : 0.f;
 #pragma unroll
         for (int i = 0; i < HD / 16; ++i) {
-            qa[i][0] = pack_f16(__uint_as_float(lo[i].x << 16) * d_lo, __uint_as_float(lo[i].x & 0xffff0000u) * d_lo);
-            qa[i][2] = pack_f16(__uint_as_float(lo[i].y << 16) * d_lo, __uint_as_float(lo[i].y & 0xffff0000u) * d_lo);
-            qa[i][1] = pack_f16(__uint_as_float(hi[i].x << 16) * d_hi, __uint_as_float(hi[i].x & 0xffff0000u) * d_hi);
-            qa[i][3] = pack_f16(__uint_as_float(hi[i].y << 16) * d_hi, __uint_as_float(hi[i].y & 0xffff0000u) * d_hi);
+            qb[n][i][0] = pack_f16(__uint_as_float(w[i].x << 16) * div, __uint_as_float(w[i].x & 0xffff0000u) * div);
+            qb[n][i][1] = pack_f16(__uint_as_float(w[i].y << 16) * div, __uint_as_float(w[i].y & 0xffff0000u) * div);
         }
-        if (a.slopes && g < heads) slope_lo = a.slopes[head0 + g] * LOG2E;
-        if (a.slopes && g + 8 < heads) slope_hi = a.slopes[head0 + g + 8] * LOG2E;
-    }
-    DcState st;
 #pragma unroll
-    for (int i = 0; i < HD / 8; ++i) st.o[i][0] = st.o[i][1] = st.o[i][2] = st.o[i][3] = 0.f;
-    st.m_lo = st.m_hi = -INFINITY;
-    st.l_lo = st.l_hi = 0.f;
-    constexpr int STEP = DC_WARPS * GROUP;
+        for (int j = 0; j < 2; ++j) {
+            f[n][j] = __shfl_sync(0xffffffffu, mul, (2 * t + j) * 4);
+            slope[n][j] = __shfl_sync(0xffffffffu, sl, (2 * t + j) * 4);
+        }
+    }
+    DcState<NT> st;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int i = 0; i < HD / 16; ++i) st.o[n][i][0] = st.o[n][i][1] = st.o[n][i][2] = st.o[n][i][3] = 0.f;
+        st.m[n][0] = st.m[n][1] = st.l[n][0] = st.l[n][1] = 0.f;
+    }
+    st.seen = 0;
+    const bool biased = a.slopes != nullptr;
     if constexpr (HD <= 128) {
         for (; key0 < k_end; key0 += 2 * STEP) {
-            if (key0 + STEP < k_end) dc_load(nxt, a.c, trow, key0 + STEP, k_end, kvh);
-            dc_compute<KIND>(st, cur, qa, key0, key_lo, k_end, pos, f_lo, f_hi, slope_lo, slope_hi);
+            if (key0 + STEP < k_end) {
+                dc_load(nxt, base, pages, key0 + STEP, a.c.num_pages);
+                dc_pages(pages, a.c, trow, key0 + 2 * STEP, k_end);
+            }
+            dc_compute<KIND, NT, GRAN>(st, cur, qb, key0, key_lo, k_end, pos, f, slope, biased);
             if (key0 + STEP >= k_end) break;
-            if (key0 + 2 * STEP < k_end) dc_load(cur, a.c, trow, key0 + 2 * STEP, k_end, kvh);
-            dc_compute<KIND>(st, nxt, qa, key0 + STEP, key_lo, k_end, pos, f_lo, f_hi, slope_lo, slope_hi);
+            if (key0 + 2 * STEP < k_end) {
+                dc_load(cur, base, pages, key0 + 2 * STEP, a.c.num_pages);
+                dc_pages(pages, a.c, trow, key0 + 3 * STEP, k_end);
+            }
+            dc_compute<KIND, NT, GRAN>(st, nxt, qb, key0 + STEP, key_lo, k_end, pos, f, slope, biased);
         }
     } else {                                                         // a group of a wide head fills the registers
         for (; key0 < k_end; key0 += STEP) {
-            dc_compute<KIND>(st, cur, qa, key0, key_lo, k_end, pos, f_lo, f_hi, slope_lo, slope_hi);
-            if (key0 + STEP < k_end) dc_load(cur, a.c, trow, key0 + STEP, k_end, kvh);
+            dc_compute<KIND, NT, GRAN>(st, cur, qb, key0, key_lo, k_end, pos, f, slope, biased);
+            if (key0 + STEP < k_end) {
+                dc_load(cur, base, pages, key0 + STEP, a.c.num_pages);
+                dc_pages(pages, a.c, trow, key0 + 2 * STEP, k_end);
+            }
         }
-    }
-#pragma unroll
-    for (int x = 1; x <= 2; x <<= 1) {
-        st.l_lo += __shfl_xor_sync(0xffffffffu, st.l_lo, x);
-        st.l_hi += __shfl_xor_sync(0xffffffffu, st.l_hi, x);
     }
     // the four warps' results, merged in order
-    float* mine = red_s + (size_t)(warp * heads + g) * REC;
-    if (g < heads) {
-        if (t == 0) mine[0] = st.m_lo, mine[1] = st.l_lo;
 #pragma unroll
-        for (int i = 0; i < HD / 8; ++i) {
-            mine[4 + dc_dim(i, 2 * t)] = st.o[i][0];
-            mine[4 + dc_dim(i, 2 * t + 1)] = st.o[i][1];
-        }
-    }
-    if (g + 8 < heads) {
-        mine += 8 * REC;
-        if (t == 0) mine[0] = st.m_hi, mine[1] = st.l_hi;
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int i = 0; i < HD / 8; ++i) {
-            mine[4 + dc_dim(i, 2 * t)] = st.o[i][2];
-            mine[4 + dc_dim(i, 2 * t + 1)] = st.o[i][3];
+        for (int j = 0; j < 2; ++j) {
+            float l = st.l[n][j];
+#pragma unroll
+            for (int o = 4; o <= 16; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+            const int h = 8 * n + 2 * t + j;
+            if (h >= heads) continue;
+            float* mine = red_s + (size_t)(warp * heads + h) * REC;
+            if (g == 0) mine[0] = st.seen >> n & 1 ? st.m[n][j] : -INFINITY, mine[1] = l;
+#pragma unroll
+            for (int i = 0; i < HD / 16; ++i)
+                *reinterpret_cast<float2*>(mine + 4 + dc_dim(i, g, 0)) = make_float2(st.o[n][i][j], st.o[n][i][2 + j]);
         }
-    }
     __syncthreads();
     for (int idx = threadIdx.x; idx < heads * HD; idx += DC_THREADS) {
         const int h = idx / HD, d = idx % HD;
@@ -359,61 +477,146 @@ attn_decode_q8_kernel(const DcArgs a) {
 #pragma unroll
         for (int w = 0; w < DC_WARPS; ++w) {
             const float* rec = red_s + (size_t)(w * heads + h) * REC;
-            const float f = rec[0] == -INFINITY ? (m == -INFINITY ? 1.f : 0.f) : ex2(rec[0] - m);       // (a warp that met only NaN kept its sums)
-            l = fmaf(rec[1], f, l);
-            acc = fmaf(rec[4 + d], f, acc);
+            const float c = rec[0] == -INFINITY ? (m == -INFINITY ? 1.f : 0.f) : ex2(rec[0] - m);       // (a warp that met only NaN kept its sums)
+            l = fmaf(rec[1], c, l);
+            acc = fmaf(rec[4 + d], c, acc);
         }
         const size_t at = (size_t)row * a.nH + head0 + h;
-        if (a.n_splits == 1) {
+        float* rec = a.scratch + (at * a.n_splits + run) * REC;
+        if (runs == 1) {
             a.out[at * HD + d] = __float2bfloat16_rn(l == 0.f ? 0.f : acc / l);
         } else {
-            float* rec = a.scratch + (at * a.n_splits + split) * REC;
             rec[4 + d] = acc;
             if (d == 0) rec[0] = m, rec[1] = l;
         }
+        if (d == 0 && run == 0 && a.n_splits > 1) rec[2] = (float)runs;          // the merge asks the first record
     }
 }
 
-// out[row, head] = sum_s o_s 2^(m_s - m) / sum_s l_s 2^(m_s - m) over the runs s, in ascending order within each of GROUPS
-// groups of them, then the groups.  A block has a (row, head); its rows are the entries' single tokens, or (portions) all rows of the
-// entries that bring more.
-template <int GROUPS>
-__global__ void __launch_bounds__(GROUPS * HD)
-attn_q8_merge_kernel(const float* __restrict__ scratch, const int* __restrict__ cu_q, bf16* __restrict__ out, int nH, int n_splits,
-                     int n_rows, int least, int most) {
+template <int KIND, int NT, int GRAN>
+__global__ void __launch_bounds__(DC_THREADS, HD <= 64 && NT == 1 ? 3 : 2)
+attn_decode_q8_kernel(const DcArgs a) {
+    extern __shared__ float red_s[];                                 // [warp][head][REC]
     ng_pdl_trigger();
-    const int e = blockIdx.y, head = blockIdx.x;
+    const int segments = a.c.nKV * a.chunks;
+    if (a.n_splits == 1) {
+        const int e = blockIdx.x / segments, n = dc_turns(a, e);
+        ng_pdl_wait();
+        if (n) dc_piece<KIND, NT, GRAN>(a, red_s, e, blockIdx.x - e * segments, 0, n, 0, 1);
+        return;
+    }
+    const int team = blockIdx.x / segments, segment = blockIdx.x - team * segments;
+    DcShare sh = dc_share(a, team, gridDim.x / segments);
+    ng_pdl_wait();
+    for (int at = sh.first; at < sh.last && sh.e < a.n_entries;) {
+        const int turns = dc_turns(a, sh.e), end = sh.before + dc_length(sh, turns);        // (entries without a single token have none)
+        if (at < end) {
+            const int turn0 = at - sh.before, turn1 = min(turns, sh.last - sh.before);
+            const int t0 = sh.before / sh.each, t1 = (sh.before + turns - 1) / sh.each;
+            if (at != sh.first) __syncthreads();                     // the piece before has been merged
+            dc_piece<KIND, NT, GRAN>(a, red_s, sh.e, segment, turn0, turn1, team - t0, t1 - t0 + 1);
+        }
+        at = max(at, end);
+        sh.before = end;
+        ++sh.e;
+    }
+}
+
+// out[row, head] = sum_s o_s 2^(m_s - m) / sum_s l_s 2^(m_s - m) over the runs s.  A warp has a (row, head) (WIDE: all four warps of a block, every
+// fourth run each, joined in order): lane s looks after run s's reference point and sum, then the lanes share the dimensions and walk the
+// runs in ascending order.  Rows are the entries' single tokens, whose first record says how many runs there are, or (portions) all rows of
+// the entries that bring more.
+#define MG_WARPS 4
+constexpr int MG_EACH = (HD + 63) / 64;                              // pairs of dimensions a lane has
+template <bool WIDE>
+__global__ void __launch_bounds__(MG_WARPS * 32)
+attn_q8_merge_kernel(const float* __restrict__ scratch, const int* __restrict__ cu_q, bf16* __restrict__ out, int nH, int room, int n_rows,
+                     int least, int most) {
+    __shared__ float part_s[WIDE ? MG_WARPS : 1][HD + 2];
+    ng_pdl_trigger();
+    const int e = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int head = WIDE ? blockIdx.x : blockIdx.x * MG_WARPS + warp;
     const int q0 = cu_q[e], n = cu_q[e + 1] - q0;
     ng_pdl_wait();
-    if (n < least || n > most) return;
+    if (n < least || n > most || (!WIDE && head >= nH)) return;
     scratch = ng_after_wait(scratch);
-    const int d = threadIdx.x % HD, g = threadIdx.x / HD;
-    __shared__ float part[GROUPS][HD], part_l[GROUPS];
+    constexpr int STEP = WIDE ? MG_WARPS : 1;
     for (int r = q0 + blockIdx.z; r < min(q0 + n, n_rows); r += gridDim.z) {
-        const float* rec = scratch + ((size_t)r * nH + head) * n_splits * REC;
-        float m = -INFINITY;
-        for (int s = 0; s < n_splits; ++s) m = fmaxf(m, rec[(size_t)s * REC]);
-        float l = 0.f, acc = 0.f;
-#pragma unroll 4
-        for (int s = g; s < n_splits; s += GROUPS) {
-            const float ms = rec[(size_t)s * REC], ls = rec[(size_t)s * REC + 1];
-            const float f = ms == -INFINITY ? (m == -INFINITY ? 1.f : 0.f) : ex2(ms - m);
-            l = fmaf(ls, f, l);
-            acc = fmaf(ls == 0.f ? 0.f : rec[(size_t)s * REC + 4 + d], f, acc);       // (an empty run wrote no row)
+        const float* rec = scratch + ((size_t)r * nH + head) * room * REC;
+        // (the first 32 runs' are asked for before it is known how many there are)
+        const int s0 = lane * STEP + (WIDE ? warp : 0);
+        float m0 = s0 < room ? rec[(size_t)s0 * REC] : -INFINITY, l0 = s0 < room ? rec[(size_t)s0 * REC + 1] : 0.f;
+        int runs = room;
+        if (most == 1) {
+            runs = (int)rec[2];
+            if (runs <= 1) continue;
         }
-        if constexpr (GROUPS > 1) {
-            __syncthreads();
-            part[g][d] = acc;
-            if (d == 0) part_l[g] = l;
-            __syncthreads();
-            if (g == 0)
+        float m = -INFINITY, l = 0.f, acc[MG_EACH][2] = {};
+        for (int b = 0; b < runs; b += 32 * STEP) {
+            const int s1 = b + s0;
+            float ms = m0, ls = l0;
+            if (b > 0) {
+                ms = s1 < runs ? rec[(size_t)s1 * REC] : -INFINITY;
+                ls = s1 < runs ? rec[(size_t)s1 * REC + 1] : 0.f;
+            }
+            if (s1 >= runs) ms = -INFINITY, ls = 0.f;
+            const float mb = fmaxf(m, ng_warp_max(ms)), c = m == -INFINITY ? (mb == -INFINITY ? 1.f : 0.f) : ex2(m - mb);
+            const float f = ms == -INFINITY ? (mb == -INFINITY ? 1.f : 0.f) : ex2(ms - mb);          // (a run that met only NaN kept its sums)
+            m = mb;
+            l = fmaf(l, c, ng_warp_sum(ls * f));
 #pragma unroll
-                for (int k = 1; k < GROUPS; ++k) {
-                    l += part_l[k];
-                    acc += part[k][d];
+            for (int i = 0; i < MG_EACH; ++i) acc[i][0] *= c, acc[i][1] *= c;
+            const uint32_t some = __ballot_sync(0xffffffffu, ls != 0.f);                               // (an empty run wrote no row)
+            const int here = min(32, (runs - b - (WIDE ? warp : 0) + STEP - 1) / STEP);
+#pragma unroll 4
+            for (int k = 0; k < here; ++k) {
+                const float fk = __shfl_sync(0xffffffffu, f, k);
+                if (!(some >> k & 1)) continue;
+                const float* row = rec + (size_t)(b + k * STEP + (WIDE ? warp : 0)) * REC + 4;
+#pragma unroll
+                for (int i = 0; i < MG_EACH; ++i) {
+                    const int d = 2 * lane + 64 * i;
+                    if (HD % 64 != 0 && d >= HD) continue;
+                    const float2 x = *reinterpret_cast<const float2*>(row + d);
+                    acc[i][0] = fmaf(x.x, fk, acc[i][0]);
+                    acc[i][1] = fmaf(x.y, fk, acc[i][1]);
                 }
+            }
         }
-        if (g == 0) out[((size_t)r * nH + head) * HD + d] = __float2bfloat16_rn(l == 0.f ? 0.f : acc / l);
+        if constexpr (WIDE) {
+            __syncthreads();                                         // the row before has been written
+            if (lane == 0) part_s[warp][0] = m, part_s[warp][1] = l;
+#pragma unroll
+            for (int i = 0; i < MG_EACH; ++i) {
+                const int d = 2 * lane + 64 * i;
+                if (HD % 64 == 0 || d < HD) part_s[warp][2 + d] = acc[i][0], part_s[warp][3 + d] = acc[i][1];
+            }
+            __syncthreads();
+            if (warp > 0) continue;
+            float top = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < MG_WARPS; ++w) top = fmaxf(top, part_s[w][0]);
+            l = 0.f;
+#pragma unroll
+            for (int i = 0; i < MG_EACH; ++i) acc[i][0] = acc[i][1] = 0.f;
+#pragma unroll
+            for (int w = 0; w < MG_WARPS; ++w) {
+                const float f = part_s[w][0] == -INFINITY ? (top == -INFINITY ? 1.f : 0.f) : ex2(part_s[w][0] - top);
+                l = fmaf(part_s[w][1], f, l);
+#pragma unroll
+                for (int i = 0; i < MG_EACH; ++i) {
+                    const int d = 2 * lane + 64 * i;
+                    if (HD % 64 == 0 || d < HD) acc[i][0] = fmaf(part_s[w][2 + d], f, acc[i][0]), acc[i][1] = fmaf(part_s[w][3 + d], f, acc[i][1]);
+                }
+            }
+        }
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+        for (int i = 0; i < MG_EACH; ++i) {
+            const int d = 2 * lane + 64 * i;
+            if (HD % 64 == 0 || d < HD)
+                *reinterpret_cast<__nv_bfloat162*>(out + ((size_t)r * nH + head) * HD + d) = __floats2bfloat162_rn(acc[i][0] * inv, acc[i][1] * inv);
+        }
     }
 }
 
@@ -702,11 +905,11 @@ static int log2_exact(int n) {               // -1: not a power of two
 static int merge(const float* scratch, const int* cu_q, void* out, int nH, int n_splits, int n_rows, int n_entries, int least, int most,
                  int rows, cudaStream_t stream) {
     const int z = rows < 1 ? 1 : rows > 65535 ? 65535 : rows;
-    constexpr int G = 1024 / HD < 4 ? 1024 / HD : 4;
-    if (n_splits > 4)
-        NG_LAUNCH((attn_q8_merge_kernel<G>), dim3(nH, n_entries, z), G * HD, 0, stream, scratch, cu_q, (bf16*)out, nH, n_splits, n_rows, least, most);
+    if (n_splits > 8 && (long long)n_entries * nH * z < 1024)        // many runs of few rows
+        NG_LAUNCH((attn_q8_merge_kernel<true>), dim3(nH, n_entries, z), MG_WARPS * 32, 0, stream, scratch, cu_q, (bf16*)out, nH, n_splits, n_rows, least, most);
     else
-        NG_LAUNCH((attn_q8_merge_kernel<1>), dim3(nH, n_entries, z), HD, 0, stream, scratch, cu_q, (bf16*)out, nH, n_splits, n_rows, least, most);
+        NG_LAUNCH((attn_q8_merge_kernel<false>), dim3((nH + MG_WARPS - 1) / MG_WARPS, n_entries, z), MG_WARPS * 32, 0, stream, scratch, cu_q, (bf16*)out,
+                  nH, n_splits, n_rows, least, most);
     return ng_launch_status();
 }
 
@@ -720,7 +923,24 @@ static bool cache_of(Cache& c, const void* k_pages, const void* v_pages, const f
     c = Cache{(const unsigned char*)k_pages, (const unsigned char*)v_pages, ks, vs, table, table_stride, num_pages, nKV, log2_exact(page_size),
               log2_exact(block)};
     return c.ps_log2 >= 3 && c.bl_log2 >= 3 && c.bl_log2 <= c.ps_log2 && nKV > 0 && table_stride > 0 && num_pages > 0 &&
-           !(((uintptr_t)k_pages | (uintptr_t)v_pages) & 15);
+           ((long long)nKV * page_size * HD) <= 0x7fffffff && !(((uintptr_t)k_pages | (uintptr_t)v_pages) & 15);
+}
+
+// blocks of the kernel that the current device holds at once (with the most shared memory it may ask for)
+template <typename K>
+static int dc_slots(std::atomic<int>* known, K kernel) {
+    int device = 0, sms = 0, each = 0;
+    if (cudaGetDevice(&device) != cudaSuccess) return 0;
+    int n = known[device & 63].load(std::memory_order_relaxed);
+    if (n) return n;
+    cudaFuncAttributes attr;
+    if (cudaFuncGetAttributes(&attr, kernel) != cudaSuccess ||
+        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess ||
+        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&each, kernel, DC_THREADS, attr.maxDynamicSharedSizeBytes) != cudaSuccess)
+        return 0;
+    n = sms * (each > 0 ? each : 1);
+    known[device & 63].store(n, std::memory_order_relaxed);
+    return n;
 }
 
 NG_EXPORT int ng_attn_decode_q8(const void* q, const void* k_pages, const void* v_pages, const float* k_scales, const float* v_scales,
@@ -731,27 +951,34 @@ NG_EXPORT int ng_attn_decode_q8(const void* q, const void* k_pages, const void* 
     DcArgs a;
     if (hd != HD || nH <= 0 || !cache_of(a.c, k_pages, v_pages, k_scales, v_scales, table, table_stride, nKV, page_size, block, num_pages) ||
         nH % nKV || n_splits < 1 || n_splits > 65535 || n_entries > 65535 || (n_splits > 1 && (!scratch || ((uintptr_t)scratch & 15))) ||
-        max_ctx < 0 || window < 0 || ((uintptr_t)q & 7) || (kind != NG_Q8_E4M3 && kind != NG_Q8_INT8))
+        max_ctx < 0 || window < 0 || ((uintptr_t)q & 7) || ((uintptr_t)out & 3) || (kind != NG_Q8_E4M3 && kind != NG_Q8_INT8))
         return NG_BAD_SIZE;
     const int G = nH / nKV;
-    // a run: whole turns of the four warps; a window's first group may begin up to a group before it
-    const long long span = (long long)(window > 0 && window < max_ctx ? window : max_ctx) + GROUP;
-    const long long turn = DC_WARPS * GROUP, per = ((span + n_splits - 1) / n_splits + turn - 1) / turn * turn;
     a.q = (const bf16*)q; a.cu_q = cu_q; a.ctx_before = ctx_before; a.out = (bf16*)out; a.scratch = scratch; a.slopes = slopes;
-    a.n_rows = n_rows; a.nH = nH; a.chunks = (G + 15) / 16; a.window = window; a.n_splits = n_splits; a.scale = scale;
-    if (per * n_splits > 0x7fffffffll) return NG_BAD_SIZE;
-    a.keys_per_split = (int)per;
-    if ((long long)nKV * a.chunks > 0x7fffffffll) return NG_BAD_SIZE;
-    const dim3 grid(nKV * a.chunks, n_entries, n_splits);
-    const int smem = DC_WARPS * (G < 16 ? G : 16) * REC * (int)sizeof(float);
-#define DC_GO(KIND)                                                                                                                   \
+    a.n_rows = n_rows; a.n_entries = n_entries; a.nH = nH; a.window = window; a.n_splits = n_splits; a.scale = scale;
+    const int nt = G > 8 ? DC_NT_MAX : 1;
+    a.chunks = (G + 8 * nt - 1) / (8 * nt);
+    const int segments = nKV * a.chunks;
+    // blocks, and all turns rounded up to whole shares, are counted in 31 bits
+    if ((long long)nKV * a.chunks * n_entries > 0x7fffffff || n_entries * (((long long)table_stride * page_size / TURN + 2) * 2) > 0x7fffffff)
+        return NG_BAD_SIZE;
+#define DC_GO(KIND, NT, GRAN)                                                                                                         \
     do {                                                                                                                              \
         static std::atomic<unsigned long long> once{0};                                                                               \
-        if (!ng_allow_smem(once, attn_decode_q8_kernel<KIND>, DC_WARPS * 16 * REC * (int)sizeof(float))) return NG_LAUNCH_FAILED;     \
-        NG_LAUNCH((attn_decode_q8_kernel<KIND>), grid, DC_THREADS, smem, stream, a);                                                  \
+        static std::atomic<int> slots[64];                                                                                            \
+        constexpr auto kernel = attn_decode_q8_kernel<KIND, NT, GRAN>;                                                                \
+        if (!ng_allow_smem(once, kernel, DC_WARPS * 8 * NT * REC * (int)sizeof(float))) return NG_LAUNCH_FAILED;                      \
+        const int smem = DC_WARPS * (G < 8 * NT ? G : 8 * NT) * REC * (int)sizeof(float);                                             \
+        const int room = n_splits > 1 ? dc_slots(slots, kernel) : 1;                                                                  \
+        if (room <= 0) return NG_LAUNCH_FAILED;                                                                                       \
+        const int teams = room / segments > 1 ? room / segments : 1;                                                                  \
+        NG_LAUNCH((kernel), dim3(n_splits > 1 ? teams * segments : n_entries * segments), DC_THREADS, smem, stream, a);                                  \
     } while (0)
-    if (kind == NG_Q8_E4M3) DC_GO(NG_Q8_E4M3);
-    else DC_GO(NG_Q8_INT8);
+#define DC_KINDS(NT, GRAN) do { if (kind == NG_Q8_E4M3) DC_GO(NG_Q8_E4M3, NT, GRAN); else DC_GO(NG_Q8_INT8, NT, GRAN); } while (0)
+    if (nt == 1 && block >= 16) DC_KINDS(1, 16);
+    else if (nt == 1) DC_KINDS(1, 8);
+    else if (block >= 16) DC_KINDS(DC_NT_MAX, 16);
+    else DC_KINDS(DC_NT_MAX, 8);
     if (n_splits > 1) return merge(scratch, cu_q, out, nH, n_splits, n_rows, n_entries, 1, 1, 1, stream);
     return ng_launch_status();
 }

@@ -541,11 +541,16 @@ def _sm_count(device) -> int:
 
 
 def attn_decode_q8_splits(n_single: int, n_heads: int, n_kv_heads: int, head_dim: int, max_ctx: int, window: Optional[int], device) -> int:
-    """Runs ``attn_decode_q8`` should cut the keys into."""
-    span = min(window, max_ctx) if window else max_ctx
-    pairs = max(1, n_single * n_kv_heads * -(-n_heads // n_kv_heads // 16))
-    want = max(-(-4 * _sm_count(device) // pairs), -(-span // 4096))
-    return max(1, min(want, span // 256))
+    """Runs ``attn_decode_q8`` may cut an entry's keys into."""
+    group = -(-n_heads // n_kv_heads)
+    segments = n_kv_heads * -(-group // (16 if group > 8 and head_dim <= 64 else 8))      # of an entry
+    turns = -(-(min(window, max_ctx) if window else max_ctx) // (128 if head_dim <= 128 else 64))
+    if turns <= 4:
+        return 1
+    slots = (3 if head_dim <= 64 and group <= 8 else 2) * _sm_count(device)
+    even = -(-turns // -(-n_single * segments * turns // slots)) + 1             # all entries as long as the longest
+    alone = -(-turns // -(-segments * turns // slots)) + 1                       # the longest alone
+    return min(alone, max(2 * even, 16))
 
 
 def attn_prefill_q8_splits(q_lens, n_heads: int, n_kv_heads: int, head_dim: int, max_ctx: int, window: Optional[int], device) -> int:
