@@ -9,32 +9,12 @@
 // w_j = 2^(z_j - m) are what meets the codes d_j, in float16 (half a step 2^-12 of the weight, smallest step 2^-24 of the
 // largest), and the denominator is sum_j w_j / t_j in 32 bits: t_j is a power of two, both forms are exact.  So a block
 // whose values are small has small weights, not small values, and the sum over the codes never leaves float16's range.
-#include "ng_q8.cuh"
-
-#ifndef NG_HEAD_DIM
-#error "compile with -DNG_HEAD_DIM=<head size>"
-#endif
-#define HD NG_HEAD_DIM
-static_assert(HD % 16 == 0 && HD >= 16 && HD <= 256, "head size must be a multiple of 16 in [16, 256]");
-#define LOG2E 1.4426950408889634f
-#define REC (HD + 4)            // floats of a run's record: reference point, sum, two unused (the row starts on 16 bytes), row in codes
-
-typedef __nv_bfloat16 bf16;
+#include "ng_q8_attention.cuh"
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
-    uint32_t d;
-    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
-    return d;
-}
-__device__ __forceinline__ float ex2(float x) {          // 2 ulp; -inf -> 0
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
 }
 // BYTES of codes from a page; no line of the first-level cache is taken (they are read once).  Not moved above the wait.
 template <int BYTES>
@@ -48,17 +28,6 @@ __device__ __forceinline__ void ld_codes(uint32_t* w, const unsigned char* p) {
     else
         asm volatile("{\n\t.reg .u16 h;\n\tld.global.L1::no_allocate.u16 h, [%1];\n\tcvt.u32.u16 %0, h;\n\t}" : "=r"(w[0]) : "l"(p) : "memory");
 }
-
-// The power of two that a row of q is divided by (its largest value becomes 1 to 2): exponent of the row's largest finite value.
-__device__ __forceinline__ int q_exponent(float top) { return min(max((int)(__float_as_uint(top) >> 23) - 127, -100), 127); }
-__device__ __forceinline__ float pow2_any(int e) { return q8_pow2(min(max(e, -126), 127)); }
-
-struct Cache {
-    const unsigned char *k, *v;          // [pages, nKV, page, HD]
-    const float *ks, *vs;                // [pages, nKV, page / block]
-    const int* table;
-    int table_stride, num_pages, nKV, ps_log2, bl_log2;
-};
 
 // ===================================================================================== single tokens
 // A segment is an entry's keys for up to 8 NT query heads of one KV head.  The block's four warps take groups of GROUP keys in turn, each on
@@ -230,7 +199,7 @@ __device__ __forceinline__ void dc_compute(DcState<NT>& st, DcGroup<GRAN>& r, co
 #pragma unroll
                 for (int o = 4; o <= 16; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
                 const bool first = !(st.seen >> n & 1);
-                const float by = x == -INFINITY ? 0.f : first ? x : fmaxf(x, 0.f), c = ex2(-by);
+                const float by = x == -INFINITY ? 0.f : first ? x : fmaxf(x, 0.f), c = q8_ex2(-by);
                 any = any && x != -INFINITY;
                 st.m[n][j] += by;
                 st.l[n][j] *= first ? 1.f : c;
@@ -250,7 +219,7 @@ __device__ __forceinline__ void dc_compute(DcState<NT>& st, DcGroup<GRAN>& r, co
         for (int s = 0; s < SUB; ++s) {
             float p[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) p[j] = ex2(sc[n][s][j]);
+            for (int j = 0; j < 4; ++j) p[j] = q8_ex2(sc[n][s][j]);
             if constexpr (UNITS == 1) {
                 const float inv = q8_recip(r.vs[s][0]);
                 st.l[n][0] = fmaf(p[0] + p[2], inv, st.l[n][0]);
@@ -477,7 +446,7 @@ __device__ __forceinline__ void dc_piece(const DcArgs& a, float* red_s, int e, i
 #pragma unroll
         for (int w = 0; w < DC_WARPS; ++w) {
             const float* rec = red_s + (size_t)(w * heads + h) * REC;
-            const float c = rec[0] == -INFINITY ? (m == -INFINITY ? 1.f : 0.f) : ex2(rec[0] - m);       // (a warp that met only NaN kept its sums)
+            const float c = rec[0] == -INFINITY ? (m == -INFINITY ? 1.f : 0.f) : q8_ex2(rec[0] - m);       // (a warp that met only NaN kept its sums)
             l = fmaf(rec[1], c, l);
             acc = fmaf(rec[4 + d], c, acc);
         }
@@ -519,104 +488,6 @@ attn_decode_q8_kernel(const DcArgs a) {
         at = max(at, end);
         sh.before = end;
         ++sh.e;
-    }
-}
-
-// out[row, head] = sum_s o_s 2^(m_s - m) / sum_s l_s 2^(m_s - m) over the runs s.  A warp has a (row, head) (WIDE: all four warps of a block, every
-// fourth run each, joined in order): lane s looks after run s's reference point and sum, then the lanes share the dimensions and walk the
-// runs in ascending order.  Rows are the entries' single tokens, whose first record says how many runs there are, or (portions) all rows of
-// the entries that bring more.
-#define MG_WARPS 4
-constexpr int MG_EACH = (HD + 63) / 64;                              // pairs of dimensions a lane has
-template <bool WIDE>
-__global__ void __launch_bounds__(MG_WARPS * 32)
-attn_q8_merge_kernel(const float* __restrict__ scratch, const int* __restrict__ cu_q, bf16* __restrict__ out, int nH, int room, int n_rows,
-                     int least, int most) {
-    __shared__ float part_s[WIDE ? MG_WARPS : 1][HD + 2];
-    ng_pdl_trigger();
-    const int e = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int head = WIDE ? blockIdx.x : blockIdx.x * MG_WARPS + warp;
-    const int q0 = cu_q[e], n = cu_q[e + 1] - q0;
-    ng_pdl_wait();
-    if (n < least || n > most || (!WIDE && head >= nH)) return;
-    scratch = ng_after_wait(scratch);
-    constexpr int STEP = WIDE ? MG_WARPS : 1;
-    for (int r = q0 + blockIdx.z; r < min(q0 + n, n_rows); r += gridDim.z) {
-        const float* rec = scratch + ((size_t)r * nH + head) * room * REC;
-        // (the first 32 runs' are asked for before it is known how many there are)
-        const int s0 = lane * STEP + (WIDE ? warp : 0);
-        float m0 = s0 < room ? rec[(size_t)s0 * REC] : -INFINITY, l0 = s0 < room ? rec[(size_t)s0 * REC + 1] : 0.f;
-        int runs = room;
-        if (most == 1) {
-            runs = (int)rec[2];
-            if (runs <= 1) continue;
-        }
-        float m = -INFINITY, l = 0.f, acc[MG_EACH][2] = {};
-        for (int b = 0; b < runs; b += 32 * STEP) {
-            const int s1 = b + s0;
-            float ms = m0, ls = l0;
-            if (b > 0) {
-                ms = s1 < runs ? rec[(size_t)s1 * REC] : -INFINITY;
-                ls = s1 < runs ? rec[(size_t)s1 * REC + 1] : 0.f;
-            }
-            if (s1 >= runs) ms = -INFINITY, ls = 0.f;
-            const float mb = fmaxf(m, ng_warp_max(ms)), c = m == -INFINITY ? (mb == -INFINITY ? 1.f : 0.f) : ex2(m - mb);
-            const float f = ms == -INFINITY ? (mb == -INFINITY ? 1.f : 0.f) : ex2(ms - mb);          // (a run that met only NaN kept its sums)
-            m = mb;
-            l = fmaf(l, c, ng_warp_sum(ls * f));
-#pragma unroll
-            for (int i = 0; i < MG_EACH; ++i) acc[i][0] *= c, acc[i][1] *= c;
-            const uint32_t some = __ballot_sync(0xffffffffu, ls != 0.f);                               // (an empty run wrote no row)
-            const int here = min(32, (runs - b - (WIDE ? warp : 0) + STEP - 1) / STEP);
-#pragma unroll 4
-            for (int k = 0; k < here; ++k) {
-                const float fk = __shfl_sync(0xffffffffu, f, k);
-                if (!(some >> k & 1)) continue;
-                const float* row = rec + (size_t)(b + k * STEP + (WIDE ? warp : 0)) * REC + 4;
-#pragma unroll
-                for (int i = 0; i < MG_EACH; ++i) {
-                    const int d = 2 * lane + 64 * i;
-                    if (HD % 64 != 0 && d >= HD) continue;
-                    const float2 x = *reinterpret_cast<const float2*>(row + d);
-                    acc[i][0] = fmaf(x.x, fk, acc[i][0]);
-                    acc[i][1] = fmaf(x.y, fk, acc[i][1]);
-                }
-            }
-        }
-        if constexpr (WIDE) {
-            __syncthreads();                                         // the row before has been written
-            if (lane == 0) part_s[warp][0] = m, part_s[warp][1] = l;
-#pragma unroll
-            for (int i = 0; i < MG_EACH; ++i) {
-                const int d = 2 * lane + 64 * i;
-                if (HD % 64 == 0 || d < HD) part_s[warp][2 + d] = acc[i][0], part_s[warp][3 + d] = acc[i][1];
-            }
-            __syncthreads();
-            if (warp > 0) continue;
-            float top = -INFINITY;
-#pragma unroll
-            for (int w = 0; w < MG_WARPS; ++w) top = fmaxf(top, part_s[w][0]);
-            l = 0.f;
-#pragma unroll
-            for (int i = 0; i < MG_EACH; ++i) acc[i][0] = acc[i][1] = 0.f;
-#pragma unroll
-            for (int w = 0; w < MG_WARPS; ++w) {
-                const float f = part_s[w][0] == -INFINITY ? (top == -INFINITY ? 1.f : 0.f) : ex2(part_s[w][0] - top);
-                l = fmaf(part_s[w][1], f, l);
-#pragma unroll
-                for (int i = 0; i < MG_EACH; ++i) {
-                    const int d = 2 * lane + 64 * i;
-                    if (HD % 64 == 0 || d < HD) acc[i][0] = fmaf(part_s[w][2 + d], f, acc[i][0]), acc[i][1] = fmaf(part_s[w][3 + d], f, acc[i][1]);
-                }
-            }
-        }
-        const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-        for (int i = 0; i < MG_EACH; ++i) {
-            const int d = 2 * lane + 64 * i;
-            if (HD % 64 == 0 || d < HD)
-                *reinterpret_cast<__nv_bfloat162*>(out + ((size_t)r * nH + head) * HD + d) = __floats2bfloat162_rn(acc[i][0] * inv, acc[i][1] * inv);
-        }
     }
 }
 
@@ -837,7 +708,7 @@ attn_prefill_q8_kernel(const PfArgs a) {
                 mx_hi = fmaxf(mx_hi, __shfl_xor_sync(0xffffffffu, mx_hi, x));
             }
             const float n_lo = fmaxf(m_lo, mx_lo), n_hi = fmaxf(m_hi, mx_hi);
-            const float c_lo = n_lo == -INFINITY ? 1.f : ex2(m_lo - n_lo), c_hi = n_hi == -INFINITY ? 1.f : ex2(m_hi - n_hi);
+            const float c_lo = n_lo == -INFINITY ? 1.f : q8_ex2(m_lo - n_lo), c_hi = n_hi == -INFINITY ? 1.f : q8_ex2(m_hi - n_hi);
             m_lo = n_lo;
             m_hi = n_hi;
             l_lo *= c_lo;
@@ -849,8 +720,8 @@ attn_prefill_q8_kernel(const PfArgs a) {
         uint32_t p[PF_KEYS / 16][4];
 #pragma unroll
         for (int nt = 0; nt < PF_KEYS / 8; ++nt) {
-            const float p0 = ex2(sc[nt][0] - ref_lo), p1 = ex2(sc[nt][1] - ref_lo);
-            const float p2 = ex2(sc[nt][2] - ref_hi), p3 = ex2(sc[nt][3] - ref_hi);
+            const float p0 = q8_ex2(sc[nt][0] - ref_lo), p1 = q8_ex2(sc[nt][1] - ref_lo);
+            const float p2 = q8_ex2(sc[nt][2] - ref_hi), p3 = q8_ex2(sc[nt][3] - ref_hi);
             const float inv = sm->vi[s][nt];
             l_lo = fmaf(p0 + p1, inv, l_lo);
             l_hi = fmaf(p2 + p3, inv, l_hi);
@@ -896,34 +767,9 @@ attn_prefill_q8_kernel(const PfArgs a) {
 }
 
 // ===================================================================================== host
-static int log2_exact(int n) {               // -1: not a power of two
-    if (n <= 0 || (n & (n - 1))) return -1;
-    int l = 0;
-    while ((1 << l) < n) ++l;
-    return l;
-}
-static int merge(const float* scratch, const int* cu_q, void* out, int nH, int n_splits, int n_rows, int n_entries, int least, int most,
-                 int rows, cudaStream_t stream) {
-    const int z = rows < 1 ? 1 : rows > 65535 ? 65535 : rows;
-    if (n_splits > 8 && (long long)n_entries * nH * z < 1024)        // many runs of few rows
-        NG_LAUNCH((attn_q8_merge_kernel<true>), dim3(nH, n_entries, z), MG_WARPS * 32, 0, stream, scratch, cu_q, (bf16*)out, nH, n_splits, n_rows, least, most);
-    else
-        NG_LAUNCH((attn_q8_merge_kernel<false>), dim3((nH + MG_WARPS - 1) / MG_WARPS, n_entries, z), MG_WARPS * 32, 0, stream, scratch, cu_q, (bf16*)out,
-                  nH, n_splits, n_rows, least, most);
-    return ng_launch_status();
-}
-
 // scratch: n_rows * nH * n_splits * REC floats, 16-byte aligned (unused when n_splits == 1)
 NG_EXPORT long long ng_attn_q8_scratch_floats(int n_rows, int nH, int n_splits) {
     return n_splits > 1 ? (long long)n_rows * nH * n_splits * REC : 0;
-}
-
-static bool cache_of(Cache& c, const void* k_pages, const void* v_pages, const float* ks, const float* vs, const int* table, int table_stride,
-                     int nKV, int page_size, int block, int num_pages) {
-    c = Cache{(const unsigned char*)k_pages, (const unsigned char*)v_pages, ks, vs, table, table_stride, num_pages, nKV, log2_exact(page_size),
-              log2_exact(block)};
-    return c.ps_log2 >= 3 && c.bl_log2 >= 3 && c.bl_log2 <= c.ps_log2 && nKV > 0 && table_stride > 0 && num_pages > 0 &&
-           ((long long)nKV * page_size * HD) <= 0x7fffffff && !(((uintptr_t)k_pages | (uintptr_t)v_pages) & 15);
 }
 
 // blocks of the kernel that the current device holds at once (with the most shared memory it may ask for)
@@ -979,7 +825,7 @@ NG_EXPORT int ng_attn_decode_q8(const void* q, const void* k_pages, const void* 
     else if (nt == 1) DC_KINDS(1, 8);
     else if (block >= 16) DC_KINDS(DC_NT_MAX, 16);
     else DC_KINDS(DC_NT_MAX, 8);
-    if (n_splits > 1) return merge(scratch, cu_q, out, nH, n_splits, n_rows, n_entries, 1, 1, 1, stream);
+    if (n_splits > 1) return q8_merge(scratch, cu_q, out, nH, n_splits, n_rows, n_entries, 1, 1, 1, stream);
     return ng_launch_status();
 }
 
@@ -1006,6 +852,6 @@ NG_EXPORT int ng_attn_prefill_q8(const void* q, const void* k_pages, const void*
     } while (0)
     if (kind == NG_Q8_E4M3) PF_GO(NG_Q8_E4M3);
     else PF_GO(NG_Q8_INT8);
-    if (n_splits > 1) return merge(scratch, cu_q, out, nH, n_splits, n_rows, n_entries, skip_single ? 2 : 1, 0x7fffffff, max_q, stream);
+    if (n_splits > 1) return q8_merge(scratch, cu_q, out, nH, n_splits, n_rows, n_entries, skip_single ? 2 : 1, 0x7fffffff, max_q, stream);
     return ng_launch_status();
 }

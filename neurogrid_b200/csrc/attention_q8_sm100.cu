@@ -1,0 +1,441 @@
+// Flash attention of prompt portions over a paged cache in 8 bits on the Blackwell tensor cores (head sizes 64 and 128, compiled with
+// -DNG_HEAD_DIM).  The arithmetic is that of attention_q8.cu: codes as float16 operands, the keys' scales on the 32-bit scores,
+// the values' scales in the exponents, the sum divided by them.
+//
+// A block owns 128 rows of one (entry, KV head); a row is a (token, query head of the KV head), heads fastest, so that the heads which share
+// keys share the tiles that are fetched and turned into float16 for them.  Eight warps (of nine, a scheduler would have five of two
+// blocks' and a thread 96 registers; a softmax thread takes 128):
+//   warps 0-3  softmax: thread r owns row r = TMEM lane r; before the first tile it brings its row of q into shared memory
+//   warps 4-6  keys and values: codes of the next 64-key tile from the pages into registers while this one is stored, as float16, in
+//              the swizzled layout that the MMA reads (K row by row, V as it lies: [key][dim], MN-major)
+//   warp 7     MMA issuer: S = Q K^T and O += P V with tcgen05.mma, accumulators in TMEM, P taken from TMEM over S
+// S is double-buffered in TMEM: the next tile's scores are computed while this tile's softmax runs.  The tensor pipe runs the
+// issuer's MMAs in order and a commit covers all before it, so "S of tile j + 2 is complete" also says that P V of tile j has read its P.
+//
+// Keys that no row of the block sees, and keys whose page is not there, are stored as zeros (their codes may be NaN).  Every mbarrier wait
+// is bounded; a waiter that gives up sets a status bit and the block runs to its end.
+//
+// Bound by the exponentials and the instructions around them (a score costs the thread of its row about three).
+#include "sm100_common.cuh"
+#include "ng_q8_attention.cuh"
+
+static_assert(HD == 64 || HD == 128, "head sizes 64 and 128");
+#define BQ 128                       // rows of a block
+#define BK 64                        // keys of a tile
+#define NB (HD / 64)                 // 64-wide blocks of a head
+#define KV_STAGES (HD == 64 ? 3 : 2)
+#define NG_STATUS_ATTN_TIMEOUT 16
+#define Q8P_THREADS 256
+#define KV_WARPS 3
+#define MIN_RUN 4                    // a run of keys is at least this many tiles
+static_assert(BQ == BLOCK_W, "a block's rows are the 128 rows of the MMA");
+
+__device__ __forceinline__ float fmax3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+// two float32 values in one 64-bit register, and packed arithmetic on them (each half rounded as the scalar instruction rounds)
+typedef unsigned long long u64;
+__device__ __forceinline__ u64 pack2(float a, float b) {
+    u64 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void unpack2(u64 v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ u64 ffma2(u64 a, u64 b, u64 c) {
+    u64 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ u64 fadd2(u64 a, u64 b) {
+    u64 d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+
+struct Smem {
+    uint16_t q[NB][BQ * 64];                     // K-major, 128-byte swizzle, a block for each 64 of the head
+    uint16_t k[KV_STAGES][NB][BK * 64];
+    uint16_t v[KV_STAGES][NB][BK * 64];
+    float ks[KV_STAGES][8], vl[KV_STAGES][8], vi[KV_STAGES][8];       // of each 8 keys: K's scale, V's log2 and reciprocal
+    uint64_t q_full, kv_full[KV_STAGES], kv_empty[KV_STAGES], s_full[2], p_full[2], o_ready[2];
+    uint32_t tmem_base;
+};
+
+struct Params {
+    Cache c;
+    const bf16* q;
+    bf16* out;
+    const int *cu_q, *ctx_before;
+    int* status;
+    int n_rows, nH, window, skip_single, n_splits;
+    float scale;
+    const float* slopes;
+    float* scratch;
+};
+
+// half of a tile row's swizzled bytes: 16-byte chunk c (8 float16) of row r
+__device__ __forceinline__ int sw128(int r, int c) { return (r >> 3) * 512 + (r & 7) * 64 + ((c ^ (r & 7)) << 3); }
+// kind::f16, float16 operands: as make_idesc without its bfloat16 bits
+__host__ __device__ constexpr uint32_t idesc_f16(int n, int b_mn) { return make_idesc(n, b_mn) & ~((1u << 7) | (1u << 10)); }
+
+template <int KIND>
+__global__ void __launch_bounds__(Q8P_THREADS, 2)
+attn_prefill_q8_sm100_kernel(const Params p) {
+    extern __shared__ unsigned char smem_raw[];
+    Smem* sm = reinterpret_cast<Smem*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    ng_pdl_trigger();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    uint32_t elected;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(elected));
+    const bool leader = elected != 0;
+    // heads run fastest and the row tiles from the last one down: the blocks with the most keys start first
+    const int e = blockIdx.z / p.n_splits, split = blockIdx.z - e * p.n_splits, kvh = blockIdx.x;
+    const int q0 = p.cu_q[e], q1 = p.cu_q[e + 1], qlen = min(q1, p.n_rows) - q0, ctx = p.ctx_before[e];
+    const int G = p.nH / p.c.nKV;
+    const int r0 = (gridDim.y - 1 - blockIdx.y) * BQ;
+    if (q0 < 0 || ctx < 0 || r0 >= qlen * G || (p.skip_single && q1 - q0 == 1)) {
+        ng_pdl_wait();                                         // (a launch none of whose blocks waited would end before the one before it)
+        return;
+    }
+    const int rows_here = min(BQ, qlen * G - r0);
+    const int pos_first = ctx + r0 / G, pos_last = ctx + (r0 + rows_here - 1) / G;
+    const int key_lo = p.window > 0 ? max(0, pos_first - p.window + 1) : 0, kv_end = pos_last + 1;
+    int tile0 = key_lo / BK, tile1 = pos_last / BK;            // inclusive
+    if (p.n_splits > 1) {
+        const int per = max(MIN_RUN, (tile1 - tile0 + p.n_splits) / p.n_splits);
+        tile0 += split * per;
+        tile1 = min(tile1, tile0 + per - 1);
+    }
+    const int n_tiles = tile1 - tile0 + 1;
+    if (n_tiles <= 0) {                                        // an empty run: records that the merge passes over
+        ng_pdl_wait();
+        if (threadIdx.x < rows_here) {
+            const int token = (r0 + threadIdx.x) / G, head = kvh * G + (r0 + threadIdx.x) - token * G;
+            float* rec = p.scratch + (((size_t)(q0 + token) * p.nH + head) * p.n_splits + split) * REC;
+            rec[0] = -INFINITY;
+            rec[1] = 0.f;
+        }
+        return;
+    }
+    if (threadIdx.x == 0) {
+        mbar_init(&sm->q_full, 4);
+        for (int s = 0; s < KV_STAGES; ++s) { mbar_init(&sm->kv_full[s], KV_WARPS); mbar_init(&sm->kv_empty[s], 1); }
+        for (int i = 0; i < 2; ++i) { mbar_init(&sm->s_full[i], 1); mbar_init(&sm->p_full[i], 4); mbar_init(&sm->o_ready[i], 1); }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 7) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 256;" :: "r"(smem_u32(&sm->tmem_base)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    ng_pdl_wait();                                             // q and the pages are this step's data
+    tcgen05_fence_before();
+    __syncthreads();
+    tcgen05_fence_after();
+    const uint32_t tmem = sm->tmem_base, tm_s0 = tmem, tm_s1 = tmem + BK, tm_o = tmem + 2 * BK;
+    bool ok = true;
+
+    if (warp >= 4 && warp < 4 + KV_WARPS) {
+        // ------------------------------------------------------------------ keys and values
+        constexpr int PER_KEY = HD / 16, PIECES = BK * PER_KEY, LOADERS = 32 * KV_WARPS, EACH = (PIECES + LOADERS - 1) / LOADERS;
+        // 16-byte pieces of a key, of a tile, and of a thread (of K; V has as many)
+        const int tid = threadIdx.x - 128, mask = (1 << p.c.ps_log2) - 1;
+        const int* trow = p.c.table + (size_t)e * p.c.table_stride;
+        const unsigned char *k_pages = ng_after_wait(p.c.k), *v_pages = ng_after_wait(p.c.v);
+        uint32_t k[EACH][4], v[EACH][4];
+        float ks = 1.f, vs = 1.f;
+        auto page_of = [&](int key, int lo) {
+            int page = -1;
+            if (key >= lo && key < kv_end && (key >> p.c.ps_log2) < p.c.table_stride) page = trow[key >> p.c.ps_log2];
+            return page >= 0 && page < p.c.num_pages ? page : -1;
+        };
+        auto load = [&](int tile) {
+#pragma unroll
+            for (int n = 0; n < EACH; ++n) {
+                const int i = tid + LOADERS * n, key = tile * BK + i / PER_KEY, page = i < PIECES ? page_of(key, key_lo) : -1;
+                if (page < 0) {
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) k[n][x] = v[n][x] = 0u;
+                } else {
+                    const size_t at = ((((size_t)page * p.c.nKV + kvh) << p.c.ps_log2) + (key & mask)) * HD + (i % PER_KEY) * 16;
+                    const uint4 a = *reinterpret_cast<const uint4*>(k_pages + at), b = *reinterpret_cast<const uint4*>(v_pages + at);
+                    k[n][0] = a.x; k[n][1] = a.y; k[n][2] = a.z; k[n][3] = a.w;
+                    v[n][0] = b.x; v[n][1] = b.y; v[n][2] = b.z; v[n][3] = b.w;
+                }
+            }
+            if (tid < 8) {
+                const int key = tile * BK + 8 * tid, page = page_of(key, key_lo - 7);
+                ks = vs = 1.f;
+                if (page >= 0) {
+                    const size_t sc = (((size_t)page * p.c.nKV + kvh) << (p.c.ps_log2 - p.c.bl_log2)) + ((key & mask) >> p.c.bl_log2);
+                    ks = ng_after_wait(p.c.ks)[sc];
+                    vs = ng_after_wait(p.c.vs)[sc];
+                }
+            }
+        };
+        auto put = [](uint16_t* tile, int row, int c, const uint32_t (&w)[4]) {          // 16 codes: chunks c and c + 1 of the row
+            uint32_t h[8];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) q8_to_half<KIND>(w[x], h[2 * x], h[2 * x + 1]);
+            *reinterpret_cast<uint4*>(tile + sw128(row, c)) = make_uint4(h[0], h[1], h[2], h[3]);
+            *reinterpret_cast<uint4*>(tile + sw128(row, c + 1)) = make_uint4(h[4], h[5], h[6], h[7]);
+        };
+        load(tile0);
+        for (int j = 0; j < n_tiles && ok; ++j) {
+            const int s = j % KV_STAGES;
+            ok = __all_sync(0xffffffffu, mbar_wait(&sm->kv_empty[s], ((j / KV_STAGES) & 1) ^ 1));
+            if (!ok) break;
+#pragma unroll
+            for (int n = 0; n < EACH; ++n) {
+                const int i = tid + LOADERS * n, row = i / PER_KEY, c = i % PER_KEY * 2;
+                if (i >= PIECES) break;
+                put(sm->k[s][c / 8], row, c % 8, k[n]);
+                put(sm->v[s][c / 8], row, c % 8, v[n]);
+            }
+            if (tid < 8) {
+                sm->ks[s][tid] = ks;
+                sm->vl[s][tid] = q8_log2(vs);
+                sm->vi[s][tid] = q8_recip(vs);
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sm->kv_full[s]);
+            if (j + 1 < n_tiles) load(tile0 + j + 1);
+        }
+        if (!ok && lane == 0) atomicOr(p.status, NG_STATUS_ATTN_TIMEOUT);
+    } else if (warp == 7) {
+        // ------------------------------------------------------------------ MMA issuer: all lanes run the loop, one issues
+        constexpr uint32_t idesc_s = idesc_f16(BK, 0), idesc_o = idesc_f16(64, 1);
+        ok = __all_sync(0xffffffffu, mbar_wait(&sm->q_full, 0));
+        auto issue_s = [&](int j) {                            // S_j = Q K_j^T into buffer j & 1
+            const int s = j % KV_STAGES;
+            if (!__all_sync(0xffffffffu, mbar_wait(&sm->kv_full[s], (j / KV_STAGES) & 1))) { ok = false; return; }
+            tcgen05_fence_after();
+            if (leader) {
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    const uint64_t dq = make_desc_sw128(sm->q[b]), dk = make_desc_sw128(sm->k[s][b]);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        tcgen05_mma_f16((j & 1) ? tm_s1 : tm_s0, dq + (uint64_t)(2 * k), dk + (uint64_t)(2 * k), idesc_s, b > 0 || k > 0);
+                }
+                tcgen05_commit(&sm->s_full[j & 1]);
+            }
+            __syncwarp();
+        };
+        if (ok) issue_s(0);
+        if (ok && n_tiles > 1) issue_s(1);
+        for (int j = 0; j < n_tiles && ok; ++j) {
+            ok = __all_sync(0xffffffffu, mbar_wait(&sm->p_full[j & 1], (j >> 1) & 1));          // P_j in tensor memory, O rescaled
+            if (!ok) break;
+            tcgen05_fence_after();
+            const int s = j % KV_STAGES;
+            const uint32_t tp = (j & 1) ? tm_s1 : tm_s0;
+            if (leader) {
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    const uint64_t dv = make_desc_sw128_mn(sm->v[s][b]);
+#pragma unroll
+                    for (int k = 0; k < BK / 16; ++k)          // 16 keys an MMA: 8 columns of P, 2,048 bytes of V
+                        tcgen05_mma_f16_ts(tm_o + 64 * b, tp + 8 * k, dv + (uint64_t)(128 * k), idesc_o, j > 0 || k > 0);
+                }
+                tcgen05_commit(&sm->kv_empty[s]);              // K_j and V_j may be overwritten
+                tcgen05_commit(&sm->o_ready[j & 1]);           // O holds tiles 0..j
+            }
+            __syncwarp();
+            if (j + 2 < n_tiles) issue_s(j + 2);
+        }
+        if (!ok && leader) atomicOr(p.status, NG_STATUS_ATTN_TIMEOUT);
+    } else {
+        // ------------------------------------------------------------------ softmax: thread = row
+        const int r = threadIdx.x, rr = r0 + min(r, rows_here - 1);        // rows past the last mirror it
+        const int token = rr / G, head = kvh * G + rr - token * G, pos = ctx + token;
+        float f;
+        {
+            // the row of q, divided by a power of two, as float16
+            const bf16* q = ng_after_wait(p.q) + ((size_t)(q0 + token) * p.nH + head) * HD;
+            float top = 0.f;
+#pragma unroll 4
+            for (int c = 0; c < HD / 8; ++c) {
+                const uint4 w = *reinterpret_cast<const uint4*>(q + 8 * c);
+                const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float a = fabsf(__uint_as_float(x[i] << 16)), b = fabsf(__uint_as_float(x[i] & 0xffff0000u));
+                    if (a < INFINITY) top = fmaxf(top, a);
+                    if (b < INFINITY) top = fmaxf(top, b);
+                }
+            }
+            const int ex = q_exponent(top);
+            const float div = pow2_any(-ex);
+            f = p.scale * LOG2E * pow2_any(ex);
+#pragma unroll 4
+            for (int c = 0; c < HD / 8; ++c) {
+                const uint4 w = *reinterpret_cast<const uint4*>(q + 8 * c);
+                const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+                uint32_t h[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) h[i] = pack_f16(__uint_as_float(x[i] << 16) * div, __uint_as_float(x[i] & 0xffff0000u) * div);
+                *reinterpret_cast<uint4*>(sm->q[c / 8] + sw128(r, c % 8)) = make_uint4(h[0], h[1], h[2], h[3]);
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sm->q_full);
+        }
+        const uint32_t lane_base = (uint32_t)(warp * 32) << 16;
+        // m is the reference point of the exponentials; it moves to the first tile's maximum and then follows lazily: only when a tile exceeds
+        // it by more than 2^8 is O in TMEM rescaled (which has to wait for the product before).
+        float m = 0.f, l = 0.f;
+        bool seen = false;
+        const float slope = p.slopes ? p.slopes[head] * LOG2E : 0.f;
+        for (int j = 0; j < n_tiles && ok; ++j) {
+            const int s = j % KV_STAGES;
+            ok = mbar_wait(&sm->kv_full[s], (j / KV_STAGES) & 1) && mbar_wait(&sm->s_full[j & 1], (j >> 1) & 1);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            tcgen05_fence_after();
+            const uint32_t ts = ((j & 1) ? tm_s1 : tm_s0) + lane_base;
+            const int key0 = (tile0 + j) * BK;
+            float sc[BK];
+            tmem_ld64(ts, sc);
+            // z less the reference point as it stands
+#pragma unroll
+            for (int b = 0; b < 8; ++b) {
+                const float fk = f * sm->ks[s][b], lg = sm->vl[s][b] - m;
+                const u64 fk2 = pack2(fk, fk), lg2 = pack2(lg, lg);
+#pragma unroll
+                for (int i = 8 * b; i < 8 * b + 8; i += 2) unpack2(ffma2(pack2(sc[i], sc[i + 1]), fk2, lg2), sc[i], sc[i + 1]);
+            }
+            // only tiles that cross a row's diagonal or the window's edge need the mask
+            if (!(key0 + BK - 1 <= pos_first && (p.window <= 0 || key0 > pos_last - p.window)) || slope != 0.f) {
+#pragma unroll
+                for (int i = 0; i < BK; ++i) {
+                    const int key = key0 + i;
+                    const bool vis = key <= pos && (p.window <= 0 || key > pos - p.window);
+                    sc[i] = vis ? fmaf(slope, (float)(key - pos), sc[i]) : -INFINITY;
+                }
+            }
+            float m0 = sc[0], m1 = sc[1], m2 = sc[2], m3 = sc[3];          // four chains: a single one waits for itself
+#pragma unroll
+            for (int i = 4; i < BK - 4; i += 8) {
+                m0 = fmax3(m0, sc[i], sc[i + 1]);
+                m1 = fmax3(m1, sc[i + 2], sc[i + 3]);
+                m2 = fmax3(m2, sc[i + 4], sc[i + 5]);
+                m3 = fmax3(m3, sc[i + 6], sc[i + 7]);
+            }
+            m0 = fmax3(m0, sc[BK - 4], sc[BK - 3]);
+            m1 = fmax3(m1, sc[BK - 2], sc[BK - 1]);
+            const float mx = fmaxf(fmax3(m0, m1, m2), m3);
+            float corr = 1.f;
+            if (mx > 8.f || (!seen && mx > -INFINITY)) {                   // move the reference point
+                corr = seen ? q8_ex2(-mx) : 0.f;
+                seen = true;
+                m += mx;
+                const u64 by = pack2(-mx, -mx);
+#pragma unroll
+                for (int i = 0; i < BK; i += 2) unpack2(fadd2(pack2(sc[i], sc[i + 1]), by), sc[i], sc[i + 1]);
+                l *= corr;
+            }
+            uint32_t pk[BK / 2];
+#pragma unroll
+            for (int b = 0; b < 8; ++b) {
+                u64 sum2 = pack2(0.f, 0.f);
+#pragma unroll
+                for (int i = 8 * b; i < 8 * b + 8; i += 2) {
+                    const float x = q8_ex2(sc[i]), y = q8_ex2(sc[i + 1]);
+                    sum2 = fadd2(sum2, pack2(x, y));
+                    pk[i / 2] = pack_f16(x, y);
+                }
+                float x, y;
+                unpack2(sum2, x, y);
+                l = fmaf(x + y, sm->vi[s][b], l);
+            }
+            if (j > 0 && __any_sync(0xffffffffu, corr != 1.f)) {           // rescale this warp's rows of O
+                ok = mbar_wait(&sm->o_ready[(j - 1) & 1], ((j - 1) >> 1) & 1);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                tcgen05_fence_after();
+#pragma unroll
+                for (int c = 0; c < HD; c += 16) {
+                    float x[16];
+                    tmem_ld16(tm_o + lane_base + c, x);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) x[i] *= corr;
+                    tmem_st16(tm_o + lane_base + c, x);
+                }
+                tmem_st_wait();
+            }
+            // P -> tensor memory, over this row's S (whose last other reader, the product of tile j - 2, is complete with S_j)
+            tmem_st32(ts, pk);
+            tmem_st_wait();
+            tcgen05_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sm->p_full[j & 1]);
+        }
+        if (ok) {
+            ok = mbar_wait(&sm->o_ready[(n_tiles - 1) & 1], ((n_tiles - 1) >> 1) & 1);
+            ok = __all_sync(0xffffffffu, ok);
+        }
+        if (ok) {
+            tcgen05_fence_after();
+            const size_t at = (size_t)(q0 + token) * p.nH + head;
+            float* rec = p.scratch + (at * p.n_splits + split) * REC;
+            if (p.n_splits > 1 && r < rows_here) rec[0] = seen ? m : -INFINITY, rec[1] = l;
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+            for (int c = 0; c < HD; c += 16) {
+                float x[16];
+                tmem_ld16(tm_o + lane_base + c, x);
+                if (r < rows_here && p.n_splits > 1) {
+#pragma unroll
+                    for (int i = 0; i < 16; i += 4) *reinterpret_cast<float4*>(rec + 4 + c + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+                } else if (r < rows_here) {
+                    uint32_t w[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i] * inv, x[2 * i + 1] * inv);
+                        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+                    }
+                    *reinterpret_cast<uint4*>(p.out + at * HD + c) = make_uint4(w[0], w[1], w[2], w[3]);
+                    *reinterpret_cast<uint4*>(p.out + at * HD + c + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+                }
+                __syncwarp();
+            }
+        } else if (lane == 0) {
+            atomicOr(p.status, NG_STATUS_ATTN_TIMEOUT);
+        }
+    }
+    tcgen05_fence_before();
+    __syncthreads();
+    if (warp == 7) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 256;" :: "r"(tmem) : "memory");
+}
+
+NG_EXPORT int ng_attn_prefill_q8_sm100(const void* q, const void* k_pages, const void* v_pages, const float* k_scales, const float* v_scales,
+                                       const int* table, int table_stride, const int* cu_q, const int* ctx_before, void* out, float* scratch,
+                                       int n_rows, int n_entries, int max_q, int nH, int nKV, int hd, int page_size, int block, int num_pages,
+                                       int kind, int window, float scale, int skip_single, int n_splits, const float* slopes, int* status,
+                                       cudaStream_t stream) {
+    if (n_entries <= 0 || n_rows <= 0 || max_q <= 0) return NG_OK;
+    Params p;
+    if (hd != HD || nH <= 0 || !cache_of(p.c, k_pages, v_pages, k_scales, v_scales, table, table_stride, nKV, page_size, block, num_pages) ||
+        nH % nKV || n_splits < 1 || (long long)n_entries * n_splits > 65535 || (n_splits > 1 && (!scratch || ((uintptr_t)scratch & 15))) ||
+        window < 0 || ((uintptr_t)q & 15) || ((uintptr_t)out & 15) || (kind != NG_Q8_E4M3 && kind != NG_Q8_INT8) || !status)
+        return NG_BAD_SIZE;
+    const long long tiles = ((long long)max_q * (nH / nKV) + BQ - 1) / BQ;
+    if (tiles > 65535) return NG_BAD_SIZE;
+    p.q = (const bf16*)q; p.out = (bf16*)out; p.cu_q = cu_q; p.ctx_before = ctx_before; p.status = status; p.n_rows = n_rows; p.nH = nH;
+    p.window = window; p.skip_single = skip_single; p.n_splits = n_splits; p.scale = scale; p.slopes = slopes; p.scratch = scratch;
+    const dim3 grid(nKV, (unsigned)tiles, n_entries * n_splits);
+    constexpr int smem = (int)sizeof(Smem) + 1024;
+#define Q8P_GO(KIND)                                                                                                     \
+    do {                                                                                                                 \
+        static std::atomic<unsigned long long> once{0};                                                                  \
+        if (!ng_allow_smem(once, attn_prefill_q8_sm100_kernel<KIND>, smem)) return NG_LAUNCH_FAILED;                     \
+        NG_LAUNCH((attn_prefill_q8_sm100_kernel<KIND>), grid, Q8P_THREADS, smem, stream, p);                             \
+    } while (0)
+    if (kind == NG_Q8_E4M3) Q8P_GO(NG_Q8_E4M3);
+    else Q8P_GO(NG_Q8_INT8);
+    if (n_splits > 1) return q8_merge(scratch, cu_q, out, nH, n_splits, n_rows, n_entries, skip_single ? 2 : 1, 0x7fffffff, max_q, stream);
+    return ng_launch_status();
+}

@@ -38,6 +38,7 @@ SOURCES: Dict[str, Sequence[str]] = {
     "input_conv": (), "retention": (), "latent": (), "latent_mma": (), "moe": (), "token_side": (),
     "mapped_attention": (), "mapped_attention_mma": (), "mapped_attention_sm100": (), "gated_delta": (),
     "hyper": (), "gated_linear": (), "decayed_linear": (), "cache_q8": (), "attention_q8": (),
+    "attention_q8_sm100": (),
 }
 
 _lock = threading.RLock()
@@ -182,4 +183,5 @@ def build_all(extra: Sequence[Tuple[str, Mapping[str, object]]] = (), *, verbose
 # sources that only exist as ``-D`` specialisations (never built bare)
 SPECIALISED: Dict[str, Sequence[str]] = {"attention_bf16": ("NG_HEAD_DIM",), "shortconv": ("NG_CONV_L",),
                                          "rope_cache": ("NG_ROPE_PAIRS",), "latent_mma": ("NG_LAT_RANK",),
-                                         "mapped_attention_mma": ("NG_MA_D", "NG_MA_DV"), "attention_q8": ("NG_HEAD_DIM",)}
+                                         "mapped_attention_mma": ("NG_MA_D", "NG_MA_DV"), "attention_q8": ("NG_HEAD_DIM",),
+                                         "attention_q8_sm100": ("NG_HEAD_DIM",)}

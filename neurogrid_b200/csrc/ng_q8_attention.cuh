@@ -1,0 +1,159 @@
+// What the attention kernels over a cache in 8 bits share: the head size they are compiled for (-DNG_HEAD_DIM), the cache as their
+// arguments have it, the records that runs of the keys leave and the kernel that merges them.
+#pragma once
+#include "ng_q8.cuh"
+
+#ifndef NG_HEAD_DIM
+#error "compile with -DNG_HEAD_DIM=<head size>"
+#endif
+#define HD NG_HEAD_DIM
+static_assert(HD % 16 == 0 && HD >= 16 && HD <= 256, "head size must be a multiple of 16 in [16, 256]");
+#define LOG2E 1.4426950408889634f
+#define REC (HD + 4)            // floats of a run's record: reference point, sum, number of runs (single tokens), one unused, row in codes
+
+typedef __nv_bfloat16 bf16;
+
+__device__ __forceinline__ float q8_ex2(float x) {       // 2^x, 2 ulp; -inf -> 0
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// The power of two that a row of q is divided by (its largest value becomes 1 to 2): exponent of the row's largest finite value.
+__device__ __forceinline__ int q_exponent(float top) { return min(max((int)(__float_as_uint(top) >> 23) - 127, -100), 127); }
+__device__ __forceinline__ float pow2_any(int e) { return q8_pow2(min(max(e, -126), 127)); }
+
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+    uint32_t d;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+    return d;
+}
+
+struct Cache {
+    const unsigned char *k, *v;          // [pages, nKV, page, HD]
+    const float *ks, *vs;                // [pages, nKV, page / block]
+    const int* table;
+    int table_stride, num_pages, nKV, ps_log2, bl_log2;
+};
+
+// out[row, head] = sum_s o_s 2^(m_s - m) / sum_s l_s 2^(m_s - m) over the runs s.  A warp has a (row, head) (WIDE: all four warps of a block, every
+// fourth run each, joined in order): lane s looks after run s's reference point and sum, then the lanes share the dimensions and walk the
+// runs in ascending order.  Rows are the entries' single tokens, whose first record says how many runs there are, or (portions) all rows of
+// the entries that bring more.
+#define MG_WARPS 4
+constexpr int MG_EACH = (HD + 63) / 64;                              // pairs of dimensions a lane has
+template <bool WIDE>
+__global__ void __launch_bounds__(MG_WARPS * 32)
+attn_q8_merge_kernel(const float* __restrict__ scratch, const int* __restrict__ cu_q, bf16* __restrict__ out, int nH, int room, int n_rows,
+                     int least, int most) {
+    __shared__ float part_s[WIDE ? MG_WARPS : 1][HD + 2];
+    ng_pdl_trigger();
+    const int e = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int head = WIDE ? blockIdx.x : blockIdx.x * MG_WARPS + warp;
+    const int q0 = cu_q[e], n = cu_q[e + 1] - q0;
+    ng_pdl_wait();
+    if (n < least || n > most || (!WIDE && head >= nH)) return;
+    scratch = ng_after_wait(scratch);
+    constexpr int STEP = WIDE ? MG_WARPS : 1;
+    for (int r = q0 + blockIdx.z; r < min(q0 + n, n_rows); r += gridDim.z) {
+        const float* rec = scratch + ((size_t)r * nH + head) * room * REC;
+        // (the first 32 runs' are asked for before it is known how many there are)
+        const int s0 = lane * STEP + (WIDE ? warp : 0);
+        float m0 = s0 < room ? rec[(size_t)s0 * REC] : -INFINITY, l0 = s0 < room ? rec[(size_t)s0 * REC + 1] : 0.f;
+        int runs = room;
+        if (most == 1) {
+            runs = (int)rec[2];
+            if (runs <= 1) continue;
+        }
+        float m = -INFINITY, l = 0.f, acc[MG_EACH][2] = {};
+        for (int b = 0; b < runs; b += 32 * STEP) {
+            const int s1 = b + s0;
+            float ms = m0, ls = l0;
+            if (b > 0) {
+                ms = s1 < runs ? rec[(size_t)s1 * REC] : -INFINITY;
+                ls = s1 < runs ? rec[(size_t)s1 * REC + 1] : 0.f;
+            }
+            if (s1 >= runs) ms = -INFINITY, ls = 0.f;
+            const float mb = fmaxf(m, ng_warp_max(ms)), c = m == -INFINITY ? (mb == -INFINITY ? 1.f : 0.f) : q8_ex2(m - mb);
+            const float f = ms == -INFINITY ? (mb == -INFINITY ? 1.f : 0.f) : q8_ex2(ms - mb);          // (a run that met only NaN kept its sums)
+            m = mb;
+            l = fmaf(l, c, ng_warp_sum(ls * f));
+#pragma unroll
+            for (int i = 0; i < MG_EACH; ++i) acc[i][0] *= c, acc[i][1] *= c;
+            const uint32_t some = __ballot_sync(0xffffffffu, ls != 0.f);                               // (an empty run wrote no row)
+            const int here = min(32, (runs - b - (WIDE ? warp : 0) + STEP - 1) / STEP);
+#pragma unroll 4
+            for (int k = 0; k < here; ++k) {
+                const float fk = __shfl_sync(0xffffffffu, f, k);
+                if (!(some >> k & 1)) continue;
+                const float* row = rec + (size_t)(b + k * STEP + (WIDE ? warp : 0)) * REC + 4;
+#pragma unroll
+                for (int i = 0; i < MG_EACH; ++i) {
+                    const int d = 2 * lane + 64 * i;
+                    if (HD % 64 != 0 && d >= HD) continue;
+                    const float2 x = *reinterpret_cast<const float2*>(row + d);
+                    acc[i][0] = fmaf(x.x, fk, acc[i][0]);
+                    acc[i][1] = fmaf(x.y, fk, acc[i][1]);
+                }
+            }
+        }
+        if constexpr (WIDE) {
+            __syncthreads();                                         // the row before has been written
+            if (lane == 0) part_s[warp][0] = m, part_s[warp][1] = l;
+#pragma unroll
+            for (int i = 0; i < MG_EACH; ++i) {
+                const int d = 2 * lane + 64 * i;
+                if (HD % 64 == 0 || d < HD) part_s[warp][2 + d] = acc[i][0], part_s[warp][3 + d] = acc[i][1];
+            }
+            __syncthreads();
+            if (warp > 0) continue;
+            float top = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < MG_WARPS; ++w) top = fmaxf(top, part_s[w][0]);
+            l = 0.f;
+#pragma unroll
+            for (int i = 0; i < MG_EACH; ++i) acc[i][0] = acc[i][1] = 0.f;
+#pragma unroll
+            for (int w = 0; w < MG_WARPS; ++w) {
+                const float f = part_s[w][0] == -INFINITY ? (top == -INFINITY ? 1.f : 0.f) : q8_ex2(part_s[w][0] - top);
+                l = fmaf(part_s[w][1], f, l);
+#pragma unroll
+                for (int i = 0; i < MG_EACH; ++i) {
+                    const int d = 2 * lane + 64 * i;
+                    if (HD % 64 == 0 || d < HD) acc[i][0] = fmaf(part_s[w][2 + d], f, acc[i][0]), acc[i][1] = fmaf(part_s[w][3 + d], f, acc[i][1]);
+                }
+            }
+        }
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+        for (int i = 0; i < MG_EACH; ++i) {
+            const int d = 2 * lane + 64 * i;
+            if (HD % 64 == 0 || d < HD)
+                *reinterpret_cast<__nv_bfloat162*>(out + ((size_t)r * nH + head) * HD + d) = __floats2bfloat162_rn(acc[i][0] * inv, acc[i][1] * inv);
+        }
+    }
+}
+
+static int q8_merge(const float* scratch, const int* cu_q, void* out, int nH, int n_splits, int n_rows, int n_entries, int least, int most,
+                 int rows, cudaStream_t stream) {
+    const int z = rows < 1 ? 1 : rows > 65535 ? 65535 : rows;
+    if (n_splits > 8 && (long long)n_entries * nH * z < 1024)        // many runs of few rows
+        NG_LAUNCH((attn_q8_merge_kernel<true>), dim3(nH, n_entries, z), MG_WARPS * 32, 0, stream, scratch, cu_q, (bf16*)out, nH, n_splits, n_rows, least, most);
+    else
+        NG_LAUNCH((attn_q8_merge_kernel<false>), dim3((nH + MG_WARPS - 1) / MG_WARPS, n_entries, z), MG_WARPS * 32, 0, stream, scratch, cu_q, (bf16*)out,
+                  nH, n_splits, n_rows, least, most);
+    return ng_launch_status();
+}
+
+static int log2_exact(int n) {               // -1: not a power of two
+    if (n <= 0 || (n & (n - 1))) return -1;
+    int l = 0;
+    while ((1 << l) < n) ++l;
+    return l;
+}
+static bool cache_of(Cache& c, const void* k_pages, const void* v_pages, const float* ks, const float* vs, const int* table, int table_stride,
+                     int nKV, int page_size, int block, int num_pages) {
+    c = Cache{(const unsigned char*)k_pages, (const unsigned char*)v_pages, ks, vs, table, table_stride, num_pages, nKV, log2_exact(page_size),
+              log2_exact(block)};
+    return c.ps_log2 >= 3 && c.bl_log2 >= 3 && c.bl_log2 <= c.ps_log2 && nKV > 0 && table_stride > 0 && num_pages > 0 &&
+           ((long long)nKV * page_size * HD) <= 0x7fffffff && !(((uintptr_t)k_pages | (uintptr_t)v_pages) & 15);
+}

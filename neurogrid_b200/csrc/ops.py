@@ -559,7 +559,8 @@ def attn_prefill_q8_splits(q_lens, n_heads: int, n_kv_heads: int, head_dim: int,
     group = n_heads // n_kv_heads
     blocks = sum(-(-n * group // 128) for n in q_lens) * n_kv_heads
     span = min(window + max(q_lens), max_ctx) if window else max_ctx
-    return max(1, min(_sm_count(device) // max(1, blocks), span // 512, 65535 // max(1, len(q_lens))))
+    slots = (2 if head_dim in (64, 128) else 1) * _sm_count(device)
+    return max(1, min(slots // max(1, blocks), span // 512, 65535 // max(1, len(q_lens))))
 
 
 def _q8_attention(what, q, out, scratch, cache, cu_q, ctx_before, n_entries, n_heads, n_splits):
@@ -610,12 +611,18 @@ def attn_prefill_q8(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     cache = (k_pages, v_pages, k_scales, v_scales, table)
     kind, num_pages, n_kv, page_size, hd, block = _q8_attention("attn_prefill_q8", q, out, scratch, cache, cu_q, ctx_before, n_entries,
                                                                 n_heads, n_splits)
-    f = _fn("attention_q8", "ng_attn_prefill_q8", [_c_void_p] * 6 + [_c_int] + [_c_void_p] * 4 + [_c_int] * 11
-            + [_c_float, _c_int, _c_int, _c_void_p, _c_void_p], {"NG_HEAD_DIM": hd})
-    _check(f(_ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(k_scales), _ptr(v_scales), _ptr(table), table.shape[1], _ptr(cu_q),
-             _ptr(ctx_before), _ptr(out), _ptr(scratch) if n_splits > 1 else None, q.shape[0], n_entries, int(max_q), n_heads, n_kv, hd,
-             page_size, block, num_pages, kind, int(window or 0), float(scale), int(bool(skip_single)), int(n_splits),
-             _slopes(slopes, n_heads), _stream()), "attn_prefill_q8")
+    tail = [_ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(k_scales), _ptr(v_scales), _ptr(table), table.shape[1], _ptr(cu_q),
+            _ptr(ctx_before), _ptr(out), _ptr(scratch) if n_splits > 1 else None, q.shape[0], n_entries, int(max_q), n_heads, n_kv, hd,
+            page_size, block, num_pages, kind, int(window or 0), float(scale), int(bool(skip_single)), int(n_splits),
+            _slopes(slopes, n_heads)]
+    types = [_c_void_p] * 6 + [_c_int] + [_c_void_p] * 4 + [_c_int] * 11 + [_c_float, _c_int, _c_int, _c_void_p]
+    if ATTN_BACKEND == "sm100" and hd in (64, 128) and q.data_ptr() % 16 == 0 and out.data_ptr() % 16 == 0:
+        f = _fn("attention_q8_sm100", "ng_attn_prefill_q8_sm100", types + [_c_void_p] * 2, {"NG_HEAD_DIM": hd})
+        rc = f(*tail, _ptr(_gemm_status(q.device)), _stream())
+    else:
+        f = _fn("attention_q8", "ng_attn_prefill_q8", types + [_c_void_p], {"NG_HEAD_DIM": hd})
+        rc = f(*tail, _stream())
+    _check(rc, "attn_prefill_q8")
 
 
 # ----------------------------------------------------------------------------- attention with float32 weights
