@@ -16,19 +16,6 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], u
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// BYTES of codes from a page; no line of the first-level cache is taken (they are read once).  Not moved above the wait.
-template <int BYTES>
-__device__ __forceinline__ void ld_codes(uint32_t* w, const unsigned char* p) {
-    if constexpr (BYTES == 16)
-        asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "l"(p) : "memory");
-    else if constexpr (BYTES == 8)
-        asm volatile("ld.global.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "l"(p) : "memory");
-    else if constexpr (BYTES == 4)
-        asm volatile("ld.global.L1::no_allocate.u32 %0, [%1];" : "=r"(w[0]) : "l"(p) : "memory");
-    else
-        asm volatile("{\n\t.reg .u16 h;\n\tld.global.L1::no_allocate.u16 h, [%1];\n\tcvt.u32.u16 %0, h;\n\t}" : "=r"(w[0]) : "l"(p) : "memory");
-}
-
 // ===================================================================================== single tokens
 // A segment is an entry's keys for up to 8 NT query heads of one KV head.  The block's four warps take groups of GROUP keys in turn, each on
 // its own (no barrier until the end of a piece).  Keys are the rows of the first product's tiles and dimensions those of the second's,

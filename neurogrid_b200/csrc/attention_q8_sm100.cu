@@ -16,6 +16,8 @@
 // is bounded; a waiter that gives up sets a status bit and the block runs to its end.
 //
 // Bound by the exponentials and the instructions around them (a score costs the thread of its row about three).
+#include <type_traits>
+
 #include "sm100_common.cuh"
 #include "ng_q8_attention.cuh"
 
@@ -84,7 +86,8 @@ template <int KIND>
 __global__ void __launch_bounds__(Q8P_THREADS, 2)
 attn_prefill_q8_sm100_kernel(const Params p) {
     extern __shared__ unsigned char smem_raw[];
-    Smem* sm = reinterpret_cast<Smem*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    // (an offset, not a rounded address: the compiler then knows that what it points to is shared memory)
+    Smem* sm = reinterpret_cast<Smem*>(smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u));
     ng_pdl_trigger();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     uint32_t elected;
@@ -138,71 +141,87 @@ attn_prefill_q8_sm100_kernel(const Params p) {
 
     if (warp >= 4 && warp < 4 + KV_WARPS) {
         // ------------------------------------------------------------------ keys and values
-        constexpr int PER_KEY = HD / 16, PIECES = BK * PER_KEY, LOADERS = 32 * KV_WARPS, EACH = (PIECES + LOADERS - 1) / LOADERS;
-        // 16-byte pieces of a key, of a tile, and of a thread (of K; V has as many)
-        const int tid = threadIdx.x - 128, mask = (1 << p.c.ps_log2) - 1;
+        // A unit is eight keys (they lie in one page and one block) of K and of V: UNIT_LOADS requests of 16 bytes a lane each.  A warp has
+        // every third unit; page numbers are asked for a tile before the codes, the codes DEPTH tiles before they are stored.
+        constexpr int UNIT_LOADS = HD / 64, UNITS = (8 + KV_WARPS - 1) / KV_WARPS, DEPTH = HD == 64 ? 2 : 1;
+        const int w = __shfl_sync(0xffffffffu, warp - 4, 0), mask = (1 << p.c.ps_log2) - 1;
         const int* trow = p.c.table + (size_t)e * p.c.table_stride;
-        const unsigned char *k_pages = ng_after_wait(p.c.k), *v_pages = ng_after_wait(p.c.v);
-        uint32_t k[EACH][4], v[EACH][4];
-        float ks = 1.f, vs = 1.f;
-        auto page_of = [&](int key, int lo) {
-            int page = -1;
-            if (key >= lo && key < kv_end && (key >> p.c.ps_log2) < p.c.table_stride) page = trow[key >> p.c.ps_log2];
-            return page >= 0 && page < p.c.num_pages ? page : -1;
+        const long long page_bytes = (long long)(p.c.nKV << p.c.ps_log2) * HD, head_at = (long long)(kvh << p.c.ps_log2) * HD + lane * 16;
+        const unsigned char *k_pages = p.c.k + head_at, *v_pages = p.c.v + head_at;
+        uint32_t k[DEPTH][UNITS][UNIT_LOADS][4], v[DEPTH][UNITS][UNIT_LOADS][4];
+        float ks[DEPTH], vs[DEPTH];
+        int page[UNITS], my_page;                              // of the next tile to ask for; my_page: lane u's, unit u's (the scales)
+        auto page_of = [&](int key) {
+            const int i = key >> p.c.ps_log2;
+            const int id = key + 7 >= key_lo && key < kv_end && i < p.c.table_stride ? trow[i] : -1;
+            return (unsigned)id < (unsigned)p.c.num_pages ? id : -1;
         };
-        auto load = [&](int tile) {
+        auto pages = [&](int tile) {
 #pragma unroll
-            for (int n = 0; n < EACH; ++n) {
-                const int i = tid + LOADERS * n, key = tile * BK + i / PER_KEY, page = i < PIECES ? page_of(key, key_lo) : -1;
-                if (page < 0) {
+            for (int n = 0; n < UNITS; ++n) page[n] = w + KV_WARPS * n < 8 ? page_of(tile * BK + 8 * (w + KV_WARPS * n)) : -1;
+            my_page = w == KV_WARPS - 1 && lane < 8 ? page_of(tile * BK + 8 * lane) : -1;
+        };
+        auto load = [&](int d, int tile) {
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) k[n][x] = v[n][x] = 0u;
-                } else {
-                    const size_t at = ((((size_t)page * p.c.nKV + kvh) << p.c.ps_log2) + (key & mask)) * HD + (i % PER_KEY) * 16;
-                    const uint4 a = *reinterpret_cast<const uint4*>(k_pages + at), b = *reinterpret_cast<const uint4*>(v_pages + at);
-                    k[n][0] = a.x; k[n][1] = a.y; k[n][2] = a.z; k[n][3] = a.w;
-                    v[n][0] = b.x; v[n][1] = b.y; v[n][2] = b.z; v[n][3] = b.w;
+            for (int n = 0; n < UNITS; ++n) {
+                const int key0 = tile * BK + 8 * (w + KV_WARPS * n);
+                const long long at = (long long)max(page[n], 0) * page_bytes + (key0 & mask) * HD;
+#pragma unroll
+                for (int i = 0; i < UNIT_LOADS; ++i) {
+                    const int key = key0 + (i * 512 + lane * 16) / HD;
+                    const bool in = page[n] >= 0 && key >= key_lo && key < kv_end;
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) k[d][n][i][x] = v[d][n][i][x] = 0u;
+                    if (in) ld_codes<16>(k[d][n][i], k_pages + at + i * 512), ld_codes<16>(v[d][n][i], v_pages + at + i * 512);
                 }
             }
-            if (tid < 8) {
-                const int key = tile * BK + 8 * tid, page = page_of(key, key_lo - 7);
-                ks = vs = 1.f;
-                if (page >= 0) {
-                    const size_t sc = (((size_t)page * p.c.nKV + kvh) << (p.c.ps_log2 - p.c.bl_log2)) + ((key & mask) >> p.c.bl_log2);
-                    ks = ng_after_wait(p.c.ks)[sc];
-                    vs = ng_after_wait(p.c.vs)[sc];
-                }
+            ks[d] = vs[d] = 1.f;
+            if (my_page >= 0) {
+                const long long sc = ((long long)my_page * p.c.nKV + kvh << (p.c.ps_log2 - p.c.bl_log2)) + ((tile * BK + 8 * lane & mask) >> p.c.bl_log2);
+                ld_codes<4>(reinterpret_cast<uint32_t*>(&ks[d]), reinterpret_cast<const unsigned char*>(p.c.ks + sc));
+                ld_codes<4>(reinterpret_cast<uint32_t*>(&vs[d]), reinterpret_cast<const unsigned char*>(p.c.vs + sc));
             }
         };
-        auto put = [](uint16_t* tile, int row, int c, const uint32_t (&w)[4]) {          // 16 codes: chunks c and c + 1 of the row
+        auto put = [](uint16_t* tile, int row, int c, const uint32_t (&x)[4]) {          // 16 codes: chunks c and c + 1 of the row
             uint32_t h[8];
 #pragma unroll
-            for (int x = 0; x < 4; ++x) q8_to_half<KIND>(w[x], h[2 * x], h[2 * x + 1]);
+            for (int i = 0; i < 4; ++i) q8_to_half<KIND>(x[i], h[2 * i], h[2 * i + 1]);
             *reinterpret_cast<uint4*>(tile + sw128(row, c)) = make_uint4(h[0], h[1], h[2], h[3]);
             *reinterpret_cast<uint4*>(tile + sw128(row, c + 1)) = make_uint4(h[4], h[5], h[6], h[7]);
         };
-        load(tile0);
-        for (int j = 0; j < n_tiles && ok; ++j) {
-            const int s = j % KV_STAGES;
-            ok = __all_sync(0xffffffffu, mbar_wait(&sm->kv_empty[s], ((j / KV_STAGES) & 1) ^ 1));
-            if (!ok) break;
+        pages(tile0);
 #pragma unroll
-            for (int n = 0; n < EACH; ++n) {
-                const int i = tid + LOADERS * n, row = i / PER_KEY, c = i % PER_KEY * 2;
-                if (i >= PIECES) break;
-                put(sm->k[s][c / 8], row, c % 8, k[n]);
-                put(sm->v[s][c / 8], row, c % 8, v[n]);
-            }
-            if (tid < 8) {
-                sm->ks[s][tid] = ks;
-                sm->vl[s][tid] = q8_log2(vs);
-                sm->vi[s][tid] = q8_recip(vs);
-            }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sm->kv_full[s]);
-            if (j + 1 < n_tiles) load(tile0 + j + 1);
+        for (int d = 0; d < DEPTH; ++d) {
+            load(d, tile0 + d);
+            pages(tile0 + d + 1);
         }
+        for (int j0 = 0; j0 < n_tiles && ok; j0 += DEPTH)
+#pragma unroll
+            for (int d = 0; d < DEPTH; ++d) {
+                const int j = j0 + d, s = j % KV_STAGES;
+                if (j >= n_tiles || !ok) break;
+                ok = __all_sync(0xffffffffu, mbar_wait(&sm->kv_empty[s], ((j / KV_STAGES) & 1) ^ 1));
+                if (!ok) break;
+#pragma unroll
+                for (int n = 0; n < UNITS; ++n)
+                    if (w + KV_WARPS * n < 8)
+#pragma unroll
+                        for (int i = 0; i < UNIT_LOADS; ++i) {
+                            const int o = i * 512 + lane * 16, row = 8 * (w + KV_WARPS * n) + o / HD, c = o % HD / 8;
+                            put(sm->k[s][c / 8], row, c % 8, k[d][n][i]);
+                            put(sm->v[s][c / 8], row, c % 8, v[d][n][i]);
+                        }
+                if (w == KV_WARPS - 1 && lane < 8) {
+                    sm->ks[s][lane] = ks[d];
+                    sm->vl[s][lane] = q8_log2(vs[d]);
+                    sm->vi[s][lane] = q8_recip(vs[d]);
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sm->kv_full[s]);
+                load(d, tile0 + j + DEPTH);                    // (behind the last tile: zeros, from no page)
+                pages(tile0 + j + DEPTH + 1);
+            }
         if (!ok && lane == 0) atomicOr(p.status, NG_STATUS_ATTN_TIMEOUT);
     } else if (warp == 7) {
         // ------------------------------------------------------------------ MMA issuer: all lanes run the loop, one issues
@@ -299,58 +318,83 @@ attn_prefill_q8_sm100_kernel(const Params p) {
             const int key0 = (tile0 + j) * BK;
             float sc[BK];
             tmem_ld64(ts, sc);
-            // z less the reference point as it stands
+            // only tiles that cross a row's diagonal or the window's edge need the mask; z is then formed here.  A distance bias alone is linear
+            // in the key: its part within each eight keys is added here, the rest goes with the values' scale.
+            const bool masked = !(key0 + BK - 1 <= pos_first && (p.window <= 0 || key0 > pos_last - p.window));
+            const bool formed = masked || slope != 0.f;
+            if (masked) {
 #pragma unroll
-            for (int b = 0; b < 8; ++b) {
-                const float fk = f * sm->ks[s][b], lg = sm->vl[s][b] - m;
-                const u64 fk2 = pack2(fk, fk), lg2 = pack2(lg, lg);
+                for (int b = 0; b < 8; ++b) {
+                    const float fk = f * sm->ks[s][b], lg = sm->vl[s][b];
 #pragma unroll
-                for (int i = 8 * b; i < 8 * b + 8; i += 2) unpack2(ffma2(pack2(sc[i], sc[i + 1]), fk2, lg2), sc[i], sc[i + 1]);
-            }
-            // only tiles that cross a row's diagonal or the window's edge need the mask
-            if (!(key0 + BK - 1 <= pos_first && (p.window <= 0 || key0 > pos_last - p.window)) || slope != 0.f) {
-#pragma unroll
-                for (int i = 0; i < BK; ++i) {
-                    const int key = key0 + i;
-                    const bool vis = key <= pos && (p.window <= 0 || key > pos - p.window);
-                    sc[i] = vis ? fmaf(slope, (float)(key - pos), sc[i]) : -INFINITY;
+                    for (int i = 8 * b; i < 8 * b + 8; ++i) {
+                        const int key = key0 + i;
+                        const bool vis = key <= pos && (p.window <= 0 || key > pos - p.window);
+                        sc[i] = vis ? fmaf(slope, (float)(key - pos), fmaf(sc[i], fk, lg)) : -INFINITY;
+                    }
                 }
-            }
-            float m0 = sc[0], m1 = sc[1], m2 = sc[2], m3 = sc[3];          // four chains: a single one waits for itself
+            } else if (formed) {
 #pragma unroll
-            for (int i = 4; i < BK - 4; i += 8) {
-                m0 = fmax3(m0, sc[i], sc[i + 1]);
-                m1 = fmax3(m1, sc[i + 2], sc[i + 3]);
-                m2 = fmax3(m2, sc[i + 4], sc[i + 5]);
-                m3 = fmax3(m3, sc[i + 6], sc[i + 7]);
-            }
-            m0 = fmax3(m0, sc[BK - 4], sc[BK - 3]);
-            m1 = fmax3(m1, sc[BK - 2], sc[BK - 1]);
-            const float mx = fmaxf(fmax3(m0, m1, m2), m3);
-            float corr = 1.f;
-            if (mx > 8.f || (!seen && mx > -INFINITY)) {                   // move the reference point
-                corr = seen ? q8_ex2(-mx) : 0.f;
-                seen = true;
-                m += mx;
-                const u64 by = pack2(-mx, -mx);
+                for (int b = 0; b < 8; ++b) {
+                    const float fk = f * sm->ks[s][b];
+                    const u64 fk2 = pack2(fk, fk);
 #pragma unroll
-                for (int i = 0; i < BK; i += 2) unpack2(fadd2(pack2(sc[i], sc[i + 1]), by), sc[i], sc[i + 1]);
-                l *= corr;
+                    for (int i = 0; i < 8; i += 2)
+                        unpack2(ffma2(pack2(sc[8 * b + i], sc[8 * b + i + 1]), fk2, pack2(slope * i, slope * (i + 1))), sc[8 * b + i], sc[8 * b + i + 1]);
+                }
             }
             uint32_t pk[BK / 2];
+            float corr = 1.f;
+            // z = sc fk + lg for each eight keys (f and the scales are positive, so the largest sc has the largest z)
+            auto weigh = [&](auto is_formed) {
+                constexpr bool FORMED = decltype(is_formed)::value;
+                const float far = masked ? 0.f : slope * (float)(key0 - pos), far8 = masked ? 0.f : 8.f * slope, own = masked ? 0.f : 1.f;
+                float mx = -INFINITY;
 #pragma unroll
-            for (int b = 0; b < 8; ++b) {
-                u64 sum2 = pack2(0.f, 0.f);
+                for (int b = 0; b < 8; b += 4) {
+                    const float4 k4 = *reinterpret_cast<const float4*>(&sm->ks[s][b]), v4 = *reinterpret_cast<const float4*>(&sm->vl[s][b]);
+                    const float ks[4] = {k4.x, k4.y, k4.z, k4.w}, vl[4] = {v4.x, v4.y, v4.z, v4.w};
+                    float mz[4];
 #pragma unroll
-                for (int i = 8 * b; i < 8 * b + 8; i += 2) {
-                    const float x = q8_ex2(sc[i]), y = q8_ex2(sc[i + 1]);
-                    sum2 = fadd2(sum2, pack2(x, y));
-                    pk[i / 2] = pack_f16(x, y);
+                    for (int i = 0; i < 4; ++i) {
+                        const float* x = sc + 8 * (b + i);
+                        const float y = fmaxf(fmax3(fmax3(x[0], x[1], x[2]), fmax3(x[3], x[4], x[5]), x[6]), x[7]);
+                        mz[i] = FORMED ? y + fmaf(own, vl[i], fmaf(far8, (float)(b + i), far)) : fmaf(y, f * ks[i], vl[i]);
+                    }
+                    mx = fmax3(mx, fmaxf(mz[0], mz[1]), fmaxf(mz[2], mz[3]));
                 }
-                float x, y;
-                unpack2(sum2, x, y);
-                l = fmaf(x + y, sm->vi[s][b], l);
-            }
+                if (mx > m + 8.f || (!seen && mx > -INFINITY)) {           // move the reference point
+                    corr = seen ? q8_ex2(m - mx) : 0.f;
+                    seen = true;
+                    m = mx;
+                    l *= corr;
+                }
+#pragma unroll
+                for (int b = 0; b < 8; b += 4) {
+                    const float4 k4 = *reinterpret_cast<const float4*>(&sm->ks[s][b]), v4 = *reinterpret_cast<const float4*>(&sm->vl[s][b]);
+                    const float4 i4 = *reinterpret_cast<const float4*>(&sm->vi[s][b]);
+                    const float ks[4] = {k4.x, k4.y, k4.z, k4.w}, vl[4] = {v4.x, v4.y, v4.z, v4.w}, vi[4] = {i4.x, i4.y, i4.z, i4.w};
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        const float fk = f * ks[u], lg = (FORMED ? fmaf(own, vl[u], fmaf(far8, (float)(b + u), far)) : vl[u]) - m;
+                        const u64 fk2 = pack2(fk, fk), lg2 = pack2(lg, lg);
+                        u64 sum2 = pack2(0.f, 0.f);
+#pragma unroll
+                        for (int i = 8 * (b + u); i < 8 * (b + u) + 8; i += 2) {
+                            float x, y;
+                            unpack2(FORMED ? fadd2(pack2(sc[i], sc[i + 1]), lg2) : ffma2(pack2(sc[i], sc[i + 1]), fk2, lg2), x, y);
+                            x = q8_ex2(x), y = q8_ex2(y);
+                            sum2 = fadd2(sum2, pack2(x, y));
+                            pk[i / 2] = pack_f16(x, y);
+                        }
+                        float x, y;
+                        unpack2(sum2, x, y);
+                        l = fmaf(x + y, vi[u], l);
+                    }
+                }
+            };
+            if (formed) weigh(std::true_type{});
+            else weigh(std::false_type{});
             if (j > 0 && __any_sync(0xffffffffu, corr != 1.f)) {           // rescale this warp's rows of O
                 ok = mbar_wait(&sm->o_ready[(j - 1) & 1], ((j - 1) >> 1) & 1);
                 ok = __all_sync(0xffffffffu, ok);
@@ -420,7 +464,7 @@ NG_EXPORT int ng_attn_prefill_q8_sm100(const void* q, const void* k_pages, const
     Params p;
     if (hd != HD || nH <= 0 || !cache_of(p.c, k_pages, v_pages, k_scales, v_scales, table, table_stride, nKV, page_size, block, num_pages) ||
         nH % nKV || n_splits < 1 || (long long)n_entries * n_splits > 65535 || (n_splits > 1 && (!scratch || ((uintptr_t)scratch & 15))) ||
-        window < 0 || ((uintptr_t)q & 15) || ((uintptr_t)out & 15) || (kind != NG_Q8_E4M3 && kind != NG_Q8_INT8) || !status)
+        window < 0 || !(scale > 0.f) || ((uintptr_t)q & 15) || ((uintptr_t)out & 15) || (kind != NG_Q8_E4M3 && kind != NG_Q8_INT8) || !status)
         return NG_BAD_SIZE;
     const long long tiles = ((long long)max_q * (nH / nKV) + BQ - 1) / BQ;
     if (tiles > 65535) return NG_BAD_SIZE;

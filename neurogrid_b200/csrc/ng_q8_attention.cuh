@@ -35,6 +35,19 @@ struct Cache {
     int table_stride, num_pages, nKV, ps_log2, bl_log2;
 };
 
+// BYTES of codes from a page; no line of the first-level cache is taken (they are read once).  Not moved above the wait.
+template <int BYTES>
+__device__ __forceinline__ void ld_codes(uint32_t* w, const unsigned char* p) {
+    if constexpr (BYTES == 16)
+        asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "l"(p) : "memory");
+    else if constexpr (BYTES == 8)
+        asm volatile("ld.global.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "l"(p) : "memory");
+    else if constexpr (BYTES == 4)
+        asm volatile("ld.global.L1::no_allocate.u32 %0, [%1];" : "=r"(w[0]) : "l"(p) : "memory");
+    else
+        asm volatile("{\n\t.reg .u16 h;\n\tld.global.L1::no_allocate.u16 h, [%1];\n\tcvt.u32.u16 %0, h;\n\t}" : "=r"(w[0]) : "l"(p) : "memory");
+}
+
 // out[row, head] = sum_s o_s 2^(m_s - m) / sum_s l_s 2^(m_s - m) over the runs s.  A warp has a (row, head) (WIDE: all four warps of a block, every
 // fourth run each, joined in order): lane s looks after run s's reference point and sum, then the lanes share the dimensions and walk the
 // runs in ascending order.  Rows are the entries' single tokens, whose first record says how many runs there are, or (portions) all rows of

@@ -616,7 +616,7 @@ def attn_prefill_q8(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
             page_size, block, num_pages, kind, int(window or 0), float(scale), int(bool(skip_single)), int(n_splits),
             _slopes(slopes, n_heads)]
     types = [_c_void_p] * 6 + [_c_int] + [_c_void_p] * 4 + [_c_int] * 11 + [_c_float, _c_int, _c_int, _c_void_p]
-    if ATTN_BACKEND == "sm100" and hd in (64, 128) and q.data_ptr() % 16 == 0 and out.data_ptr() % 16 == 0:
+    if ATTN_BACKEND == "sm100" and hd in (64, 128) and scale > 0 and q.data_ptr() % 16 == 0 and out.data_ptr() % 16 == 0:
         f = _fn("attention_q8_sm100", "ng_attn_prefill_q8_sm100", types + [_c_void_p] * 2, {"NG_HEAD_DIM": hd})
         rc = f(*tail, _ptr(_gemm_status(q.device)), _stream())
     else:
