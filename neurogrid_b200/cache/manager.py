@@ -30,7 +30,8 @@ class PagedNeed:
     ``values`` False: one vector per token and head only (a layer that caches a latent from which
     it forms keys and values itself); such pages have no value half.  ``v_heads`` / ``v_dim``: the value half's
     heads and size where they differ from the keys' (None: the same).  ``keep_first``: with a window, the pages
-    that hold the first that many tokens are kept as well (a mask that never loses sight of them)."""
+    that hold the first that many tokens are kept as well (a mask that never loses sight of them).  ``eight_bit``: the layer can also
+    work on pages of codes with a scale for each block of tokens and head (a cache opened with an 8-bit type then holds them so)."""
     n_kv_heads: int
     head_dim: int
     window: Optional[int] = None
@@ -38,6 +39,7 @@ class PagedNeed:
     v_heads: Optional[int] = None
     v_dim: Optional[int] = None
     keep_first: int = 0
+    eight_bit: bool = False
 
     def value_shape(self):
         """(heads, size) of the value half."""
@@ -200,6 +202,56 @@ class CacheManager:
         self.slots.give_back(r.slot)
         return r.slot
 
+    # ---------------------------------------------------------------- forks, compaction
+    def can_fork(self, src_id) -> bool:
+        """Whether a slot and the pages for a copy of the last, partly filled pages are free."""
+        tail = self._req[src_id].length % self.page_size != 0
+        return self.slots.free > 0 and all(p.free >= tail for p in self.pools)
+
+    def fork(self, src_id, new_id):
+        """Make ``new_id`` a second request with ``src_id``'s tokens so far.  Full pages are shared (they are never written again);
+        of the last page, if it is partly filled, the new request gets one of its own.  Returns (source slot, new slot, copies), copies a
+        list per group of (page, its copy): the caller copies the pages' contents and the slots' state.  All or nothing."""
+        if new_id in self._req:
+            raise KeyError(f"request {new_id!r} is already live")
+        r = self._req[src_id]
+        if not self.slots.free:
+            raise OutOfSlots(f"all {self.max_requests} request slots are in use")
+        full, tail = r.length // self.page_size, r.length % self.page_size != 0
+        if any(p.free < tail for p in self.pools):
+            raise OutOfPages(f"a fork of request {src_id!r} needs a page of each group, free {[p.free for p in self.pools]}")
+        f = _Request(self.slots.take_one(), r.length, [], list(r.first_live))
+        copies: List[List[Tuple[int, int]]] = []
+        for g, pool in enumerate(self.pools):
+            table = list(r.tables[g][:full])
+            for p in table:
+                if p >= 0:
+                    pool.share(p)
+            copies.append([])
+            if tail:
+                page = pool.take(1)[0]
+                copies[g].append((r.tables[g][full], page))
+                table.append(page)
+            f.tables.append(table)
+            self.table_rows[g][f.slot, :len(table)] = table
+        self._req[new_id] = f
+        return r.slot, f.slot, copies
+
+    def compact(self) -> List[Dict[int, int]]:
+        """Rename the held pages of every group to its lowest numbers.  Returns the moves per group, old number -> new number; the
+        caller moves the contents before the next step."""
+        moves = []
+        for g, pool in enumerate(self.pools):
+            m = pool.compact()
+            moves.append(m)
+            for r in self._req.values():
+                t = r.tables[g]
+                for j, p in enumerate(t):
+                    if p in m:
+                        t[j] = m[p]
+                        self.table_rows[g][r.slot, j] = m[p]
+        return moves
+
     # ---------------------------------------------------------------- accounting
     def pages_free(self) -> List[int]:
         return [p.free for p in self.pools]
@@ -211,13 +263,18 @@ class CacheManager:
         return [sum(1 for p in t if p >= 0) for t in self._req[req_id].tables]
 
     def check(self) -> None:
-        """Invariants: every page is free or held by exactly one request; same for slots."""
+        """Invariants: every page is free or held by as many requests as its pool counts, by more than one only if it is full in all of
+        them; every slot is free or held by one."""
         for g, pool in enumerate(self.pools):
-            held: List[int] = []
+            held: Dict[int, int] = {}
             for r in self._req.values():
-                held.extend(p for p in r.tables[g] if p >= 0)
-            if len(held) != len(set(held)):
-                raise AssertionError(f"group {g}: a page is held twice")
+                for j, p in enumerate(r.tables[g]):
+                    if p >= 0:
+                        held[p] = held.get(p, 0) + 1
+                        if pool.holders(p) > 1 and (j + 1) * self.page_size > r.length:
+                            raise AssertionError(f"group {g}: page {p} is shared and not full")
+            if any(n != pool.holders(p) for p, n in held.items()):
+                raise AssertionError(f"group {g}: a page is held by more or fewer requests than its pool counts")
             if sorted(held) != pool.held_pages():
                 raise AssertionError(f"group {g}: pages held by requests and by the pool differ")
             if len(held) + pool.free != pool.num_pages:

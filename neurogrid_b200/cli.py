@@ -29,6 +29,8 @@ def build_parser() -> argparse.ArgumentParser:
     a("-write-model", "--write-model", default="", metavar="DIR",
       help="Write config.json and model.safetensors for -config and -random-weights into DIR, then exit")
     a("-dtype", "--dtype", default="bf16", choices=["bf16", "bfloat16", "fp32", "float32"], help="Compute dtype")
+    a("-cache-dtype", "--cache-dtype", default=None, choices=["e4m3", "int8"],
+      help="Hold keys and values of grouped-query attention in 8 bits, with a scale per block of tokens and head (default: the compute dtype)")
     a("-page-size", "--page-size", type=int, default=16, help="Tokens per cache page")
     a("-num-pages", "--num-pages", type=int, default=None, help="Pages in the cache pool (default: from memory)")
     a("-max-requests", "--max-requests", type=int, default=8, help="Requests live at a time")
@@ -71,7 +73,7 @@ def main(argv: Optional[List[str]] = None) -> int:
     eng = Engine(args.model or None, config=config, random_weights=args.random_weights, dtype=args.dtype,
                  gpu=args.gpu, max_seq_len=args.max_seq_len, page_size=args.page_size, num_pages=args.num_pages,
                  max_requests=args.max_requests, max_tokens_per_step=args.max_tokens_per_step,
-                 chunk_size=args.chunk_size)
+                 chunk_size=args.chunk_size, cache_dtype=args.cache_dtype)
     log(f"model ready in {time.time() - t0:.1f} s: {eng.model.spec.architecture}, "
         f"{eng.model.weight_bytes() / 1e6:.1f} MB of weights, {eng.runner.cache.pools[0].num_pages if eng.runner.cache.pools else 0} pages")
     prompts = [[int(x) for x in p.replace(" ", "").split(",") if x] for p in args.prompt_tokens]

@@ -438,7 +438,7 @@ __device__ __forceinline__ void dc_piece(const DcArgs& a, float* red_s, int e, i
             acc = fmaf(rec[4 + d], c, acc);
         }
         const size_t at = (size_t)row * a.nH + head0 + h;
-        float* rec = a.scratch + (at * a.n_splits + run) * REC;
+        float* rec = a.scratch + (((size_t)e * a.nH + head0 + h) * a.n_splits + run) * REC;
         if (runs == 1) {
             a.out[at * HD + d] = __float2bfloat16_rn(l == 0.f ? 0.f : acc / l);
         } else {
@@ -754,11 +754,6 @@ attn_prefill_q8_kernel(const PfArgs a) {
 }
 
 // ===================================================================================== host
-// scratch: n_rows * nH * n_splits * REC floats, 16-byte aligned (unused when n_splits == 1)
-NG_EXPORT long long ng_attn_q8_scratch_floats(int n_rows, int nH, int n_splits) {
-    return n_splits > 1 ? (long long)n_rows * nH * n_splits * REC : 0;
-}
-
 // blocks of the kernel that the current device holds at once (with the most shared memory it may ask for)
 template <typename K>
 static int dc_slots(std::atomic<int>* known, K kernel) {
@@ -776,6 +771,7 @@ static int dc_slots(std::atomic<int>* known, K kernel) {
     return n;
 }
 
+// scratch (n_splits > 1): n_entries * nH * n_splits * REC floats, 16-byte aligned
 NG_EXPORT int ng_attn_decode_q8(const void* q, const void* k_pages, const void* v_pages, const float* k_scales, const float* v_scales,
                                 const int* table, int table_stride, const int* cu_q, const int* ctx_before, void* out, float* scratch,
                                 int n_rows, int n_entries, int nH, int nKV, int hd, int page_size, int block, int num_pages, int kind,
@@ -816,6 +812,7 @@ NG_EXPORT int ng_attn_decode_q8(const void* q, const void* k_pages, const void* 
     return ng_launch_status();
 }
 
+// scratch (n_splits > 1): n_rows * nH * n_splits * REC floats, 16-byte aligned
 NG_EXPORT int ng_attn_prefill_q8(const void* q, const void* k_pages, const void* v_pages, const float* k_scales, const float* v_scales,
                                  const int* table, int table_stride, const int* cu_q, const int* ctx_before, void* out, float* scratch,
                                  int n_rows, int n_entries, int max_q, int nH, int nKV, int hd, int page_size, int block, int num_pages,

@@ -68,7 +68,7 @@ attn_q8_merge_kernel(const float* __restrict__ scratch, const int* __restrict__ 
     scratch = ng_after_wait(scratch);
     constexpr int STEP = WIDE ? MG_WARPS : 1;
     for (int r = q0 + blockIdx.z; r < min(q0 + n, n_rows); r += gridDim.z) {
-        const float* rec = scratch + ((size_t)r * nH + head) * room * REC;
+        const float* rec = scratch + ((size_t)(most == 1 ? e : r) * nH + head) * room * REC;      // (single tokens': by entry)
         // (the first 32 runs' are asked for before it is known how many there are)
         const int s0 = lane * STEP + (WIDE ? warp : 0);
         float m0 = s0 < room ? rec[(size_t)s0 * REC] : -INFINITY, l0 = s0 < room ? rec[(size_t)s0 * REC + 1] : 0.f;

@@ -260,11 +260,12 @@ def rope_pairs(head_dim: int) -> int:
 def rope_cache(qkv: torch.Tensor, q_out: torch.Tensor, q_weight: Optional[torch.Tensor],
                k_weight: Optional[torch.Tensor], inv_freq: Optional[torch.Tensor], half_pairing: bool,
                pos_scale: float, k_pages: Optional[torch.Tensor], v_pages: Optional[torch.Tensor],
-               table: torch.Tensor, positions: torch.Tensor, row_entry: torch.Tensor, n_heads: int,
+               table: Optional[torch.Tensor], positions: torch.Tensor, row_entry: torch.Tensor, n_heads: int,
                n_kv_heads: int, head_dim: int, eps: float, status: torch.Tensor) -> None:
     """Per-head norm of q and k, rotation, q -> q_out[N, nH*hd], k and v -> pages[P, nKV, page, hd].
 
-    ``n_kv_heads`` 0 (with no pages) handles a layer that only reads another layer's cache.
+    ``n_kv_heads`` 0 (with no pages) handles a layer that only reads another layer's cache.  ``table`` None: k and v of row i go to
+    "page" i of one token, k_pages and v_pages [N, nKV, 1, hd] (rows that another kernel takes on).
     """
     n = q_out.shape[0]
     if q_out.shape != (n, n_heads * head_dim):
@@ -277,13 +278,15 @@ def rope_cache(qkv: torch.Tensor, q_out: torch.Tensor, q_weight: Optional[torch.
                 or k_pages.shape[3] != head_dim:
             raise KernelError("rope_cache: pages do not fit the projection")
         num_pages, page_size = k_pages.shape[0], k_pages.shape[2]
+        if table is None and (num_pages < n or page_size != 1):
+            raise KernelError("rope_cache: without a table a row has a page of one token")
     _f32(q_weight, "q norm weight"), _f32(k_weight, "k norm weight"), _f32(inv_freq, "inv_freq")
     _i32(table, "table"), _i32(positions, "positions"), _i32(row_entry, "row_entry"), _i32(status, "status")
     f = _fn("rope_cache", "ng_rope_cache",
             [_c_void_p] * 5 + [_c_int, _c_float] + [_c_void_p] * 3 + [_c_int] + [_c_void_p] * 2 + [_c_int] * 6
             + [_c_float, _c_void_p, _c_int, _c_int, _c_ll, _c_void_p], {"NG_ROPE_PAIRS": rope_pairs(head_dim)})
     _check(f(_ptr(qkv), _ptr(q_out), _ptr(q_weight), _ptr(k_weight), _ptr(inv_freq), int(half_pairing),
-             float(pos_scale), _ptr(k_pages), _ptr(v_pages), _ptr(table), table.shape[1], _ptr(positions),
+             float(pos_scale), _ptr(k_pages), _ptr(v_pages), _ptr(table), table.shape[1] if table is not None else 0, _ptr(positions),
              _ptr(row_entry), n, n_heads, n_kv_heads, head_dim, page_size, num_pages, float(eps), _ptr(status),
              act, n_part, stride, _stream()), "rope_cache")
 
@@ -433,6 +436,17 @@ def attn_decode_prep_bf16(qkv: torch.Tensor, q_weight: Optional[torch.Tensor], k
 
 
 # ----------------------------------------------------------------------------- a cache in 8 bits
+def q8_takes(head_dim: int) -> bool:
+    """Whether the kernels over a cache in 8 bits take heads of this size."""
+    return head_dim % 16 == 0 and 16 <= head_dim <= 256
+
+
+def q8_libraries(head_dim: int):
+    """The libraries that a layer with heads of this size launches over a cache in 8 bits."""
+    jobs = [("cache_q8", None), ("attention_q8", {"NG_HEAD_DIM": head_dim})]
+    return jobs + ([("attention_q8_sm100", {"NG_HEAD_DIM": head_dim})] if head_dim in (64, 128) else [])
+
+
 Q8_KINDS = {torch.float8_e4m3fn: 0, torch.int8: 1}
 
 
@@ -531,7 +545,8 @@ def copy_pages(pools, src, dst) -> None:
 
 
 def attn_q8_scratch_floats(n_rows: int, n_heads: int, head_dim: int, n_splits: int) -> int:
-    """float32 values the attention over a cache in 8 bits needs when it cuts the keys into ``n_splits`` runs."""
+    """float32 values the attention over a cache in 8 bits needs when it cuts the keys into ``n_splits`` runs: of ``n_rows`` rows
+    (portions) or entries (single tokens)."""
     return n_rows * n_heads * n_splits * (head_dim + 4) if n_splits > 1 else 0
 
 
@@ -563,7 +578,7 @@ def attn_prefill_q8_splits(q_lens, n_heads: int, n_kv_heads: int, head_dim: int,
     return max(1, min(slots // max(1, blocks), span // 512, 65535 // max(1, len(q_lens))))
 
 
-def _q8_attention(what, q, out, scratch, cache, cu_q, ctx_before, n_entries, n_heads, n_splits):
+def _q8_attention(what, q, out, scratch, cache, cu_q, ctx_before, n_entries, n_heads, n_splits, n_records):
     kind, num_pages, n_kv, page_size, hd, block = _q8_cache(what, *cache)
     if q.dtype != torch.bfloat16 or out.dtype != torch.bfloat16:
         raise KernelError(f"{what} takes bfloat16 queries")
@@ -573,7 +588,7 @@ def _q8_attention(what, q, out, scratch, cache, cu_q, ctx_before, n_entries, n_h
         raise KernelError(f"{what}: shapes do not fit")
     if n_splits < 1:
         raise KernelError(f"{what}: {n_splits} runs")
-    need = attn_q8_scratch_floats(q.shape[0], n_heads, hd, n_splits)
+    need = attn_q8_scratch_floats(n_records, n_heads, hd, n_splits)
     if need and (scratch is None or scratch.numel() < need or scratch.dtype != torch.float32):
         raise KernelError(f"{what} needs {need} float32 values of scratch")
     _i32(cu_q, "cu_q"), _i32(ctx_before, "ctx_before")
@@ -589,10 +604,10 @@ def attn_decode_q8(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
                    slopes: Optional[torch.Tensor] = None) -> None:
     """``attn_decode_bf16`` over a cache in 8 bits (``cache_write_q8``): split-context attention of the entries that bring one token, any
     number of query heads a KV head.  The rows of other entries stay as they were.  ``n_splits`` (``attn_decode_q8_splits``) runs of
-    the keys; ``scratch`` holds ``attn_q8_scratch_floats`` float32 values when there is more than one."""
+    the keys; ``scratch`` holds ``attn_q8_scratch_floats`` (of ``n_entries``) float32 values when there is more than one."""
     cache = (k_pages, v_pages, k_scales, v_scales, table)
     kind, num_pages, n_kv, page_size, hd, block = _q8_attention("attn_decode_q8", q, out, scratch, cache, cu_q, ctx_before, n_entries,
-                                                                n_heads, n_splits)
+                                                                n_heads, n_splits, n_entries)
     f = _fn("attention_q8", "ng_attn_decode_q8", [_c_void_p] * 6 + [_c_int] + [_c_void_p] * 4 + [_c_int] * 10
             + [_c_float, _c_int, _c_int, _c_void_p, _c_void_p], {"NG_HEAD_DIM": hd})
     _check(f(_ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(k_scales), _ptr(v_scales), _ptr(table), table.shape[1], _ptr(cu_q),
@@ -607,10 +622,10 @@ def attn_prefill_q8(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
                     scratch: Optional[torch.Tensor] = None, n_splits: int = 1) -> None:
     """Flash attention of the step's portions over a cache in 8 bits (``cache_write_q8``); their own keys are read from the cache too.
     Entries of one token are left to ``attn_decode_q8`` when ``skip_single``.  ``n_splits`` (``attn_prefill_q8_splits``) runs of every
-    block's keys, merged through ``scratch`` (``attn_q8_scratch_floats``)."""
+    block's keys, merged through ``scratch`` (``attn_q8_scratch_floats`` of q's rows)."""
     cache = (k_pages, v_pages, k_scales, v_scales, table)
     kind, num_pages, n_kv, page_size, hd, block = _q8_attention("attn_prefill_q8", q, out, scratch, cache, cu_q, ctx_before, n_entries,
-                                                                n_heads, n_splits)
+                                                                n_heads, n_splits, q.shape[0])
     tail = [_ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(k_scales), _ptr(v_scales), _ptr(table), table.shape[1], _ptr(cu_q),
             _ptr(ctx_before), _ptr(out), _ptr(scratch) if n_splits > 1 else None, q.shape[0], n_entries, int(max_q), n_heads, n_kv, hd,
             page_size, block, num_pages, kind, int(window or 0), float(scale), int(bool(skip_single)), int(n_splits),

@@ -92,7 +92,7 @@ rope_cache_kernel(const TI* __restrict__ qkv, T* __restrict__ q_out, const float
     size_t page_base = 0;
     bool page_ok = true;
     if (nKV > 0) {
-        const int page = table[(size_t)entry * table_stride + pos / page_size];
+        const int page = table ? table[(size_t)entry * table_stride + pos / page_size] : row;      // (no table: a page of one token a row)
         page_ok = page >= 0 && page < num_pages;
         page_base = (size_t)(page_ok ? page : 0) * nKV * page_size * hd + (size_t)(pos % page_size) * hd;
     }
@@ -205,7 +205,7 @@ rope_cache_half64_kernel(const __nv_bfloat16* __restrict__ qkv, __nv_bfloat16* _
     size_t page_base = 0;
     bool page_ok = true;
     if (nKV > 0) {
-        const int page = table[(size_t)entry * table_stride + pos / page_size];
+        const int page = table ? table[(size_t)entry * table_stride + pos / page_size] : row;      // (no table: a page of one token a row)
         page_ok = page >= 0 && page < num_pages;
         if (!page_ok && threadIdx.x == 0 && blockIdx.y == 0) atomicOr(status, NG_STATUS_BAD_PAGE);
         page_base = (size_t)(page_ok ? page : 0) * nKV * page_size * hd + (size_t)(pos % page_size) * hd;

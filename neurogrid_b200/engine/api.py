@@ -24,13 +24,15 @@ class Engine:
                  random_weights: Optional[int] = None, dtype="bfloat16", gpu: int = 0,
                  max_seq_len: int = 4096, page_size: int = 16, num_pages: Optional[int] = None,
                  max_requests: int = 8, max_tokens_per_step: int = 2048, chunk_size: Optional[int] = None,
-                 cache_memory_fraction: float = 0.25, pipeline: bool = True):
+                 cache_memory_fraction: float = 0.25, pipeline: bool = True, cache_dtype: Optional[str] = None):
         """``model``: folder with config.json and safetensors.  Without it, ``config`` (the
         config.json mapping) and ``random_weights`` (a seed) build a model with random weights
         on the device.  ``max_seq_len`` caps the model's max_position_embeddings (as the
         reference's flag does).  ``num_pages`` defaults to room for ``max_requests`` full
         contexts, limited to ``cache_memory_fraction`` of the free device memory (the reference
-        sizes its pool to 25% of free VRAM, pkg/inference/engine_gpu.go:224-243)."""
+        sizes its pool to 25% of free VRAM, pkg/inference/engine_gpu.go:224-243).  ``cache_dtype``: "e4m3" or "int8" holds the
+        keys and values of grouped-query attention in 8 bits (half the memory and, in decoding, half the traffic of bfloat16;
+        a value is off by at most 2^-4 of itself (e4m3) or half a step of its block's scale (int8))."""
         self.device = require_cuda(f"cuda:{gpu}")
         self.dtype = parse_dtype(dtype)
         if model is not None:
@@ -43,7 +45,7 @@ class Engine:
         self.max_seq_len = min(int(max_seq_len), spec.max_positions) if spec.max_positions else int(max_seq_len)
         if num_pages is None:
             num_pages = max_requests * -(-self.max_seq_len // page_size)
-            probe = ModelRunner.bytes_per_page(self.model, page_size)
+            probe = ModelRunner.bytes_per_page(self.model, page_size, cache_dtype)
             if probe:
                 # the eager workspace and the one the portion graphs keep are allocated at the first
                 # steps, after the pool: leave them their room
@@ -53,7 +55,7 @@ class Engine:
                 num_pages = max(1, min(num_pages, int(max(0, free - reserve) * cache_memory_fraction) // probe))
         self.runner = ModelRunner(self.model, num_pages=num_pages, page_size=page_size,
                                   max_requests=max_requests, max_seq_len=self.max_seq_len,
-                                  max_tokens_per_step=max_tokens_per_step)
+                                  max_tokens_per_step=max_tokens_per_step, cache_dtype=cache_dtype)
         self.scheduler = Scheduler(self.runner.cache, max_tokens_per_step=max_tokens_per_step,
                                    max_requests=max_requests, chunk_size=chunk_size,
                                    eos_token_ids=spec.eos_token_ids)
@@ -74,6 +76,25 @@ class Engine:
         if request_id is None:
             request_id = self._next_id
             self._next_id += 1
+        req = self._request(prompt, params, request_id, rng_key)
+        self._requests[request_id] = req
+        self.scheduler.add(req)
+        return request_id
+
+    def add_samples(self, prompt: Sequence[int], n: int, params: Optional[SamplingParams] = None,
+                    rng_keys: Optional[Sequence[int]] = None) -> List[Hashable]:
+        """Queue ``n`` requests for the same prompt, each with a random stream of its own.  The prompt is read once; the others start
+        from copies of its state and share the pages that it has filled."""
+        if n < 1 or (rng_keys is not None and len(rng_keys) != n):
+            raise ValueError("n is at least 1, with a random stream for each sample or for none")
+        ids = list(range(self._next_id, self._next_id + n))
+        reqs = [self._request(prompt, params, i, rng_keys[j] if rng_keys is not None else None) for j, i in enumerate(ids)]
+        self._next_id += n
+        self._requests.update(zip(ids, reqs))
+        self.scheduler.add_samples(reqs[0], reqs[1:])
+        return ids
+
+    def _request(self, prompt, params, request_id, rng_key) -> Request:
         if request_id in self._requests:
             raise KeyError(f"request id {request_id!r} is in use")
         V = self.model.spec.vocab_size
@@ -83,10 +104,7 @@ class Engine:
                 raise ValueError(f"prompt token {t} is outside the vocabulary (0..{V - 1})")
         if len(prompt) >= self.max_seq_len:
             raise ValueError(f"prompt of {len(prompt)} tokens leaves no room in a context of {self.max_seq_len}")
-        req = Request(request_id, prompt, params or SamplingParams(), key=rng_key)
-        self._requests[request_id] = req
-        self.scheduler.add(req)
-        return request_id
+        return Request(request_id, prompt, params or SamplingParams(), key=rng_key)
 
     def step(self) -> List[Request]:
         """One turn of the loop; returns the requests that finished in it.
@@ -99,6 +117,8 @@ class Engine:
         if self._inflight is None:
             plan = self.scheduler.plan()
             done += plan.failed
+            for f in plan.forks:
+                self.runner.copy_fork(*f)
             if not plan.entries:
                 return done
             rec = self._launch(plan, None)
@@ -160,18 +180,19 @@ class Engine:
 
     def generate(self, prompts: Sequence[Sequence[int]], *, max_new_tokens: int = 16, temperature: float = 0.0,
                  top_p: float = 1.0, seed: int = DEFAULT_SEED, stop_token_ids: Sequence[int] = (),
-                 ignore_eos: bool = False) -> List[List[int]]:
-        """Generated token ids for each prompt (prompt not included), in the order given."""
+                 ignore_eos: bool = False, n: int = 1) -> List[List[int]]:
+        """Generated token ids for each prompt (prompt not included), in the order given.  ``n`` > 1: a list of that many
+        samples for each prompt, which is read once for all of them."""
         params = SamplingParams(temperature=temperature, top_p=top_p, max_new_tokens=max_new_tokens, seed=seed,
                                 stop_token_ids=tuple(stop_token_ids), ignore_eos=ignore_eos)
-        ids = [self.add_request(p, params, rng_key=i) for i, p in enumerate(prompts)]
+        ids = [i for k, p in enumerate(prompts) for i in self.add_samples(p, n, params, range(k * n, k * n + n))]
         self.run()
         self.runner.check_status()
         out = [self._requests[i].output for i in ids]
         self.last_finish_reasons = [self._requests[i].finish_reason for i in ids]
         for i in ids:
             del self._requests[i]
-        return out
+        return out if n == 1 else [out[i:i + n] for i in range(0, len(out), n)]
 
     def stats(self) -> Dict[str, object]:
         s = self.runner.stats()

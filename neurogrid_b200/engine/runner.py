@@ -20,9 +20,9 @@ from typing import Dict, Hashable, List, Optional, Sequence
 import numpy as np
 import torch
 
-from ..cache.manager import CacheManager
+from ..cache.manager import CacheManager, PagedNeed
 from ..cache.pages import OutOfPages
-from ..cache.storage import CacheStorage
+from ..cache.storage import CacheStorage, page_bytes, parse_cache_dtype
 from ..parts.base import PagedView, SlotView, StepContext, Workspace
 
 
@@ -51,7 +51,10 @@ class ModelRunner:
     MAX_PORTION_LOGITS_BYTES = 64 << 20   # ... and for this much of logits (a portion that wants more rows runs eagerly)
 
     def __init__(self, model, *, num_pages, page_size: int = 16, max_requests: int = 8,
-                 max_seq_len: Optional[int] = None, max_tokens_per_step: int = 2048, cuda_graphs: bool = True):
+                 max_seq_len: Optional[int] = None, max_tokens_per_step: int = 2048, cuda_graphs: bool = True,
+                 cache_dtype: Optional[str] = None):
+        """``cache_dtype``: "e4m3" or "int8" holds keys and values in 8 bits, with a scale for each block of tokens and head, in the
+        layers that can (grouped-query attention of a bfloat16 model); None: in the compute dtype."""
         self.model = model
         self.device, self.dtype = model.device, model.dtype
         spec = model.spec
@@ -59,8 +62,15 @@ class ModelRunner:
         self.max_seq_len = int(max_seq_len or spec.max_positions or num_pages * page_size)
         self.max_tokens_per_step = int(max_tokens_per_step)
         self.max_requests = int(max_requests)
-        self.storage = CacheStorage(model.cache_needs(), pages_per_group=num_pages, page_size=page_size,
-                                    max_requests=max_requests, dtype=self.dtype, device=self.device)
+        self.cache_dtype = parse_cache_dtype(cache_dtype)
+        needs = model.cache_needs()
+        if self.cache_dtype is not None:
+            if self.dtype != torch.bfloat16:
+                raise ValueError("a cache in 8 bits goes with bfloat16 compute")
+            if not any(n.eight_bit for n in self._paged(needs)):
+                raise ValueError("no layer of this model keeps keys and values that can be held in 8 bits")
+        self.storage = CacheStorage(needs, pages_per_group=num_pages, page_size=page_size, max_requests=max_requests,
+                                    dtype=self.dtype, device=self.device, cache_dtype=self.cache_dtype)
         self.cache = CacheManager(self.storage.paged_needs, self.storage.pages_per_group, page_size,
                                   max_requests, self.max_seq_len)
         self.ws = Workspace(self.max_tokens_per_step, self.device)
@@ -74,8 +84,9 @@ class ModelRunner:
         if self._on_cuda:
             # compile (side by side) what this model launches, rather than one library at a time
             # when the first step first meets each kernel
-            from ..csrc import build, kernel_sets
-            build.compile_many(kernel_sets.needed_by(model))
+            from ..csrc import build, kernel_sets, ops
+            heads = {n.head_dim for n in self.storage.paged_needs if n.eight_bit and self.cache_dtype is not None}
+            build.compile_many(kernel_sets.unique(kernel_sets.needed_by(model) + [j for d in sorted(heads) for j in ops.q8_libraries(d)]))
         # the batch description is staged in pinned host buffers used in turn; a buffer is
         # written again only after the copy that last read it has finished
         self._ring = [torch.zeros(cap, dtype=torch.int32, pin_memory=self._on_cuda) for _ in range(4)]
@@ -115,12 +126,15 @@ class ModelRunner:
         self.keep_graphs = False       # keep the captured graphs beside their executables (for `graph_kernel_nodes`)
 
     @staticmethod
-    def bytes_per_page(model, page_size: int) -> int:
+    def _paged(needs):
+        flat = [n for need in needs.values() for n in (need if isinstance(need, tuple) else (need,))]
+        return [n for n in flat if isinstance(n, PagedNeed)]
+
+    @classmethod
+    def bytes_per_page(cls, model, page_size: int, cache_dtype: Optional[str] = None) -> int:
         """Device bytes one page id costs over all paged layers (keys and values)."""
-        from ..cache.manager import PagedNeed
-        esz = torch.empty((), dtype=model.dtype).element_size()
-        flat = [n for need in model.cache_needs().values() for n in (need if isinstance(need, tuple) else (need,))]
-        return sum(n.elements_per_token() * page_size * esz for n in flat if isinstance(n, PagedNeed))
+        cache_dtype = parse_cache_dtype(cache_dtype)
+        return sum(page_bytes(n, page_size, model.dtype, cache_dtype) for n in cls._paged(model.cache_needs()))
 
     # ------------------------------------------------------------------ requests
     def admit(self, req_id: Hashable) -> int:
@@ -132,6 +146,30 @@ class ModelRunner:
         """Give back the request's pages and slot."""
         if self.cache.is_live(req_id):
             self.cache.release(req_id)
+
+    def fork(self, src_id: Hashable, new_id: Hashable) -> None:
+        """Start ``new_id`` with everything ``src_id`` has in the cache: full pages are shared, the last, partly filled page and the
+        state are copied (on the current stream, behind the steps that were launched before)."""
+        self.copy_fork(*self.cache.fork(src_id, new_id))
+
+    def copy_fork(self, src_slot: int, new_slot: int, copies) -> None:
+        """The device's part of a fork that the cache manager has made."""
+        from ..csrc import ops
+        for g, pairs in enumerate(copies):
+            if pairs:
+                ops.copy_pages(self.storage.pools(g), [a for a, _ in pairs], [b for _, b in pairs])
+        self.storage.copy_slot(src_slot, new_slot)
+
+    def compact(self) -> int:
+        """Move the pages that requests hold to the front of their pools (a pool's pages from ``num_pages - free`` on are then all
+        free).  Returns the number of pages moved."""
+        from ..csrc import ops
+        moved = 0
+        for g, moves in enumerate(self.cache.compact()):
+            if moves:
+                ops.copy_pages(self.storage.pools(g), list(moves), list(moves.values()))
+                moved += len(moves)
+        return moved
 
     # ------------------------------------------------------------------ the step
     def step(self, entries: Sequence[StepEntry], token_feed=None, greedy_into: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
@@ -612,8 +650,10 @@ class ModelRunner:
         def view(lc, writes):
             if lc.kind == "paged":
                 v = st.v[lc.group]
+                ks, vs = st.k_scales[lc.group], st.v_scales[lc.group]
                 return PagedView(st.k[lc.group][lc.index], v[lc.index] if v is not None else None,
-                                 self._tables[lc.group], writes=writes)
+                                 self._tables[lc.group], writes=writes, k_scales=ks[lc.index] if ks is not None else None,
+                                 v_scales=vs[lc.index] if vs is not None else None)
             if lc.kind == "slot":
                 return SlotView(st.state[lc.group][lc.index])
             return None

@@ -41,6 +41,7 @@ class Request:
     state: str = WAITING
     finish_reason: Optional[str] = None
     preemptions: int = 0
+    forks: List["Request"] = field(default_factory=list)   # more samples of the same prompt, which wait until all but its last token is read
 
     @property
     def tokens(self) -> List[int]:
@@ -65,6 +66,7 @@ class StepPlan:
     entries: List[PlannedEntry] = field(default_factory=list)
     preempted: List[Request] = field(default_factory=list)
     failed: List[Request] = field(default_factory=list)
+    forks: list = field(default_factory=list)     # (source slot, new slot, copies) of requests forked in front of the step
 
     @property
     def n_tokens(self) -> int:
@@ -95,6 +97,39 @@ class Scheduler:
         self._next_key += 1
         req.state = WAITING
         self.waiting.append(req)
+
+    def add_samples(self, req: Request, more: Sequence[Request]) -> None:
+        """Queue ``req`` and further samples of its prompt.  The prompt is read once, up to its last token; then the others are forked
+        off, each with the pages of what was read (they read the prompt themselves where no slot or page is free for that)."""
+        self.add(req)
+        for r in more:
+            if len(req.prompt) < 2:
+                self.add(r)
+                continue
+            if r.key is None:
+                r.key = self._next_key
+            self._next_key += 1
+            r.state = WAITING
+            req.forks.append(r)
+
+    def _fork(self, plan: StepPlan) -> None:
+        """Fork the requests whose prompt has been read up to its last token."""
+        for req in list(self.running):
+            if not req.forks or req.fed < len(req.prompt) - 1:
+                continue
+            for r in req.forks:
+                if len(self.running) < self.max_requests and self.cache.can_fork(req.id):
+                    plan.forks.append(self.cache.fork(req.id, r.id))
+                    r.fed, r.state = req.fed, RUNNING
+                    self.running.append(r)
+                else:
+                    self.waiting.append(r)
+            req.forks = []
+
+    def _portion(self, req: Request, most: int) -> int:
+        """Tokens of the request's next portion: a prompt that others wait for is read up to its last token first."""
+        n = min(req.pending, most, self.chunk_size)
+        return min(n, len(req.prompt) - 1 - req.fed) if req.forks else n
 
     def has_work(self) -> bool:
         return bool(self.waiting or self.running)
@@ -128,6 +163,7 @@ class Scheduler:
         """Decide the next step.  Preempted requests have already been released and re-queued,
         failed ones released and marked finished, when this returns."""
         plan = StepPlan()
+        self._fork(plan)
         while True:
             plan.entries = []
             free = list(self.cache.pages_free())
@@ -136,7 +172,7 @@ class Scheduler:
             for req in self.running:
                 if budget == 0:
                     break
-                want = min(req.pending, budget, self.chunk_size)
+                want = self._portion(req, budget)
                 if not self.cache.windowed and self.cache.is_live(req.id) and want <= self.cache.slack(req.id):
                     n = want                                 # fits in the pages it holds: nothing to charge
                 else:
@@ -171,7 +207,7 @@ class Scheduler:
                         plan.failed.append(req)
                         continue
                     break
-                n = min(req.pending, budget, self.chunk_size)
+                n = self._portion(req, budget)
                 self.waiting.popleft()
                 req.state = RUNNING
                 self.running.append(req)
@@ -196,6 +232,9 @@ class Scheduler:
         if self.cache.is_live(req.id):
             self.cache.release(req.id)
         req.state, req.finish_reason = FINISHED, reason
+        for r in req.forks:                                      # (they would fail for the same reason)
+            r.state, r.finish_reason = FINISHED, reason
+        req.forks = []
 
     # ------------------------------------------------------------------ one step ahead
     def commit_ahead(self, plan: StepPlan) -> None:

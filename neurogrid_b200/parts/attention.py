@@ -66,7 +66,7 @@ class Attention:
                 self.k_norm = t[f"{n['k_norm']}.weight"].to(**f32).contiguous()
 
     def cache_need(self):
-        return PagedNeed(self.spec.n_kv_heads, self.spec.head_dim, self.spec.window)
+        return PagedNeed(self.spec.n_kv_heads, self.spec.head_dim, self.spec.window, eight_bit=ops.q8_takes(self.spec.head_dim))
 
     def scratch_bytes_per_row(self):
         """Workspace per row of a step besides the products' outputs: the records of the portion kernel's runs."""
@@ -109,6 +109,19 @@ class Attention:
             qkv_q.copy_(qkv[:, : s.n_heads * s.head_dim])
             qkv, n_kv = qkv_q, 0
         a = ctx.ws.buf("attn_out", n, s.n_heads * s.head_dim, self.dtype)
+        if cache.k_scales is not None:
+            # pages of codes: the rotated keys, and the values, as rows; then a block of tokens' codes and scale at a time
+            rows = [None, None]
+            if n_kv:
+                rows = [ctx.ws.buf(name, n, n_kv * s.head_dim, self.dtype) for name in ("attn_k_rows", "attn_v_rows")]
+            k_rows, v_rows = (r.view(n, n_kv, 1, s.head_dim) if r is not None else None for r in rows)
+            ops.rope_cache(qkv, q, self.q_norm, self.k_norm, inv_freq, half, pos_scale, k_rows, v_rows, None,
+                           ctx.positions, ctx.row_entry, s.n_heads, n_kv, s.head_dim, s.qk_norm_eps, ctx.status)
+            if n_kv:
+                ops.cache_write_q8(*rows, cache.k_pages, cache.v_pages, cache.k_scales, cache.v_scales, cache.table,
+                                   ctx.row_entry, ctx.cu_q, ctx.ctx_before, ctx.status)
+            self.attend_q8(q, cache, ctx, a, pa.score_slopes)
+            return ops.linear_to_residual(a, self.w_o, self.b_o, ctx.ws, "mixer_out", residual=ctx.residual)
         plan = self._decode_plan(cache, ctx, n) if n_kv and self._one_launch(ctx) else None
         if plan is not None and ctx.n_entries * n_kv * plan[1] <= sm_count(self.device):
             # single tokens in few blocks: the attention prepares its rows itself
@@ -161,6 +174,39 @@ class Attention:
             ops.attn_decode_bf16(q, cache.k_pages, cache.v_pages, cache.table, ctx.cu_q, ctx.ctx_before, out,
                                  scratch, ctx.n_entries, s.n_heads, s.window, self.scale, n_splits, max_ctx, slopes)
 
+    def attend_q8(self, q, cache, ctx, out, slopes=None):
+        """``attend`` over pages of 8-bit codes."""
+        s = self.spec
+        pages = (cache.k_pages, cache.v_pages, cache.k_scales, cache.v_scales, cache.table)
+        singles = [c + 1 for c, n in zip(ctx.ctx_lens, ctx.q_lens) if n == 1]
+        multi = [n for n in ctx.q_lens if n > 1]
+        if ctx.fixed_launches:                       # a graph that serves every mix of its size: both kernels, always
+            multi, singles = [ctx.max_q] if ctx.max_q > 1 else [], singles or [1]
+
+        def scratch_for(records, n_splits):
+            """The runs' records; a workspace of fixed addresses holds as many as any step of it asks for."""
+            floats = ops.attn_q8_scratch_floats(records, s.n_heads, s.head_dim, n_splits)
+            if not floats and not ctx.ws.fixed:
+                return None
+            return ctx.ws.flat("attn_q8_scratch", floats, torch.float32, reserve=Q8_SCRATCH_FLOATS)
+
+        if multi:
+            if ctx.prefill_ctx:                      # a graph for a class of steps: planned for one portion of max_q rows
+                span, lens = ctx.prefill_ctx, [ctx.max_q]
+            else:
+                span, lens = max(c + n for c, n in zip(ctx.ctx_lens, ctx.q_lens) if n > 1), multi
+            n_splits = ops.attn_prefill_q8_splits(lens, s.n_heads, s.n_kv_heads, s.head_dim, span, s.window, self.device)
+            n_splits = max(1, min(n_splits, Q8_SCRATCH_FLOATS // ops.attn_q8_scratch_floats(q.shape[0], s.n_heads, s.head_dim, 2) * 2))
+            ops.attn_prefill_q8(q, *pages, ctx.cu_q, ctx.ctx_before, out, ctx.n_entries, ctx.max_q, s.n_heads, s.window, self.scale,
+                                bool(singles), slopes, scratch_for(q.shape[0], n_splits), n_splits)
+        if singles:
+            max_ctx = ctx.decode_max_ctx or max(singles)
+            n_splits = ops.attn_decode_q8_splits(ctx.decode_batch or len(singles), s.n_heads, s.n_kv_heads, s.head_dim, max_ctx,
+                                                 s.window, self.device)
+            n_splits = max(1, min(n_splits, Q8_SCRATCH_FLOATS // ops.attn_q8_scratch_floats(ctx.n_entries, s.n_heads, s.head_dim, 2) * 2))
+            ops.attn_decode_q8(q, *pages, ctx.cu_q, ctx.ctx_before, out, scratch_for(ctx.n_entries, n_splits), ctx.n_entries, s.n_heads,
+                               s.window, self.scale, n_splits, max_ctx, slopes)
+
     def _one_launch(self, ctx):
         """Whether the step is single tokens alone, in bfloat16, with heads that the decode kernel takes: then one launch may
         prepare the rows and attend.  It is the faster, or as fast, where no SM has two of its blocks (every block prepares its
@@ -205,6 +251,7 @@ def sm_count(device) -> int:
     return _SM_COUNT[key]
 
 
+Q8_SCRATCH_FLOATS = 16 << 20        # 64 MB: records of the runs over a cache in 8 bits (64 rows x 32 heads x 16 runs of 64: 2.2 M floats)
 PREFILL_MAX_SPLITS = 4
 PREFILL_SPLIT_MIN_CTX = 8192        # keys a portion sees before its blocks are worth cutting (the merge costs a pass)
 

@@ -111,6 +111,8 @@ class PagedView:
     v_pages: Optional[torch.Tensor]      # None for pages without a value half
     table: torch.Tensor
     writes: bool = True          # False: this run of the layer reads another layer's cache
+    k_scales: Optional[torch.Tensor] = None      # float32 [pages, n_kv_heads, page_size / block]: the pages then hold 8-bit codes,
+    v_scales: Optional[torch.Tensor] = None      # a code c standing for c * its block's scale
 
 
 @dataclass

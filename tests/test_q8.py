@@ -68,7 +68,7 @@ def attend(fn, q=None, out=None, c=None, heads=4, splits=1, scratch=None, n=2, c
     (dict(heads=3, q=torch.zeros(3, 96, dtype=torch.bfloat16)), "shapes"),
     (dict(c=cache(hd=272), q=torch.zeros(3, 4 * 272, dtype=torch.bfloat16)), "above 256"),
     (dict(splits=2), "scratch"),
-    (dict(splits=2, scratch=torch.zeros(3 * 4 * 2 * 36 - 1)), "scratch"),
+    (dict(splits=2, scratch=torch.zeros(2 * 4 * 2 * 36 - 1)), "scratch"),
     (dict(splits=2, scratch=torch.zeros(10000, dtype=torch.float64)), "scratch"),
     (dict(splits=0), "runs"),
     (dict(n=3), "batch description"),
