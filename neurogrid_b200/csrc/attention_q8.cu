@@ -771,25 +771,21 @@ static int dc_slots(std::atomic<int>* known, K kernel) {
     return n;
 }
 
-// scratch (n_splits > 1): n_entries * nH * n_splits * REC floats, 16-byte aligned
-NG_EXPORT int ng_attn_decode_q8(const void* q, const void* k_pages, const void* v_pages, const float* k_scales, const float* v_scales,
-                                const int* table, int table_stride, const int* cu_q, const int* ctx_before, void* out, float* scratch,
-                                int n_rows, int n_entries, int nH, int nKV, int hd, int page_size, int block, int num_pages, int kind,
-                                int window, float scale, int n_splits, int max_ctx, const float* slopes, cudaStream_t stream) {
-    if (n_entries <= 0 || n_rows <= 0) return NG_OK;
+// scratch (n_splits > 1): n_entries * n_heads * n_splits * REC floats, 16-byte aligned
+NG_EXPORT int ng_attn_decode_q8(const NgAttnQ8* call, cudaStream_t stream) {
+    const NgAttnQ8& c = *call;
+    const int n_entries = c.n_entries, nKV = c.n_kv, nH = c.n_heads, n_splits = c.n_splits, kind = c.kind, block = c.block;
+    if (n_entries <= 0 || c.n_rows <= 0) return NG_OK;
     DcArgs a;
-    if (hd != HD || nH <= 0 || !cache_of(a.c, k_pages, v_pages, k_scales, v_scales, table, table_stride, nKV, page_size, block, num_pages) ||
-        nH % nKV || n_splits < 1 || n_splits > 65535 || n_entries > 65535 || (n_splits > 1 && (!scratch || ((uintptr_t)scratch & 15))) ||
-        max_ctx < 0 || window < 0 || ((uintptr_t)q & 7) || ((uintptr_t)out & 3) || (kind != NG_Q8_E4M3 && kind != NG_Q8_INT8))
-        return NG_BAD_SIZE;
+    if (!attn_q8_args(c, a.c) || n_splits > 65535 || n_entries > 65535 || ((uintptr_t)c.q & 7) || ((uintptr_t)c.out & 3)) return NG_BAD_SIZE;
     const int G = nH / nKV;
-    a.q = (const bf16*)q; a.cu_q = cu_q; a.ctx_before = ctx_before; a.out = (bf16*)out; a.scratch = scratch; a.slopes = slopes;
-    a.n_rows = n_rows; a.n_entries = n_entries; a.nH = nH; a.window = window; a.n_splits = n_splits; a.scale = scale;
+    a.q = (const bf16*)c.q; a.cu_q = c.cu_q; a.ctx_before = c.ctx_before; a.out = (bf16*)c.out; a.scratch = c.scratch; a.slopes = c.slopes;
+    a.n_rows = c.n_rows; a.n_entries = n_entries; a.nH = nH; a.window = c.window; a.n_splits = n_splits; a.scale = c.scale;
     const int nt = G > 8 ? DC_NT_MAX : 1;
     a.chunks = (G + 8 * nt - 1) / (8 * nt);
     const int segments = nKV * a.chunks;
     // blocks, and all turns rounded up to whole shares, are counted in 31 bits
-    if ((long long)nKV * a.chunks * n_entries > 0x7fffffff || n_entries * (((long long)table_stride * page_size / TURN + 2) * 2) > 0x7fffffff)
+    if ((long long)nKV * a.chunks * n_entries > 0x7fffffff || n_entries * (((long long)c.table_stride * c.page_size / TURN + 2) * 2) > 0x7fffffff)
         return NG_BAD_SIZE;
 #define DC_GO(KIND, NT, GRAN)                                                                                                         \
     do {                                                                                                                              \
@@ -808,26 +804,22 @@ NG_EXPORT int ng_attn_decode_q8(const void* q, const void* k_pages, const void* 
     else if (nt == 1) DC_KINDS(1, 8);
     else if (block >= 16) DC_KINDS(DC_NT_MAX, 16);
     else DC_KINDS(DC_NT_MAX, 8);
-    if (n_splits > 1) return q8_merge(scratch, cu_q, out, nH, n_splits, n_rows, n_entries, 1, 1, 1, stream);
+    if (n_splits > 1) return q8_merge(c.scratch, c.cu_q, c.out, nH, n_splits, c.n_rows, n_entries, 1, 1, 1, stream);
     return ng_launch_status();
 }
 
-// scratch (n_splits > 1): n_rows * nH * n_splits * REC floats, 16-byte aligned
-NG_EXPORT int ng_attn_prefill_q8(const void* q, const void* k_pages, const void* v_pages, const float* k_scales, const float* v_scales,
-                                 const int* table, int table_stride, const int* cu_q, const int* ctx_before, void* out, float* scratch,
-                                 int n_rows, int n_entries, int max_q, int nH, int nKV, int hd, int page_size, int block, int num_pages,
-                                 int kind, int window, float scale, int skip_single, int n_splits, const float* slopes, cudaStream_t stream) {
-    if (n_entries <= 0 || n_rows <= 0 || max_q <= 0) return NG_OK;
+// scratch (n_splits > 1): n_rows * n_heads * n_splits * REC floats, 16-byte aligned
+NG_EXPORT int ng_attn_prefill_q8(const NgAttnQ8* call, cudaStream_t stream) {
+    const NgAttnQ8& c = *call;
+    const int kind = c.kind;
+    if (c.n_entries <= 0 || c.n_rows <= 0 || c.max_q <= 0) return NG_OK;
     PfArgs a;
-    if (hd != HD || nH <= 0 || !cache_of(a.c, k_pages, v_pages, k_scales, v_scales, table, table_stride, nKV, page_size, block, num_pages) ||
-        nH % nKV || n_splits < 1 || (long long)n_entries * n_splits > 65535 || (n_splits > 1 && (!scratch || ((uintptr_t)scratch & 15))) ||
-        window < 0 || ((uintptr_t)q & 3) || ((uintptr_t)out & 3) || (kind != NG_Q8_E4M3 && kind != NG_Q8_INT8))
-        return NG_BAD_SIZE;
-    const long long rows = (long long)max_q * (nH / nKV), tiles = (rows + PF_ROWS - 1) / PF_ROWS;
+    if (!attn_q8_args(c, a.c) || (long long)c.n_entries * c.n_splits > 65535 || (((uintptr_t)c.q | (uintptr_t)c.out) & 3)) return NG_BAD_SIZE;
+    const long long tiles = ((long long)c.max_q * (c.n_heads / c.n_kv) + PF_ROWS - 1) / PF_ROWS;
     if (tiles > 65535) return NG_BAD_SIZE;
-    a.q = (const bf16*)q; a.cu_q = cu_q; a.ctx_before = ctx_before; a.out = (bf16*)out; a.scratch = scratch; a.slopes = slopes;
-    a.n_rows = n_rows; a.nH = nH; a.window = window; a.n_splits = n_splits; a.skip_single = skip_single; a.scale = scale;
-    const dim3 grid(nKV, (unsigned)tiles, n_entries * n_splits);
+    a.q = (const bf16*)c.q; a.cu_q = c.cu_q; a.ctx_before = c.ctx_before; a.out = (bf16*)c.out; a.scratch = c.scratch; a.slopes = c.slopes;
+    a.n_rows = c.n_rows; a.nH = c.n_heads; a.window = c.window; a.n_splits = c.n_splits; a.skip_single = c.skip_single; a.scale = c.scale;
+    const dim3 grid(c.n_kv, (unsigned)tiles, c.n_entries * c.n_splits);
 #define PF_GO(KIND)                                                                                                  \
     do {                                                                                                             \
         static std::atomic<unsigned long long> once{0};                                                              \
@@ -836,6 +828,7 @@ NG_EXPORT int ng_attn_prefill_q8(const void* q, const void* k_pages, const void*
     } while (0)
     if (kind == NG_Q8_E4M3) PF_GO(NG_Q8_E4M3);
     else PF_GO(NG_Q8_INT8);
-    if (n_splits > 1) return q8_merge(scratch, cu_q, out, nH, n_splits, n_rows, n_entries, skip_single ? 2 : 1, 0x7fffffff, max_q, stream);
+    if (c.n_splits > 1)
+        return q8_merge(c.scratch, c.cu_q, c.out, c.n_heads, c.n_splits, c.n_rows, c.n_entries, c.skip_single ? 2 : 1, 0x7fffffff, c.max_q, stream);
     return ng_launch_status();
 }

@@ -455,22 +455,21 @@ attn_prefill_q8_sm100_kernel(const Params p) {
     if (warp == 7) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 256;" :: "r"(tmem) : "memory");
 }
 
-NG_EXPORT int ng_attn_prefill_q8_sm100(const void* q, const void* k_pages, const void* v_pages, const float* k_scales, const float* v_scales,
-                                       const int* table, int table_stride, const int* cu_q, const int* ctx_before, void* out, float* scratch,
-                                       int n_rows, int n_entries, int max_q, int nH, int nKV, int hd, int page_size, int block, int num_pages,
-                                       int kind, int window, float scale, int skip_single, int n_splits, const float* slopes, int* status,
-                                       cudaStream_t stream) {
-    if (n_entries <= 0 || n_rows <= 0 || max_q <= 0) return NG_OK;
+// scratch (n_splits > 1): n_rows * n_heads * n_splits * REC floats, 16-byte aligned
+NG_EXPORT int ng_attn_prefill_q8_sm100(const NgAttnQ8* call, cudaStream_t stream) {
+    const NgAttnQ8& c = *call;
+    const int kind = c.kind;
+    if (c.n_entries <= 0 || c.n_rows <= 0 || c.max_q <= 0) return NG_OK;
     Params p;
-    if (hd != HD || nH <= 0 || !cache_of(p.c, k_pages, v_pages, k_scales, v_scales, table, table_stride, nKV, page_size, block, num_pages) ||
-        nH % nKV || n_splits < 1 || (long long)n_entries * n_splits > 65535 || (n_splits > 1 && (!scratch || ((uintptr_t)scratch & 15))) ||
-        window < 0 || !(scale > 0.f) || ((uintptr_t)q & 15) || ((uintptr_t)out & 15) || (kind != NG_Q8_E4M3 && kind != NG_Q8_INT8) || !status)
+    if (!attn_q8_args(c, p.c) || (long long)c.n_entries * c.n_splits > 65535 || !(c.scale > 0.f) || !c.status ||
+        (((uintptr_t)c.q | (uintptr_t)c.out) & 15))
         return NG_BAD_SIZE;
-    const long long tiles = ((long long)max_q * (nH / nKV) + BQ - 1) / BQ;
+    const long long tiles = ((long long)c.max_q * (c.n_heads / c.n_kv) + BQ - 1) / BQ;
     if (tiles > 65535) return NG_BAD_SIZE;
-    p.q = (const bf16*)q; p.out = (bf16*)out; p.cu_q = cu_q; p.ctx_before = ctx_before; p.status = status; p.n_rows = n_rows; p.nH = nH;
-    p.window = window; p.skip_single = skip_single; p.n_splits = n_splits; p.scale = scale; p.slopes = slopes; p.scratch = scratch;
-    const dim3 grid(nKV, (unsigned)tiles, n_entries * n_splits);
+    p.q = (const bf16*)c.q; p.out = (bf16*)c.out; p.cu_q = c.cu_q; p.ctx_before = c.ctx_before; p.status = c.status; p.n_rows = c.n_rows;
+    p.nH = c.n_heads; p.window = c.window; p.skip_single = c.skip_single; p.n_splits = c.n_splits; p.scale = c.scale; p.slopes = c.slopes;
+    p.scratch = c.scratch;
+    const dim3 grid(c.n_kv, (unsigned)tiles, c.n_entries * c.n_splits);
     constexpr int smem = (int)sizeof(Smem) + 1024;
 #define Q8P_GO(KIND)                                                                                                     \
     do {                                                                                                                 \
@@ -480,6 +479,7 @@ NG_EXPORT int ng_attn_prefill_q8_sm100(const void* q, const void* k_pages, const
     } while (0)
     if (kind == NG_Q8_E4M3) Q8P_GO(NG_Q8_E4M3);
     else Q8P_GO(NG_Q8_INT8);
-    if (n_splits > 1) return q8_merge(scratch, cu_q, out, nH, n_splits, n_rows, n_entries, skip_single ? 2 : 1, 0x7fffffff, max_q, stream);
+    if (c.n_splits > 1)
+        return q8_merge(c.scratch, c.cu_q, c.out, c.n_heads, c.n_splits, c.n_rows, c.n_entries, c.skip_single ? 2 : 1, 0x7fffffff, c.max_q, stream);
     return ng_launch_status();
 }

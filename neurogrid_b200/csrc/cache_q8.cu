@@ -162,27 +162,36 @@ static int log2_of(int n) {
 }
 static bool power_of_two(int n) { return n > 0 && !(n & (n - 1)); }
 
-NG_EXPORT int ng_cache_write_q8(const void* k, const void* v, long long k_pitch, long long v_pitch, void* k_pages, void* v_pages,
-                                float* k_scales, float* v_scales, const int* table, int table_stride, const int* row_entry,
-                                const int* cu_q, const int* ctx_before, int n_rows, int n_entries, int nKV, int hd, int page_size,
-                                int block, int num_pages, int kind, int in_bf16, int* status, cudaStream_t stream) {
-    if (n_rows <= 0 || n_entries <= 0) return NG_OK;
-    if (nKV <= 0 || hd <= 0 || hd % 16 || !power_of_two(page_size) || !power_of_two(block) || block < 8 || block > page_size ||
-        num_pages <= 0 || table_stride <= 0 || !status || (kind != NG_Q8_E4M3 && kind != NG_Q8_INT8) ||
-        ((uintptr_t)k_pages & 7) || ((uintptr_t)v_pages & 7))
+// The arguments, packed (a call through ctypes pays for every argument: 26 of them took 5 us, a struct takes 1).
+struct NgCacheWriteQ8 {
+    const void *k, *v;
+    void *k_pages, *v_pages;
+    float *k_scales, *v_scales;
+    const int *table, *row_entry, *cu_q, *ctx_before;
+    int* status;
+    long long k_pitch, v_pitch;                     // elements between rows
+    int table_stride, n_rows, n_entries, n_kv, head_dim, page_size, block, num_pages, kind, in_bf16;
+};
+NG_EXPORT int ng_cache_write_q8(const NgCacheWriteQ8* c, cudaStream_t stream) {
+    const int n_rows = c->n_rows, nKV = c->n_kv, kind = c->kind;
+    if (n_rows <= 0 || c->n_entries <= 0) return NG_OK;
+    if (nKV <= 0 || c->head_dim <= 0 || c->head_dim % 16 || !power_of_two(c->page_size) || !power_of_two(c->block) || c->block < 8 ||
+        c->block > c->page_size || c->num_pages <= 0 || c->table_stride <= 0 || !c->status || (kind != NG_Q8_E4M3 && kind != NG_Q8_INT8) ||
+        (((uintptr_t)c->k_pages | (uintptr_t)c->v_pages) & 7))
         return NG_BAD_SIZE;
     // decode steps: a row a block, every row begins a unit; prompts: one row in `block` does, and a block looks eight of them over
     const int rpb = n_rows <= 512 ? 1 : 8;
-    const CwArgs a{k, v, k_pitch, v_pitch, (unsigned char*)k_pages, (unsigned char*)v_pages, k_scales, v_scales, table, row_entry, cu_q,
-                   ctx_before, status, table_stride, n_rows, n_entries, nKV, hd, log2_of(page_size), log2_of(block), num_pages, rpb};
+    const CwArgs a{c->k, c->v, c->k_pitch, c->v_pitch, (unsigned char*)c->k_pages, (unsigned char*)c->v_pages, c->k_scales, c->v_scales,
+                   c->table, c->row_entry, c->cu_q, c->ctx_before, c->status, c->table_stride, n_rows, c->n_entries, nKV, c->head_dim,
+                   log2_of(c->page_size), log2_of(c->block), c->num_pages, rpb};
     dim3 grid((n_rows + rpb - 1) / rpb, (2 * nKV + CW_WARPS - 1) / CW_WARPS);
     if (grid.y > 65535) return NG_BAD_SIZE;
-    const int esz = in_bf16 ? 2 : 4;
-    const bool vec = !(((uintptr_t)k | (uintptr_t)v) & 15) && k_pitch * esz % 16 == 0 && v_pitch * esz % 16 == 0;
+    const int esz = c->in_bf16 ? 2 : 4;
+    const bool vec = !(((uintptr_t)c->k | (uintptr_t)c->v) & 15) && c->k_pitch * esz % 16 == 0 && c->v_pitch * esz % 16 == 0;
 #define CW_GO(T, KIND, VEC) NG_LAUNCH((cache_write_q8_kernel<T, KIND, VEC>), grid, CW_WARPS * 32, 0, stream, a)
 #define CW_KINDS(T, VEC) do { if (kind == NG_Q8_E4M3) CW_GO(T, NG_Q8_E4M3, VEC); else CW_GO(T, NG_Q8_INT8, VEC); } while (0)
-    if (in_bf16 && vec) CW_KINDS(__nv_bfloat16, true);
-    else if (in_bf16) CW_KINDS(__nv_bfloat16, false);
+    if (c->in_bf16 && vec) CW_KINDS(__nv_bfloat16, true);
+    else if (c->in_bf16) CW_KINDS(__nv_bfloat16, false);
     else if (vec) CW_KINDS(float, true);
     else CW_KINDS(float, false);
     return ng_launch_status();
@@ -274,15 +283,18 @@ static int cp_launch(CpPool* pools, int n_pools, const int* src, const int* dst,
     return NG_OK;
 }
 
-// pools: n_pools base addresses, with the layers, pages and bytes of a page of each (a layer's pages follow one another)
-NG_EXPORT int ng_copy_pages(void* const* base, const int* layers, const int* pages, const long long* page_bytes, int n_pools,
-                            const int* src, const int* dst, int n, cudaStream_t stream) {
+struct NgPool {
+    void* base;
+    long long page_bytes;
+    int layers, pages;               // a layer's pages follow one another, and so do the layers
+};
+NG_EXPORT int ng_copy_pages(const NgPool* pool, int n_pools, const int* src, const int* dst, int n, cudaStream_t stream) {
     if (n < 0 || n_pools < 0 || n_pools > CP_POOLS) return NG_BAD_SIZE;
     if (n == 0 || n_pools == 0) return NG_OK;
     int fewest = 0x7fffffff;
     for (int k = 0; k < n_pools; ++k) {
-        if (layers[k] < 0 || pages[k] < 0 || page_bytes[k] <= 0) return NG_BAD_SIZE;
-        fewest = pages[k] < fewest ? pages[k] : fewest;
+        if (pool[k].layers < 0 || pool[k].pages < 0 || pool[k].page_bytes <= 0) return NG_BAD_SIZE;
+        fewest = pool[k].pages < fewest ? pool[k].pages : fewest;
     }
     for (int i = 0; i < n; ++i)
         if (src[i] < 0 || src[i] >= fewest || dst[i] < 0 || dst[i] >= fewest) return NG_BAD_PAGES;
@@ -302,12 +314,12 @@ NG_EXPORT int ng_copy_pages(void* const* base, const int* layers, const int* pag
     CpPool pools[CP_POOLS];
     for (int k = 0; k < n_pools; ++k) {
         CpPool& p = pools[k];
-        p.base = (unsigned char*)base[k];
-        p.layers = layers[k];
-        p.layer_bytes = page_bytes[k] * pages[k];
-        const unsigned long long at = (uintptr_t)p.base | (unsigned long long)page_bytes[k];        // layers are whole pages apart
+        p.base = (unsigned char*)pool[k].base;
+        p.layers = pool[k].layers;
+        p.layer_bytes = pool[k].page_bytes * pool[k].pages;
+        const unsigned long long at = (uintptr_t)p.base | (unsigned long long)pool[k].page_bytes;        // layers are whole pages apart
         p.piece_log2 = at % 16 == 0 ? 4 : at % 4 == 0 ? 2 : 0;
-        const long long pieces = page_bytes[k] >> p.piece_log2;
+        const long long pieces = pool[k].page_bytes >> p.piece_log2;
         if (pieces > (1 << 20)) return NG_BAD_SIZE;               // 1,024 pairs of them are counted in 31 bits
         p.pieces = (uint32_t)pieces;
         // i / pieces for i < 2^31, the round-up method: with 2^shift' >= pieces, m = ceil(2^(32 + s) / pieces), s = shift' - 1

@@ -163,10 +163,24 @@ static int log2_exact(int n) {               // -1: not a power of two
     while ((1 << l) < n) ++l;
     return l;
 }
-static bool cache_of(Cache& c, const void* k_pages, const void* v_pages, const float* ks, const float* vs, const int* table, int table_stride,
-                     int nKV, int page_size, int block, int num_pages) {
-    c = Cache{(const unsigned char*)k_pages, (const unsigned char*)v_pages, ks, vs, table, table_stride, num_pages, nKV, log2_exact(page_size),
-              log2_exact(block)};
-    return c.ps_log2 >= 3 && c.bl_log2 >= 3 && c.bl_log2 <= c.ps_log2 && nKV > 0 && table_stride > 0 && num_pages > 0 &&
-           ((long long)nKV * page_size * HD) <= 0x7fffffff && !(((uintptr_t)k_pages | (uintptr_t)v_pages) & 15);
+// The arguments of the attention entries, packed (a call through ctypes pays for every argument).
+struct NgAttnQ8 {
+    const void *q, *k_pages, *v_pages;
+    const float *k_scales, *v_scales;
+    const int *table, *cu_q, *ctx_before;
+    void* out;
+    float* scratch;
+    const float* slopes;
+    int* status;
+    int table_stride, n_rows, n_entries, max_q, n_heads, n_kv, head_dim, page_size, block, num_pages, kind, window, skip_single, n_splits;
+    float scale;
+};
+// What every entry refuses; fills in the cache.
+static bool attn_q8_args(const NgAttnQ8& c, Cache& to) {
+    to = Cache{(const unsigned char*)c.k_pages, (const unsigned char*)c.v_pages, c.k_scales, c.v_scales, c.table, c.table_stride, c.num_pages,
+               c.n_kv, log2_exact(c.page_size), log2_exact(c.block)};
+    return c.head_dim == HD && c.n_heads > 0 && c.n_kv > 0 && c.n_heads % c.n_kv == 0 && to.ps_log2 >= 3 && to.bl_log2 >= 3 &&
+           to.bl_log2 <= to.ps_log2 && c.table_stride > 0 && c.num_pages > 0 && (long long)c.n_kv * c.page_size * HD <= 0x7fffffff &&
+           !(((uintptr_t)c.k_pages | (uintptr_t)c.v_pages) & 15) && (c.kind == NG_Q8_E4M3 || c.kind == NG_Q8_INT8) && c.window >= 0 &&
+           c.n_splits >= 1 && (c.n_splits == 1 || (c.scratch && !((uintptr_t)c.scratch & 15)));
 }

@@ -11,6 +11,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import os
+import struct
 from typing import Optional, Tuple
 
 import torch
@@ -448,21 +449,29 @@ def q8_libraries(head_dim: int):
 
 
 Q8_KINDS = {torch.float8_e4m3fn: 0, torch.int8: 1}
+# the launchers' arguments (NgCacheWriteQ8, NgPool, NgAttnQ8), packed: a ctypes call pays for every argument
+_Q8_WRITE = struct.Struct("@11P2q10i")
+_Q8_POOL = struct.Struct("@Pq2i")
+_Q8_ATTENTION = struct.Struct("@12P14if")
+_Q8_CALL = [ctypes.c_char_p, _c_void_p]
 
 
 def _q8_cache(what: str, k_pages, v_pages, k_scales, v_scales, table):
     """(kind, pages, KV heads, page, head size, block) of a cache in 8 bits, after its checks."""
-    kind = Q8_KINDS.get(k_pages.dtype)
-    if kind is None or v_pages.dtype != k_pages.dtype:
-        raise KernelError(f"{what}: pages in 8 bits are float8_e4m3fn or int8 (keys and values alike), got {k_pages.dtype} and {v_pages.dtype}")
-    if k_pages.dim() != 4 or v_pages.shape != k_pages.shape:
+    dtype, shape, of_scales = k_pages.dtype, k_pages.shape, k_scales.shape
+    kind = Q8_KINDS.get(dtype)
+    if kind is None or v_pages.dtype is not dtype:
+        raise KernelError(f"{what}: pages in 8 bits are float8_e4m3fn or int8 (keys and values alike), got {dtype} and {v_pages.dtype}")
+    if len(shape) != 4 or v_pages.shape != shape:
         raise KernelError(f"{what}: pages are [pages, KV heads, page, head], keys and values alike")
-    num_pages, n_kv, page_size, hd = k_pages.shape
-    if k_scales.shape != v_scales.shape or k_scales.dim() != 3 or tuple(k_scales.shape[:2]) != (num_pages, n_kv) \
-            or k_scales.shape[2] < 1 or page_size % k_scales.shape[2]:
+    num_pages, n_kv, page_size, hd = shape
+    if len(of_scales) != 3 or v_scales.shape != of_scales or of_scales[0] != num_pages or of_scales[1] != n_kv \
+            or of_scales[2] < 1 or page_size % of_scales[2]:
         raise KernelError(f"{what}: scales are [pages, KV heads, page / block], keys' and values' alike")
-    _f32(k_scales, "key scales"), _f32(v_scales, "value scales"), _i32(table, "table")
-    block = page_size // k_scales.shape[2]
+    if k_scales.dtype is not torch.float32 or v_scales.dtype is not torch.float32:
+        raise KernelError(f"{what}: scales must be float32")
+    _i32(table, "table")
+    block = page_size // of_scales[2]
     if page_size & (page_size - 1) or block & (block - 1) or block < 8:
         raise KernelError(f"{what}: pages and blocks are powers of two, blocks of at least 8 tokens; got {page_size} and {block}")
     if hd % 16 or table.dim() != 2:
@@ -470,14 +479,21 @@ def _q8_cache(what: str, k_pages, v_pages, k_scales, v_scales, table):
     return kind, num_pages, n_kv, page_size, hd, block
 
 
-def _one_device(what: str, *tensors) -> None:
-    """The launch goes to the current device's stream: what it reads and writes has to be there."""
-    if not torch.cuda.is_available():
-        return                                                # (each tensor's own check says what is wrong)
-    here = torch.cuda.current_device()
-    for t in tensors:
-        if t is not None and t.is_cuda and t.device.index != here:
-            raise KernelError(f"{what}: a tensor is on {t.device}, the current device is cuda:{here}")
+def _current(what: str, t: torch.Tensor) -> int:
+    """The current device, whose stream the launch goes to; ``t``, and every other tensor of the call, has to be there."""
+    if not t.is_cuda:
+        _ptr(t, what)
+    return _current_device() if _current_device is not None else torch.cuda.current_device()
+
+
+def _on(what: str, t: torch.Tensor, here: int) -> int:
+    """The address of a contiguous tensor of device ``here``."""
+    if t.get_device() != here:
+        _ptr(t, what)
+        raise KernelError(f"{what}: a tensor is on {t.device}, the current device is cuda:{here}")
+    if not t.is_contiguous():
+        raise KernelError(f"{what}: a tensor must be contiguous")
+    return t.data_ptr()
 
 
 def cache_write_q8(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, k_scales: torch.Tensor,
@@ -494,19 +510,22 @@ def cache_write_q8(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pa
     int8.  Places of a page that no row goes to stay as they were.  A page that is not in the table sets the bad-page bit."""
     what = "cache_write_q8"
     kind, num_pages, n_kv, page_size, hd, block = _q8_cache(what, k_pages, v_pages, k_scales, v_scales, table)
-    if k.dim() != 2 or k.shape != v.shape or k.shape[1] != n_kv * hd or k.dtype != v.dtype:
+    shape = k.shape
+    if len(shape) != 2 or v.shape != shape or shape[1] != n_kv * hd or k.dtype is not v.dtype:
         raise KernelError(f"{what}: keys {tuple(k.shape)} and values {tuple(v.shape)} do not fit the pages")
-    act = _act_flag(k, "keys")
+    act, n_entries = _act_flag(k, "keys"), ctx_before.numel()
     _i32(row_entry, "row_entry"), _i32(cu_q, "cu_q"), _i32(ctx_before, "ctx_before"), _i32(status, "status")
-    n_entries = ctx_before.numel()
-    if row_entry.numel() != k.shape[0] or cu_q.numel() != n_entries + 1 or table.shape[0] < n_entries:
-        raise KernelError(f"{what}: the batch description does not fit {k.shape[0]} rows of {n_entries} entries")
-    _one_device(what, k, v, k_pages, v_pages, k_scales, v_scales, table, row_entry, cu_q, ctx_before, status)
-    f = _fn("cache_q8", "ng_cache_write_q8", [_c_void_p] * 2 + [_c_ll] * 2 + [_c_void_p] * 5 + [_c_int] + [_c_void_p] * 3 + [_c_int] * 9
-            + [_c_void_p] * 2)
-    _check(f(k.data_ptr(), v.data_ptr(), _column_block(k, "keys"), _column_block(v, "values"), _ptr(k_pages), _ptr(v_pages),
-             _ptr(k_scales), _ptr(v_scales), _ptr(table), table.shape[1], _ptr(row_entry), _ptr(cu_q), _ptr(ctx_before), k.shape[0],
-             n_entries, n_kv, hd, page_size, block, num_pages, kind, act, _ptr(status), _stream()), what)
+    if row_entry.numel() != shape[0] or cu_q.numel() != n_entries + 1 or table.shape[0] < n_entries:
+        raise KernelError(f"{what}: the batch description does not fit {shape[0]} rows of {n_entries} entries")
+    here = _current(what, k)
+    for t in (k, v):
+        if t.get_device() != here:
+            _on(what, t, here)
+    f = _fn("cache_q8", "ng_cache_write_q8", _Q8_CALL)
+    _check(f(_Q8_WRITE.pack(k.data_ptr(), v.data_ptr(), _on(what, k_pages, here), _on(what, v_pages, here), _on(what, k_scales, here),
+                            _on(what, v_scales, here), _on(what, table, here), _on(what, row_entry, here), _on(what, cu_q, here),
+                            _on(what, ctx_before, here), _on(what, status, here), _column_block(k, "keys"), _column_block(v, "values"),
+                            table.shape[1], shape[0], n_entries, n_kv, hd, page_size, block, num_pages, kind, act), _stream()), what)
 
 
 def copy_pages(pools, src, dst) -> None:
@@ -528,20 +547,21 @@ def copy_pages(pools, src, dst) -> None:
             raise KernelError(f"{what}: {_ERR[6]}")
     a, b = np.ascontiguousarray(a, dtype=np.int32), np.ascontiguousarray(b, dtype=np.int32)
     pools = [t for t in pools if t is not None]
-    for t in pools:
-        if t.dim() < 2 or t.shape[1] != pools[0].shape[1]:
-            raise KernelError(f"{what}: pools are [layers, pages, ...] with the same pages")
-        _ptr(t, "a pool")
-    _one_device(what, *pools)
-    pools = [t for t in pools if t.shape[0] and t.numel()]
-    f = _fn("cache_q8", "ng_copy_pages", [_c_void_p] * 4 + [_c_int] + [_c_void_p] * 2 + [_c_int, _c_void_p])
-    for i in range(0, len(pools), 8):
-        part = pools[i:i + 8]
-        n = len(part)
-        base = (ctypes.c_void_p * n)(*[t.data_ptr() for t in part])
-        layers, pages = (ctypes.c_int * n)(*[t.shape[0] for t in part]), (ctypes.c_int * n)(*[t.shape[1] for t in part])
-        size = (ctypes.c_longlong * n)(*[t.stride(1) * t.element_size() if t.shape[1] > 1 else t[0].numel() * t.element_size() for t in part])
-        _check(f(base, layers, pages, size, n, a.ctypes.data, b.ctypes.data, a.size, _stream()), what)
+    if not pools:
+        return
+    shapes = [t.shape for t in pools]
+    if any(len(x) < 2 or x[1] != shapes[0][1] for x in shapes):
+        raise KernelError(f"{what}: pools are [layers, pages, ...] with the same pages")
+    here, of_page = _current(what, pools[0]), []
+    for t, shape in zip(pools, shapes):
+        at, n = _on(what, t, here), t.numel()
+        if n:
+            of_page.append(_Q8_POOL.pack(at, n // (shape[0] * shape[1]) * t.element_size(), shape[0], shape[1]))
+    f = _fn("cache_q8", "ng_copy_pages", [ctypes.c_char_p, _c_int, ctypes.c_char_p, ctypes.c_char_p, _c_int, _c_void_p])
+    a, b, n = a.tobytes(), b.tobytes(), a.size
+    for i in range(0, len(of_page), 8):
+        part = of_page[i:i + 8]
+        _check(f(b"".join(part), len(part), a, b, n, _stream()), what)
 
 
 def attn_q8_scratch_floats(n_rows: int, n_heads: int, head_dim: int, n_splits: int) -> int:
@@ -578,24 +598,32 @@ def attn_prefill_q8_splits(q_lens, n_heads: int, n_kv_heads: int, head_dim: int,
     return max(1, min(slots // max(1, blocks), span // 512, 65535 // max(1, len(q_lens))))
 
 
-def _q8_attention(what, q, out, scratch, cache, cu_q, ctx_before, n_entries, n_heads, n_splits, n_records):
-    kind, num_pages, n_kv, page_size, hd, block = _q8_cache(what, *cache)
-    if q.dtype != torch.bfloat16 or out.dtype != torch.bfloat16:
+def _q8_attention(what, q, k_pages, v_pages, k_scales, v_scales, table, cu_q, ctx_before, out, scratch, n_entries, max_q, n_heads, window,
+                  scale, skip_single, n_splits, slopes, n_records):
+    """Checks, and the launcher's arguments but for the status word's address: (head size, a function of that address that packs them)."""
+    kind, num_pages, n_kv, page_size, hd, block = _q8_cache(what, k_pages, v_pages, k_scales, v_scales, table)
+    shape = q.shape
+    if q.dtype is not torch.bfloat16 or out.dtype is not torch.bfloat16:
         raise KernelError(f"{what} takes bfloat16 queries")
     if hd > 256:
         raise KernelError(f"{what}: head size {hd} is above 256")
-    if q.dim() != 2 or q.shape[1] != n_heads * hd or out.shape != q.shape or n_heads % n_kv:
+    if len(shape) != 2 or shape[1] != n_heads * hd or out.shape != shape or n_heads % n_kv:
         raise KernelError(f"{what}: shapes do not fit")
     if n_splits < 1:
         raise KernelError(f"{what}: {n_splits} runs")
     need = attn_q8_scratch_floats(n_records, n_heads, hd, n_splits)
-    if need and (scratch is None or scratch.numel() < need or scratch.dtype != torch.float32):
+    if need and (scratch is None or scratch.numel() < need or scratch.dtype is not torch.float32):
         raise KernelError(f"{what} needs {need} float32 values of scratch")
     _i32(cu_q, "cu_q"), _i32(ctx_before, "ctx_before")
-    if cu_q.numel() < n_entries + 1 or ctx_before.numel() < n_entries or cache[4].shape[0] < n_entries:
+    if cu_q.numel() < n_entries + 1 or ctx_before.numel() < n_entries or table.shape[0] < n_entries:
         raise KernelError(f"{what}: the batch description does not fit {n_entries} entries")
-    _one_device(what, q, out, scratch if need else None, *cache, cu_q, ctx_before)
-    return kind, num_pages, n_kv, page_size, hd, block
+    here = _current(what, q)
+    at = (_on(what, q, here), _on(what, k_pages, here), _on(what, v_pages, here), _on(what, k_scales, here), _on(what, v_scales, here),
+          _on(what, table, here), _on(what, cu_q, here), _on(what, ctx_before, here), _on(what, out, here), _on(what, scratch, here) if need else 0,
+          _slopes(slopes, n_heads) or 0)
+    rest = (table.shape[1], shape[0], n_entries, max_q, n_heads, n_kv, hd, page_size, block, num_pages, kind, window or 0, skip_single,
+            n_splits, scale)
+    return hd, lambda status: _Q8_ATTENTION.pack(*at, status, *rest)
 
 
 def attn_decode_q8(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, k_scales: torch.Tensor, v_scales: torch.Tensor,
@@ -604,16 +632,12 @@ def attn_decode_q8(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
                    slopes: Optional[torch.Tensor] = None) -> None:
     """``attn_decode_bf16`` over a cache in 8 bits (``cache_write_q8``): split-context attention of the entries that bring one token, any
     number of query heads a KV head.  The rows of other entries stay as they were.  ``n_splits`` (``attn_decode_q8_splits``) runs of
-    the keys; ``scratch`` holds ``attn_q8_scratch_floats`` (of ``n_entries``) float32 values when there is more than one."""
-    cache = (k_pages, v_pages, k_scales, v_scales, table)
-    kind, num_pages, n_kv, page_size, hd, block = _q8_attention("attn_decode_q8", q, out, scratch, cache, cu_q, ctx_before, n_entries,
-                                                                n_heads, n_splits, n_entries)
-    f = _fn("attention_q8", "ng_attn_decode_q8", [_c_void_p] * 6 + [_c_int] + [_c_void_p] * 4 + [_c_int] * 10
-            + [_c_float, _c_int, _c_int, _c_void_p, _c_void_p], {"NG_HEAD_DIM": hd})
-    _check(f(_ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(k_scales), _ptr(v_scales), _ptr(table), table.shape[1], _ptr(cu_q),
-             _ptr(ctx_before), _ptr(out), _ptr(scratch) if n_splits > 1 else None, q.shape[0], n_entries, n_heads, n_kv, hd, page_size,
-             block, num_pages, kind, int(window or 0), float(scale), int(n_splits), int(max_ctx), _slopes(slopes, n_heads), _stream()),
-           "attn_decode_q8")
+    the keys, planned for contexts of up to ``max_ctx`` (longer ones are right too); ``scratch`` holds ``attn_q8_scratch_floats`` (of
+    ``n_entries``) float32 values when there is more than one."""
+    hd, pack = _q8_attention("attn_decode_q8", q, k_pages, v_pages, k_scales, v_scales, table, cu_q, ctx_before, out, scratch, n_entries, 1,
+                             n_heads, window, scale, 0, n_splits, slopes, n_entries)
+    f = _fn("attention_q8", "ng_attn_decode_q8", _Q8_CALL, {"NG_HEAD_DIM": hd})
+    _check(f(pack(0), _stream()), "attn_decode_q8")
 
 
 def attn_prefill_q8(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, k_scales: torch.Tensor, v_scales: torch.Tensor,
@@ -623,21 +647,15 @@ def attn_prefill_q8(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     """Flash attention of the step's portions over a cache in 8 bits (``cache_write_q8``); their own keys are read from the cache too.
     Entries of one token are left to ``attn_decode_q8`` when ``skip_single``.  ``n_splits`` (``attn_prefill_q8_splits``) runs of every
     block's keys, merged through ``scratch`` (``attn_q8_scratch_floats`` of q's rows)."""
-    cache = (k_pages, v_pages, k_scales, v_scales, table)
-    kind, num_pages, n_kv, page_size, hd, block = _q8_attention("attn_prefill_q8", q, out, scratch, cache, cu_q, ctx_before, n_entries,
-                                                                n_heads, n_splits, q.shape[0])
-    tail = [_ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(k_scales), _ptr(v_scales), _ptr(table), table.shape[1], _ptr(cu_q),
-            _ptr(ctx_before), _ptr(out), _ptr(scratch) if n_splits > 1 else None, q.shape[0], n_entries, int(max_q), n_heads, n_kv, hd,
-            page_size, block, num_pages, kind, int(window or 0), float(scale), int(bool(skip_single)), int(n_splits),
-            _slopes(slopes, n_heads)]
-    types = [_c_void_p] * 6 + [_c_int] + [_c_void_p] * 4 + [_c_int] * 11 + [_c_float, _c_int, _c_int, _c_void_p]
+    hd, pack = _q8_attention("attn_prefill_q8", q, k_pages, v_pages, k_scales, v_scales, table, cu_q, ctx_before, out, scratch, n_entries,
+                             max_q, n_heads, window, scale, int(bool(skip_single)), n_splits, slopes, q.shape[0])
     if ATTN_BACKEND == "sm100" and hd in (64, 128) and scale > 0 and q.data_ptr() % 16 == 0 and out.data_ptr() % 16 == 0:
-        f = _fn("attention_q8_sm100", "ng_attn_prefill_q8_sm100", types + [_c_void_p] * 2, {"NG_HEAD_DIM": hd})
-        rc = f(*tail, _ptr(_gemm_status(q.device)), _stream())
+        f = _fn("attention_q8_sm100", "ng_attn_prefill_q8_sm100", _Q8_CALL, {"NG_HEAD_DIM": hd})
+        packed = pack(_gemm_status(q.device).data_ptr())
     else:
-        f = _fn("attention_q8", "ng_attn_prefill_q8", types + [_c_void_p], {"NG_HEAD_DIM": hd})
-        rc = f(*tail, _stream())
-    _check(rc, "attn_prefill_q8")
+        f = _fn("attention_q8", "ng_attn_prefill_q8", _Q8_CALL, {"NG_HEAD_DIM": hd})
+        packed = pack(0)
+    _check(f(packed, _stream()), "attn_prefill_q8")
 
 
 # ----------------------------------------------------------------------------- attention with float32 weights

@@ -1,5 +1,6 @@
 """What the operators over a cache in 8 bits refuse, and their arithmetic's plain statement (no GPU)."""
 import ctypes
+import struct
 
 import numpy as np
 import pytest
@@ -92,14 +93,12 @@ def test_copy_refuses():
 def test_the_copy_launcher_checks_every_page_number_before_it_launches():
     """The library's own answer for lists that it must not launch (there is no GPU here to launch on)."""
     f = build.load("cache_q8").ng_copy_pages
-    f.argtypes = [ctypes.c_void_p] * 4 + [ctypes.c_int] + [ctypes.c_void_p] * 2 + [ctypes.c_int, ctypes.c_void_p]
+    f.argtypes = [ctypes.c_char_p, ctypes.c_int, ctypes.c_char_p, ctypes.c_char_p, ctypes.c_int, ctypes.c_void_p]
 
     def call(src, dst, pages=(50, 40)):
-        n = len(pages)
-        base, layers = (ctypes.c_void_p * n)(*[4096] * n), (ctypes.c_int * n)(*[2] * n)
-        size = (ctypes.c_longlong * n)(*[64] * n)
+        pools = b"".join(struct.pack("@Pq2i", 4096, 64, 2, p) for p in pages)
         a, b = np.asarray(src, dtype=np.int32), np.asarray(dst, dtype=np.int32)
-        return f(base, layers, (ctypes.c_int * n)(*pages), size, n, a.ctypes.data, b.ctypes.data, len(a), None)
+        return f(pools, len(pages), a.tobytes(), b.tobytes(), len(a), None)
 
     assert call([], []) == 0
     many = list(range(20))
