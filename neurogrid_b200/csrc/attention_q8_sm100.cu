@@ -2,35 +2,38 @@
 // -DNG_HEAD_DIM).  The arithmetic is that of attention_q8.cu: codes as float16 operands, the keys' scales on the 32-bit scores,
 // the values' scales in the exponents, the sum divided by them.
 //
-// A block owns 128 rows of one (entry, KV head); a row is a (token, query head of the KV head), heads fastest, so that the heads which share
-// keys share the tiles that are fetched and turned into float16 for them.  Eight warps (of nine, a scheduler would have five of two
-// blocks' and a thread 96 registers; a softmax thread takes 128):
-//   warps 0-3  softmax: thread r owns row r = TMEM lane r; before the first tile it brings its row of q into shared memory
-//   warps 4-6  keys and values: codes of the next 64-key tile from the pages into registers while this one is stored, as float16, in
-//              the swizzled layout that the MMA reads (K row by row, V as it lies: [key][dim], MN-major)
-//   warp 7     MMA issuer: S = Q K^T and O += P V with tcgen05.mma, accumulators in TMEM, P taken from TMEM over S
-// S is double-buffered in TMEM: the next tile's scores are computed while this tile's softmax runs.  The tensor pipe runs the
-// issuer's MMAs in order and a commit covers all before it, so "S of tile j + 2 is complete" also says that P V of tile j has read its P.
+// A block owns two tiles of 128 rows of one (entry, KV head); a row is a (token, query head of the KV head), heads fastest, so that the heads
+// which share keys share the key tiles that are fetched and turned into float16 for them, and both row tiles share them too.  Warps:
+//   softmax     four for each stream; thread r of a stream owns row r of its row tile = TMEM lane r.  Heads of 64: a row tile has two
+//               streams, which take the even and the odd key tiles, each with a reference point, a sum and an O of its own, joined at the end:
+//               16 warps, four a scheduler, where eight waited for their own instructions most of the time.  Heads of 128 have one stream a row
+//               tile (two O's of both do not fit TMEM).  Before the first key tile a stream brings its rows of q into shared memory
+//   loaders (3) codes of the key tile after next from the pages into registers, while the tile before is stored as float16 in
+//               the swizzled layout that the MMA reads (K row by row, V as it lies: [key][dim], MN-major)
+//   issuer (1)  S = Q K^T and O += P V with tcgen05.mma, accumulators in TMEM, P taken from TMEM over S
+// A row tile has two S buffers, for even and odd key tiles.  The tensor pipe runs the issuer's MMAs in order and a commit covers all
+// before it, so "S of tile j + 2 is complete" also says that P V of tile j has read its P.
 //
 // Keys that no row of the block sees, and keys whose page is not there, are stored as zeros (their codes may be NaN).  Every mbarrier wait
 // is bounded; a waiter that gives up sets a status bit and the block runs to its end.
-//
-// Bound by the exponentials and the instructions around them (a score costs the thread of its row about three).
 #include <type_traits>
 
 #include "sm100_common.cuh"
 #include "ng_q8_attention.cuh"
 
 static_assert(HD == 64 || HD == 128, "head sizes 64 and 128");
-#define BQ 128                       // rows of a block
+#define BQ 128                       // rows of a row tile
+#define BR (2 * BQ)                  // rows of a block
 #define BK 64                        // keys of a tile
 #define NB (HD / 64)                 // 64-wide blocks of a head
-#define KV_STAGES (HD == 64 ? 3 : 2)
+#define KV_STAGES 4
 #define NG_STATUS_ATTN_TIMEOUT 16
-#define Q8P_THREADS 256
+#define STREAMS (HD == 64 ? 2 : 1)   // of a row tile
+#define SOFTMAX_WARPS (8 * STREAMS)
+#define Q8P_THREADS (32 * (SOFTMAX_WARPS + 4))
 #define KV_WARPS 3
 #define MIN_RUN 4                    // a run of keys is at least this many tiles
-static_assert(BQ == BLOCK_W, "a block's rows are the 128 rows of the MMA");
+static_assert(BQ == BLOCK_W, "a row tile is the 128 rows of the MMA");
 
 __device__ __forceinline__ float fmax3(float a, float b, float c) {
     float d;
@@ -56,12 +59,32 @@ __device__ __forceinline__ u64 fadd2(u64 a, u64 b) {
     return d;
 }
 
+// 32 consecutive float32 columns of this thread's TMEM lane, and 16 32-bit ones back
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
+    uint32_t r[32];
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\t"
+                 "tcgen05.wait::ld.sync.aligned;"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+                   "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+                 : "r"(taddr) : "memory");
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tmem_st16u(uint32_t taddr, const uint32_t (&v)[16]) {
+    float f[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) f[i] = __uint_as_float(v[i]);
+    tmem_st16(taddr, f);
+}
+
 struct Smem {
-    uint16_t q[NB][BQ * 64];                     // K-major, 128-byte swizzle, a block for each 64 of the head
+    uint16_t q[2][NB][BQ * 64];                  // K-major, 128-byte swizzle, a block for each 64 of the head
     uint16_t k[KV_STAGES][NB][BK * 64];
     uint16_t v[KV_STAGES][NB][BK * 64];
     float ks[KV_STAGES][8], vl[KV_STAGES][8], vi[KV_STAGES][8];       // of each 8 keys: K's scale, V's log2 and reciprocal
-    uint64_t q_full, kv_full[KV_STAGES], kv_empty[KV_STAGES], s_full[2], p_full[2], o_ready[2];
+    uint64_t q_full[2], kv_full[KV_STAGES], kv_empty[KV_STAGES], s_full[2][2], p_full[2][2], o_ready[2][2];          // [row tile][tile j & 1]
+    uint64_t joined[2][4];                       // [row tile][warp]: the odd tiles' stream has left its reference point and sum
+    float odd_m[BR], odd_l[BR];
     uint32_t tmem_base;
 };
 
@@ -83,7 +106,7 @@ __device__ __forceinline__ int sw128(int r, int c) { return (r >> 3) * 512 + (r 
 __host__ __device__ constexpr uint32_t idesc_f16(int n, int b_mn) { return make_idesc(n, b_mn) & ~((1u << 7) | (1u << 10)); }
 
 template <int KIND>
-__global__ void __launch_bounds__(Q8P_THREADS, 2)
+__global__ void __launch_bounds__(Q8P_THREADS, 1)
 attn_prefill_q8_sm100_kernel(const Params p) {
     extern __shared__ unsigned char smem_raw[];
     // (an offset, not a rounded address: the compiler then knows that what it points to is shared memory)
@@ -97,21 +120,23 @@ attn_prefill_q8_sm100_kernel(const Params p) {
     const int e = blockIdx.z / p.n_splits, split = blockIdx.z - e * p.n_splits, kvh = blockIdx.x;
     const int q0 = p.cu_q[e], q1 = p.cu_q[e + 1], qlen = min(q1, p.n_rows) - q0, ctx = p.ctx_before[e];
     const int G = p.nH / p.c.nKV;
-    const int r0 = (gridDim.y - 1 - blockIdx.y) * BQ;
+    const int r0 = (gridDim.y - 1 - blockIdx.y) * BR;
     if (q0 < 0 || ctx < 0 || r0 >= qlen * G || (p.skip_single && q1 - q0 == 1)) {
         ng_pdl_wait();                                         // (a launch none of whose blocks waited would end before the one before it)
         return;
     }
-    const int rows_here = min(BQ, qlen * G - r0);
-    const int pos_first = ctx + r0 / G, pos_last = ctx + (r0 + rows_here - 1) / G;
-    const int key_lo = p.window > 0 ? max(0, pos_first - p.window + 1) : 0, kv_end = pos_last + 1;
-    int tile0 = key_lo / BK, tile1 = pos_last / BK;            // inclusive
+    const int rows_here = min(BR, qlen * G - r0), rows_0 = min(BQ, rows_here), rows_1 = max(0, rows_here - BQ);
+    const int first = ctx + r0 / G, last = ctx + (r0 + rows_here - 1) / G;          // positions
+    const int key_lo = p.window > 0 ? max(0, first - p.window + 1) : 0, kv_end = last + 1;
+    int tile0 = key_lo / BK, tile1 = last / BK;                // inclusive
     if (p.n_splits > 1) {
         const int per = max(MIN_RUN, (tile1 - tile0 + p.n_splits) / p.n_splits);
         tile0 += split * per;
         tile1 = min(tile1, tile0 + per - 1);
     }
-    const int n_tiles = tile1 - tile0 + 1;
+    // key tiles of each row tile: the first one's rows see less
+    const int n_0 = min(tile1, (ctx + (r0 + rows_0 - 1) / G) / BK) - tile0 + 1, n_1 = rows_1 > 0 ? tile1 - tile0 + 1 : 0;
+    const int n_tiles = max(n_0, n_1);
     if (n_tiles <= 0) {                                        // an empty run: records that the merge passes over
         ng_pdl_wait();
         if (threadIdx.x < rows_here) {
@@ -123,38 +148,41 @@ attn_prefill_q8_sm100_kernel(const Params p) {
         return;
     }
     if (threadIdx.x == 0) {
-        mbar_init(&sm->q_full, 4);
         for (int s = 0; s < KV_STAGES; ++s) { mbar_init(&sm->kv_full[s], KV_WARPS); mbar_init(&sm->kv_empty[s], 1); }
-        for (int i = 0; i < 2; ++i) { mbar_init(&sm->s_full[i], 1); mbar_init(&sm->p_full[i], 4); mbar_init(&sm->o_ready[i], 1); }
+        for (int t = 0; t < 2; ++t) {
+            mbar_init(&sm->q_full[t], 4 * STREAMS);
+            for (int i = 0; i < 4; ++i) mbar_init(&sm->joined[t][i], 1);
+            for (int i = 0; i < 2; ++i) { mbar_init(&sm->s_full[t][i], 1); mbar_init(&sm->p_full[t][i], 4); mbar_init(&sm->o_ready[t][i], 1); }
+        }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 7) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 256;" :: "r"(smem_u32(&sm->tmem_base)) : "memory");
+    if (warp == SOFTMAX_WARPS + KV_WARPS) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" :: "r"(smem_u32(&sm->tmem_base)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     ng_pdl_wait();                                             // q and the pages are this step's data
     tcgen05_fence_before();
     __syncthreads();
     tcgen05_fence_after();
-    const uint32_t tmem = sm->tmem_base, tm_s0 = tmem, tm_s1 = tmem + BK, tm_o = tmem + 2 * BK;
+    const uint32_t tmem = sm->tmem_base;                       // S of row tile t, tile j: 128 t + 64 (j & 1); O: tm_o(t, j)
+    auto tm_o = [&](int t, int j) { return tmem + 256 + HD * (STREAMS == 2 ? 2 * t + (j & 1) : t); };
     bool ok = true;
 
-    if (warp >= 4 && warp < 4 + KV_WARPS) {
+    if (warp >= SOFTMAX_WARPS && warp < SOFTMAX_WARPS + KV_WARPS) {
         // ------------------------------------------------------------------ keys and values
         // A unit is eight keys (they lie in one page and one block) of K and of V: UNIT_LOADS requests of 16 bytes a lane each.  A warp has
         // every third unit; page numbers are asked for a tile before the codes, the codes DEPTH tiles before they are stored.
-        constexpr int UNIT_LOADS = HD / 64, UNITS = (8 + KV_WARPS - 1) / KV_WARPS, DEPTH = HD == 64 ? 2 : 1;
-        const int w = __shfl_sync(0xffffffffu, warp - 4, 0), mask = (1 << p.c.ps_log2) - 1;
+        constexpr int UNIT_LOADS = HD / 64, UNITS = (8 + KV_WARPS - 1) / KV_WARPS, DEPTH = 2;
+        const int w = __shfl_sync(0xffffffffu, warp - SOFTMAX_WARPS, 0), mask = (1 << p.c.ps_log2) - 1;
         const int* trow = p.c.table + (size_t)e * p.c.table_stride;
         const long long page_bytes = (long long)(p.c.nKV << p.c.ps_log2) * HD, head_at = (long long)(kvh << p.c.ps_log2) * HD + lane * 16;
         const unsigned char *k_pages = p.c.k + head_at, *v_pages = p.c.v + head_at;
         uint32_t k[DEPTH][UNITS][UNIT_LOADS][4], v[DEPTH][UNITS][UNIT_LOADS][4];
         float ks[DEPTH], vs[DEPTH];
-        int page[UNITS], my_page;                              // of the next tile to ask for; my_page: lane u's, unit u's (the scales)
-        auto page_of = [&](int key) {
+        int page[UNITS], my_page;                              // of the next tile to ask for, as the table has them; my_page: lane u's, unit u's (the scales)
+        auto page_of = [&](int key) {                          // (not looked at before the next tile: the load would be waited for here)
             const int i = key >> p.c.ps_log2;
-            const int id = key + 7 >= key_lo && key < kv_end && i < p.c.table_stride ? trow[i] : -1;
-            return (unsigned)id < (unsigned)p.c.num_pages ? id : -1;
+            return key + 7 >= key_lo && key < kv_end && i < p.c.table_stride ? trow[i] : -1;
         };
         auto pages = [&](int tile) {
 #pragma unroll
@@ -165,18 +193,19 @@ attn_prefill_q8_sm100_kernel(const Params p) {
 #pragma unroll
             for (int n = 0; n < UNITS; ++n) {
                 const int key0 = tile * BK + 8 * (w + KV_WARPS * n);
-                const long long at = (long long)max(page[n], 0) * page_bytes + (key0 & mask) * HD;
+                const bool there = (unsigned)page[n] < (unsigned)p.c.num_pages;
+                const long long at = (long long)(there ? page[n] : 0) * page_bytes + (key0 & mask) * HD;
 #pragma unroll
                 for (int i = 0; i < UNIT_LOADS; ++i) {
                     const int key = key0 + (i * 512 + lane * 16) / HD;
-                    const bool in = page[n] >= 0 && key >= key_lo && key < kv_end;
+                    const bool in = there && key >= key_lo && key < kv_end;
 #pragma unroll
                     for (int x = 0; x < 4; ++x) k[d][n][i][x] = v[d][n][i][x] = 0u;
                     if (in) ld_codes<16>(k[d][n][i], k_pages + at + i * 512), ld_codes<16>(v[d][n][i], v_pages + at + i * 512);
                 }
             }
             ks[d] = vs[d] = 1.f;
-            if (my_page >= 0) {
+            if ((unsigned)my_page < (unsigned)p.c.num_pages) {
                 const long long sc = ((long long)my_page * p.c.nKV + kvh << (p.c.ps_log2 - p.c.bl_log2)) + ((tile * BK + 8 * lane & mask) >> p.c.bl_log2);
                 ld_codes<4>(reinterpret_cast<uint32_t*>(&ks[d]), reinterpret_cast<const unsigned char*>(p.c.ks + sc));
                 ld_codes<4>(reinterpret_cast<uint32_t*>(&vs[d]), reinterpret_cast<const unsigned char*>(p.c.vs + sc));
@@ -223,56 +252,69 @@ attn_prefill_q8_sm100_kernel(const Params p) {
                 pages(tile0 + j + DEPTH + 1);
             }
         if (!ok && lane == 0) atomicOr(p.status, NG_STATUS_ATTN_TIMEOUT);
-    } else if (warp == 7) {
+    } else if (warp == SOFTMAX_WARPS + KV_WARPS) {
         // ------------------------------------------------------------------ MMA issuer: all lanes run the loop, one issues
         constexpr uint32_t idesc_s = idesc_f16(BK, 0), idesc_o = idesc_f16(64, 1);
-        ok = __all_sync(0xffffffffu, mbar_wait(&sm->q_full, 0));
-        auto issue_s = [&](int j) {                            // S_j = Q K_j^T into buffer j & 1
+        for (int t = 0; t < 2 && ok; ++t)
+            if ((t ? n_1 : n_0) > 0) ok = __all_sync(0xffffffffu, mbar_wait(&sm->q_full[t], 0));
+        auto issue_s = [&](int t, int j) {                     // S = Q K_j^T into buffer j & 1 of row tile t
             const int s = j % KV_STAGES;
             if (!__all_sync(0xffffffffu, mbar_wait(&sm->kv_full[s], (j / KV_STAGES) & 1))) { ok = false; return; }
             tcgen05_fence_after();
             if (leader) {
 #pragma unroll
                 for (int b = 0; b < NB; ++b) {
-                    const uint64_t dq = make_desc_sw128(sm->q[b]), dk = make_desc_sw128(sm->k[s][b]);
+                    const uint64_t dq = make_desc_sw128(sm->q[t][b]), dk = make_desc_sw128(sm->k[s][b]);
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
-                        tcgen05_mma_f16((j & 1) ? tm_s1 : tm_s0, dq + (uint64_t)(2 * k), dk + (uint64_t)(2 * k), idesc_s, b > 0 || k > 0);
+                        tcgen05_mma_f16(tmem + 128 * t + 64 * (j & 1), dq + (uint64_t)(2 * k), dk + (uint64_t)(2 * k), idesc_s, b > 0 || k > 0);
                 }
-                tcgen05_commit(&sm->s_full[j & 1]);
+                tcgen05_commit(&sm->s_full[t][j & 1]);
             }
             __syncwarp();
         };
-        if (ok) issue_s(0);
-        if (ok && n_tiles > 1) issue_s(1);
+        for (int j = 0; j < 2; ++j)
+            for (int t = 0; t < 2; ++t)
+                if (ok && j < (t ? n_1 : n_0)) issue_s(t, j);
         for (int j = 0; j < n_tiles && ok; ++j) {
-            ok = __all_sync(0xffffffffu, mbar_wait(&sm->p_full[j & 1], (j >> 1) & 1));          // P_j in tensor memory, O rescaled
-            if (!ok) break;
-            tcgen05_fence_after();
             const int s = j % KV_STAGES;
-            const uint32_t tp = (j & 1) ? tm_s1 : tm_s0;
-            if (leader) {
 #pragma unroll
-                for (int b = 0; b < NB; ++b) {
-                    const uint64_t dv = make_desc_sw128_mn(sm->v[s][b]);
+            for (int t = 0; t < 2; ++t) {
+                const int n = t ? n_1 : n_0;
+                if (!ok) break;
+                if (j < n) {
+                    ok = __all_sync(0xffffffffu, mbar_wait(&sm->p_full[t][j & 1], (j >> 1) & 1));          // P_j in tensor memory, O rescaled
+                    if (!ok) break;
+                    tcgen05_fence_after();
+                    if (leader) {
 #pragma unroll
-                    for (int k = 0; k < BK / 16; ++k)          // 16 keys an MMA: 8 columns of P, 2,048 bytes of V
-                        tcgen05_mma_f16_ts(tm_o + 64 * b, tp + 8 * k, dv + (uint64_t)(128 * k), idesc_o, j > 0 || k > 0);
+                        for (int b = 0; b < NB; ++b) {
+                            const uint64_t dv = make_desc_sw128_mn(sm->v[s][b]);
+#pragma unroll
+                            for (int k = 0; k < BK / 16; ++k)  // 16 keys an MMA: 8 columns of P, 2,048 bytes of V
+                                tcgen05_mma_f16_ts(tm_o(t, j) + 64 * b, tmem + 128 * t + 64 * (j & 1) + 8 * k, dv + (uint64_t)(128 * k),
+                                                   idesc_o, j >= STREAMS || k > 0);
+                        }
+                        tcgen05_commit(&sm->o_ready[t][j & 1]);                // O holds tiles 0..j
+                    }
                 }
-                tcgen05_commit(&sm->kv_empty[s]);              // K_j and V_j may be overwritten
-                tcgen05_commit(&sm->o_ready[j & 1]);           // O holds tiles 0..j
+                if (t == 1 && leader) tcgen05_commit(&sm->kv_empty[s]);        // K_j and V_j may be overwritten
+                __syncwarp();
+                if (j + 2 < n) issue_s(t, j + 2);
             }
-            __syncwarp();
-            if (j + 2 < n_tiles) issue_s(j + 2);
         }
         if (!ok && leader) atomicOr(p.status, NG_STATUS_ATTN_TIMEOUT);
     } else {
         // ------------------------------------------------------------------ softmax: thread = row
-        const int r = threadIdx.x, rr = r0 + min(r, rows_here - 1);        // rows past the last mirror it
+        const int t = warp / (4 * STREAMS), odd = STREAMS == 2 ? warp >> 2 & 1 : 0, r = threadIdx.x & (BQ - 1);
+        const int n_mine = t ? n_1 : n_0, rows_mine = t ? rows_1 : rows_0;
+        const int rr = r0 + BQ * t + min(r, max(rows_mine, 1) - 1);        // rows past the last mirror it
         const int token = rr / G, head = kvh * G + rr - token * G, pos = ctx + token;
-        float f;
-        {
-            // the row of q, divided by a power of two, as float16
+        const int pos_first = ctx + (r0 + BQ * t) / G, pos_last = ctx + (r0 + BQ * t + max(rows_mine, 1) - 1) / G;
+        const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
+        float f = 0.f;
+        if (n_mine > 0) {
+            // the row of q, divided by a power of two, as float16 (of two streams, each writes half)
             const bf16* q = ng_after_wait(p.q) + ((size_t)(q0 + token) * p.nH + head) * HD;
             float top = 0.f;
 #pragma unroll 4
@@ -290,76 +332,69 @@ attn_prefill_q8_sm100_kernel(const Params p) {
             const float div = pow2_any(-ex);
             f = p.scale * LOG2E * pow2_any(ex);
 #pragma unroll 4
-            for (int c = 0; c < HD / 8; ++c) {
+            for (int c = odd * (HD / 16); c < (odd || STREAMS == 1 ? HD / 8 : HD / 16); ++c) {
                 const uint4 w = *reinterpret_cast<const uint4*>(q + 8 * c);
                 const uint32_t x[4] = {w.x, w.y, w.z, w.w};
                 uint32_t h[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) h[i] = pack_f16(__uint_as_float(x[i] << 16) * div, __uint_as_float(x[i] & 0xffff0000u) * div);
-                *reinterpret_cast<uint4*>(sm->q[c / 8] + sw128(r, c % 8)) = make_uint4(h[0], h[1], h[2], h[3]);
+                *reinterpret_cast<uint4*>(sm->q[t][c / 8] + sw128(r, c % 8)) = make_uint4(h[0], h[1], h[2], h[3]);
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
-            if (lane == 0) mbar_arrive(&sm->q_full);
+            if (lane == 0) mbar_arrive(&sm->q_full[t]);
         }
-        const uint32_t lane_base = (uint32_t)(warp * 32) << 16;
         // m is the reference point of the exponentials; it moves to the first tile's maximum and then follows lazily: only when a tile exceeds
         // it by more than 2^8 is O in TMEM rescaled (which has to wait for the product before).
         float m = 0.f, l = 0.f;
         bool seen = false;
         const float slope = p.slopes ? p.slopes[head] * LOG2E : 0.f;
-        for (int j = 0; j < n_tiles && ok; ++j) {
-            const int s = j % KV_STAGES;
-            ok = mbar_wait(&sm->kv_full[s], (j / KV_STAGES) & 1) && mbar_wait(&sm->s_full[j & 1], (j >> 1) & 1);
+        for (int j = odd; j < n_mine && ok; j += STREAMS) {
+            const int s = j % KV_STAGES, key0 = (tile0 + j) * BK;
+            ok = mbar_wait(&sm->kv_full[s], (j / KV_STAGES) & 1) && mbar_wait(&sm->s_full[t][j & 1], (j >> 1) & 1);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             tcgen05_fence_after();
-            const uint32_t ts = ((j & 1) ? tm_s1 : tm_s0) + lane_base;
-            const int key0 = (tile0 + j) * BK;
-            float sc[BK];
-            tmem_ld64(ts, sc);
-            // only tiles that cross a row's diagonal or the window's edge need the mask; z is then formed here.  A distance bias alone is linear
-            // in the key: its part within each eight keys is added here, the rest goes with the values' scale.
-            const bool masked = !(key0 + BK - 1 <= pos_first && (p.window <= 0 || key0 > pos_last - p.window));
-            const bool formed = masked || slope != 0.f;
-            if (masked) {
-#pragma unroll
-                for (int b = 0; b < 8; ++b) {
-                    const float fk = f * sm->ks[s][b], lg = sm->vl[s][b];
-#pragma unroll
-                    for (int i = 8 * b; i < 8 * b + 8; ++i) {
-                        const int key = key0 + i;
-                        const bool vis = key <= pos && (p.window <= 0 || key > pos - p.window);
-                        sc[i] = vis ? fmaf(slope, (float)(key - pos), fmaf(sc[i], fk, lg)) : -INFINITY;
-                    }
-                }
-            } else if (formed) {
-#pragma unroll
-                for (int b = 0; b < 8; ++b) {
-                    const float fk = f * sm->ks[s][b];
-                    const u64 fk2 = pack2(fk, fk);
-#pragma unroll
-                    for (int i = 0; i < 8; i += 2)
-                        unpack2(ffma2(pack2(sc[8 * b + i], sc[8 * b + i + 1]), fk2, pack2(slope * i, slope * (i + 1))), sc[8 * b + i], sc[8 * b + i + 1]);
-                }
-            }
-            uint32_t pk[BK / 2];
+            const uint32_t ts = tmem + 128 * t + 64 * (j & 1) + lane_base;
             float corr = 1.f;
-            // z = sc fk + lg for each eight keys (f and the scales are positive, so the largest sc has the largest z)
-            auto weigh = [&](auto is_formed) {
-                constexpr bool FORMED = decltype(is_formed)::value;
-                const float far = masked ? 0.f : slope * (float)(key0 - pos), far8 = masked ? 0.f : 8.f * slope, own = masked ? 0.f : 1.f;
+            // z = sc fk + lg + slope (key - pos), 32 keys of the row at a time; where no key is hidden the largest z of each eight keys has the
+            // largest sc (f and the scales are positive), or with a bias the largest sc fk + slope i.  The first pass finds the maximum, the
+            // second the weights: the last 32 scores are still there, the first are read again.
+            auto weigh = [&](auto kind) {
+                constexpr int MODE = decltype(kind)::value;                // 0: plain, 1: a bias, 2: hidden keys (and a bias)
+                const float far = slope * (float)(key0 - pos);
+                const int rel = pos - key0, out_of = p.window > 0 ? rel - p.window : -1;
+                float sc[32];
+                auto formed = [&](int b, float ks, float vl) {             // the eight scores at 8 b (of the half h) become z (2), or z less lg and far (1)
+                    if constexpr (MODE == 1) {
+                        const float fk = f * ks;
+                        const u64 fk2 = pack2(fk, fk);
+#pragma unroll
+                        for (int i = 0; i < 8; i += 2)
+                            unpack2(ffma2(pack2(sc[8 * (b & 3) + i], sc[8 * (b & 3) + i + 1]), fk2, pack2(slope * i, slope * (i + 1))),
+                                    sc[8 * (b & 3) + i], sc[8 * (b & 3) + i + 1]);
+                    } else if constexpr (MODE == 2) {
+                        const float fk = f * ks;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            float& x = sc[8 * (b & 3) + i];
+                            x = 8 * b + i <= rel && 8 * b + i > out_of ? fmaf(slope, (float)(8 * b + i), fmaf(x, fk, vl + far)) : -INFINITY;
+                        }
+                    }
+                };
                 float mx = -INFINITY;
 #pragma unroll
-                for (int b = 0; b < 8; b += 4) {
-                    const float4 k4 = *reinterpret_cast<const float4*>(&sm->ks[s][b]), v4 = *reinterpret_cast<const float4*>(&sm->vl[s][b]);
+                for (int h = 0; h < 2; ++h) {
+                    tmem_ld32(ts + 32 * h, sc);
+                    const float4 k4 = *reinterpret_cast<const float4*>(&sm->ks[s][4 * h]), v4 = *reinterpret_cast<const float4*>(&sm->vl[s][4 * h]);
                     const float ks[4] = {k4.x, k4.y, k4.z, k4.w}, vl[4] = {v4.x, v4.y, v4.z, v4.w};
                     float mz[4];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float* x = sc + 8 * (b + i);
+                    for (int u = 0; u < 4; ++u) {
+                        formed(4 * h + u, ks[u], vl[u]);
+                        const float* x = sc + 8 * u;
                         const float y = fmaxf(fmax3(fmax3(x[0], x[1], x[2]), fmax3(x[3], x[4], x[5]), x[6]), x[7]);
-                        mz[i] = FORMED ? y + fmaf(own, vl[i], fmaf(far8, (float)(b + i), far)) : fmaf(y, f * ks[i], vl[i]);
+                        mz[u] = MODE == 0 ? fmaf(y, f * ks[u], vl[u]) : MODE == 1 ? y + (vl[u] + fmaf(8.f * slope, (float)(4 * h + u), far)) : y;
                     }
                     mx = fmax3(mx, fmaxf(mz[0], mz[1]), fmaxf(mz[2], mz[3]));
                 }
@@ -369,20 +404,27 @@ attn_prefill_q8_sm100_kernel(const Params p) {
                     m = mx;
                     l *= corr;
                 }
+                uint32_t late[16];
 #pragma unroll
-                for (int b = 0; b < 8; b += 4) {
-                    const float4 k4 = *reinterpret_cast<const float4*>(&sm->ks[s][b]), v4 = *reinterpret_cast<const float4*>(&sm->vl[s][b]);
-                    const float4 i4 = *reinterpret_cast<const float4*>(&sm->vi[s][b]);
+                for (int h = 1; h >= 0; --h) {
+                    if (h == 0) {
+                        tmem_ld32(ts, sc);
+                        tmem_st16u(ts + 16, late);                         // (over scores that have just been read again)
+                    }
+                    uint32_t pk[16];
+                    const float4 k4 = *reinterpret_cast<const float4*>(&sm->ks[s][4 * h]), v4 = *reinterpret_cast<const float4*>(&sm->vl[s][4 * h]);
+                    const float4 i4 = *reinterpret_cast<const float4*>(&sm->vi[s][4 * h]);
                     const float ks[4] = {k4.x, k4.y, k4.z, k4.w}, vl[4] = {v4.x, v4.y, v4.z, v4.w}, vi[4] = {i4.x, i4.y, i4.z, i4.w};
 #pragma unroll
                     for (int u = 0; u < 4; ++u) {
-                        const float fk = f * ks[u], lg = (FORMED ? fmaf(own, vl[u], fmaf(far8, (float)(b + u), far)) : vl[u]) - m;
+                        if (h == 0) formed(u, ks[u], vl[u]);
+                        const float fk = f * ks[u], lg = (MODE == 0 ? vl[u] : MODE == 1 ? vl[u] + fmaf(8.f * slope, (float)(4 * h + u), far) : 0.f) - m;
                         const u64 fk2 = pack2(fk, fk), lg2 = pack2(lg, lg);
                         u64 sum2 = pack2(0.f, 0.f);
 #pragma unroll
-                        for (int i = 8 * (b + u); i < 8 * (b + u) + 8; i += 2) {
+                        for (int i = 8 * u; i < 8 * u + 8; i += 2) {
                             float x, y;
-                            unpack2(FORMED ? fadd2(pack2(sc[i], sc[i + 1]), lg2) : ffma2(pack2(sc[i], sc[i + 1]), fk2, lg2), x, y);
+                            unpack2(MODE == 0 ? ffma2(pack2(sc[i], sc[i + 1]), fk2, lg2) : fadd2(pack2(sc[i], sc[i + 1]), lg2), x, y);
                             x = q8_ex2(x), y = q8_ex2(y);
                             sum2 = fadd2(sum2, pack2(x, y));
                             pk[i / 2] = pack_f16(x, y);
@@ -391,68 +433,101 @@ attn_prefill_q8_sm100_kernel(const Params p) {
                         unpack2(sum2, x, y);
                         l = fmaf(x + y, vi[u], l);
                     }
+                    if (h == 0) tmem_st16u(ts, pk);
+                    else
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) late[i] = pk[i];
                 }
             };
-            if (formed) weigh(std::true_type{});
-            else weigh(std::false_type{});
-            if (j > 0 && __any_sync(0xffffffffu, corr != 1.f)) {           // rescale this warp's rows of O
-                ok = mbar_wait(&sm->o_ready[(j - 1) & 1], ((j - 1) >> 1) & 1);
+            // only tiles that cross a row's diagonal or the window's edge have hidden keys
+            if (!(key0 + BK - 1 <= pos_first && (p.window <= 0 || key0 > pos_last - p.window))) weigh(std::integral_constant<int, 2>{});
+            else if (p.slopes) weigh(std::integral_constant<int, 1>{});
+            else weigh(std::integral_constant<int, 0>{});
+            if (j >= STREAMS && __any_sync(0xffffffffu, corr != 1.f)) {    // rescale this warp's rows of O
+                ok = mbar_wait(&sm->o_ready[t][(j - STREAMS) & 1], ((j - STREAMS) >> 1) & 1);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 tcgen05_fence_after();
 #pragma unroll
                 for (int c = 0; c < HD; c += 16) {
                     float x[16];
-                    tmem_ld16(tm_o + lane_base + c, x);
+                    tmem_ld16(tm_o(t, j) + lane_base + c, x);
 #pragma unroll
                     for (int i = 0; i < 16; ++i) x[i] *= corr;
-                    tmem_st16(tm_o + lane_base + c, x);
+                    tmem_st16(tm_o(t, j) + lane_base + c, x);
                 }
-                tmem_st_wait();
             }
-            // P -> tensor memory, over this row's S (whose last other reader, the product of tile j - 2, is complete with S_j)
-            tmem_st32(ts, pk);
+            // P lies over this row's S (whose last other reader, the product of tile j - 2, is complete with S_j)
             tmem_st_wait();
             tcgen05_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&sm->p_full[j & 1]);
+            if (lane == 0) mbar_arrive(&sm->p_full[t][j & 1]);
         }
-        if (ok) {
-            ok = mbar_wait(&sm->o_ready[(n_tiles - 1) & 1], ((n_tiles - 1) >> 1) & 1);
+        // what the odd tiles' stream found goes to the even tiles', which writes the rows
+        const int last_j = n_mine - 1 - (STREAMS == 2 && (n_mine - 1 & 1) != odd ? 1 : 0);             // the stream's last tile (< 0: none)
+        if (ok && n_mine > 0 && last_j >= 0) {
+            ok = mbar_wait(&sm->o_ready[t][last_j & 1], (last_j >> 1) & 1);
             ok = __all_sync(0xffffffffu, ok);
         }
-        if (ok) {
-            tcgen05_fence_after();
+        float m_odd = -INFINITY, l_odd = 0.f;
+        if (STREAMS == 2 && n_mine > 1 && ok) {
+            if (odd) {
+                tcgen05_fence_before();
+                sm->odd_m[BQ * t + r] = seen ? m : -INFINITY;
+                sm->odd_l[BQ * t + r] = l;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sm->joined[t][warp & 3]);
+            } else {
+                ok = __all_sync(0xffffffffu, mbar_wait(&sm->joined[t][warp & 3], 0));
+                m_odd = sm->odd_m[BQ * t + r];
+                l_odd = sm->odd_l[BQ * t + r];
+            }
+        }
+        if (!ok) {
+            if (lane == 0) atomicOr(p.status, NG_STATUS_ATTN_TIMEOUT);
+        } else if (!odd) {
             const size_t at = (size_t)(q0 + token) * p.nH + head;
             float* rec = p.scratch + (at * p.n_splits + split) * REC;
-            if (p.n_splits > 1 && r < rows_here) rec[0] = seen ? m : -INFINITY, rec[1] = l;
+            const bool two = STREAMS == 2 && n_mine > 1, live = r < rows_mine;
+            const float m_even = seen ? m : -INFINITY, top = fmaxf(m_even, m_odd);
+            // (a stream that met only NaN has no reference point and keeps its sums)
+            float a = m_even == -INFINITY ? (top == -INFINITY ? 1.f : 0.f) : q8_ex2(m_even - top);
+            float b = m_odd == -INFINITY ? (top == -INFINITY ? 1.f : 0.f) : q8_ex2(m_odd - top);
+            l = fmaf(l, a, l_odd * b);
+            if (n_mine <= 0) l = 0.f;
+            if (p.n_splits > 1 && live) rec[0] = n_mine > 0 ? top : -INFINITY, rec[1] = l;
             const float inv = l == 0.f ? 0.f : 1.f / l;
+            if (p.n_splits == 1) a *= inv, b *= inv;
+            if (n_mine > 0) {
+                tcgen05_fence_after();
 #pragma unroll
-            for (int c = 0; c < HD; c += 16) {
-                float x[16];
-                tmem_ld16(tm_o + lane_base + c, x);
-                if (r < rows_here && p.n_splits > 1) {
+                for (int c = 0; c < HD; c += 16) {
+                    float x[16], y[16];
+                    tmem_ld16(tm_o(t, 0) + lane_base + c, x);
+                    if (two) tmem_ld16(tm_o(t, 1) + lane_base + c, y);
 #pragma unroll
-                    for (int i = 0; i < 16; i += 4) *reinterpret_cast<float4*>(rec + 4 + c + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
-                } else if (r < rows_here) {
-                    uint32_t w[8];
+                    for (int i = 0; i < 16; ++i) x[i] = two ? fmaf(x[i], a, y[i] * b) : x[i] * a;
+                    if (live && p.n_splits > 1) {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i] * inv, x[2 * i + 1] * inv);
-                        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+                        for (int i = 0; i < 16; i += 4) *reinterpret_cast<float4*>(rec + 4 + c + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+                    } else if (live) {
+                        uint32_t w[8];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+                            w[i] = *reinterpret_cast<const uint32_t*>(&h);
+                        }
+                        *reinterpret_cast<uint4*>(p.out + at * HD + c) = make_uint4(w[0], w[1], w[2], w[3]);
+                        *reinterpret_cast<uint4*>(p.out + at * HD + c + 8) = make_uint4(w[4], w[5], w[6], w[7]);
                     }
-                    *reinterpret_cast<uint4*>(p.out + at * HD + c) = make_uint4(w[0], w[1], w[2], w[3]);
-                    *reinterpret_cast<uint4*>(p.out + at * HD + c + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+                    __syncwarp();
                 }
-                __syncwarp();
             }
-        } else if (lane == 0) {
-            atomicOr(p.status, NG_STATUS_ATTN_TIMEOUT);
         }
     }
     tcgen05_fence_before();
     __syncthreads();
-    if (warp == 7) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 256;" :: "r"(tmem) : "memory");
+    if (warp == SOFTMAX_WARPS + KV_WARPS) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" :: "r"(tmem) : "memory");
 }
 
 // scratch (n_splits > 1): n_rows * n_heads * n_splits * REC floats, 16-byte aligned
@@ -464,7 +539,7 @@ NG_EXPORT int ng_attn_prefill_q8_sm100(const NgAttnQ8* call, cudaStream_t stream
     if (!attn_q8_args(c, p.c) || (long long)c.n_entries * c.n_splits > 65535 || !(c.scale > 0.f) || !c.status ||
         (((uintptr_t)c.q | (uintptr_t)c.out) & 15))
         return NG_BAD_SIZE;
-    const long long tiles = ((long long)c.max_q * (c.n_heads / c.n_kv) + BQ - 1) / BQ;
+    const long long tiles = ((long long)c.max_q * (c.n_heads / c.n_kv) + BR - 1) / BR;
     if (tiles > 65535) return NG_BAD_SIZE;
     p.q = (const bf16*)c.q; p.out = (bf16*)c.out; p.cu_q = c.cu_q; p.ctx_before = c.ctx_before; p.status = c.status; p.n_rows = c.n_rows;
     p.nH = c.n_heads; p.window = c.window; p.skip_single = c.skip_single; p.n_splits = c.n_splits; p.scale = c.scale; p.slopes = c.slopes;

@@ -591,11 +591,10 @@ def attn_decode_q8_splits(n_single: int, n_heads: int, n_kv_heads: int, head_dim
 def attn_prefill_q8_splits(q_lens, n_heads: int, n_kv_heads: int, head_dim: int, max_ctx: int, window: Optional[int], device) -> int:
     """Runs ``attn_prefill_q8`` should cut the keys into: where its blocks (128 rows of a KV head's query heads) leave SMs idle and see
     keys enough to share."""
-    group = n_heads // n_kv_heads
-    blocks = sum(-(-n * group // 128) for n in q_lens) * n_kv_heads
+    group, rows = n_heads // n_kv_heads, 256 if head_dim in (64, 128) else 128
+    blocks = sum(-(-n * group // rows) for n in q_lens) * n_kv_heads
     span = min(window + max(q_lens), max_ctx) if window else max_ctx
-    slots = (2 if head_dim in (64, 128) else 1) * _sm_count(device)
-    return max(1, min(slots // max(1, blocks), span // 512, 65535 // max(1, len(q_lens))))
+    return max(1, min(_sm_count(device) // max(1, blocks), span // 512, 65535 // max(1, len(q_lens))))
 
 
 def _q8_attention(what, q, k_pages, v_pages, k_scales, v_scales, table, cu_q, ctx_before, out, scratch, n_entries, max_q, n_heads, window,
