@@ -189,19 +189,17 @@ attn_prefill_q8_sm100_kernel(const Params p) {
             for (int n = 0; n < UNITS; ++n) page[n] = w + KV_WARPS * n < 8 ? page_of(tile * BK + 8 * (w + KV_WARPS * n)) : -1;
             my_page = w == KV_WARPS - 1 && lane < 8 ? page_of(tile * BK + 8 * lane) : -1;
         };
+        // (a page that is not there: page 0 is read, and the unit's keys become zeros when they are stored)
+        bool bad[DEPTH][UNITS];
         auto load = [&](int d, int tile) {
 #pragma unroll
             for (int n = 0; n < UNITS; ++n) {
-                const int key0 = tile * BK + 8 * (w + KV_WARPS * n);
-                const bool there = (unsigned)page[n] < (unsigned)p.c.num_pages;
-                const long long at = (long long)(there ? page[n] : 0) * page_bytes + (key0 & mask) * HD;
+                bad[d][n] = (unsigned)page[n] >= (unsigned)p.c.num_pages;
+                const long long at = (long long)(bad[d][n] ? 0 : page[n]) * page_bytes + (tile * BK + 8 * (w + KV_WARPS * n) & mask) * HD;
 #pragma unroll
                 for (int i = 0; i < UNIT_LOADS; ++i) {
-                    const int key = key0 + (i * 512 + lane * 16) / HD;
-                    const bool in = there && key >= key_lo && key < kv_end;
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) k[d][n][i][x] = v[d][n][i][x] = 0u;
-                    if (in) ld_codes<16>(k[d][n][i], k_pages + at + i * 512), ld_codes<16>(v[d][n][i], v_pages + at + i * 512);
+                    ld_codes<16>(k[d][n][i], k_pages + at + i * 512);
+                    ld_codes<16>(v[d][n][i], v_pages + at + i * 512);
                 }
             }
             ks[d] = vs[d] = 1.f;
@@ -233,13 +231,23 @@ attn_prefill_q8_sm100_kernel(const Params p) {
                 if (!ok) break;
 #pragma unroll
                 for (int n = 0; n < UNITS; ++n)
-                    if (w + KV_WARPS * n < 8)
+                    if (w + KV_WARPS * n < 8) {
+                        const int key0 = (tile0 + j) * BK + 8 * (w + KV_WARPS * n);
+                        if (bad[d][n] || key0 < key_lo || key0 + 8 > kv_end)         // keys that no row sees: zeros
+#pragma unroll
+                            for (int i = 0; i < UNIT_LOADS; ++i) {
+                                const int key = key0 + (i * 512 + lane * 16) / HD;
+                                if (bad[d][n] || key < key_lo || key >= kv_end)
+#pragma unroll
+                                    for (int x = 0; x < 4; ++x) k[d][n][i][x] = v[d][n][i][x] = 0u;
+                            }
 #pragma unroll
                         for (int i = 0; i < UNIT_LOADS; ++i) {
                             const int o = i * 512 + lane * 16, row = 8 * (w + KV_WARPS * n) + o / HD, c = o % HD / 8;
                             put(sm->k[s][c / 8], row, c % 8, k[d][n][i]);
                             put(sm->v[s][c / 8], row, c % 8, v[d][n][i]);
                         }
+                    }
                 if (w == KV_WARPS - 1 && lane < 8) {
                     sm->ks[s][lane] = ks[d];
                     sm->vl[s][lane] = q8_log2(vs[d]);
@@ -257,6 +265,9 @@ attn_prefill_q8_sm100_kernel(const Params p) {
         constexpr uint32_t idesc_s = idesc_f16(BK, 0), idesc_o = idesc_f16(64, 1);
         for (int t = 0; t < 2 && ok; ++t)
             if ((t ? n_1 : n_0) > 0) ok = __all_sync(0xffffffffu, mbar_wait(&sm->q_full[t], 0));
+        // descriptors of the first stage; addresses are in units of 16 bytes, and so are the distances added to them
+        const uint64_t q_desc = make_desc_sw128(sm->q[0][0]), k_desc = make_desc_sw128(sm->k[0][0]), v_desc = make_desc_sw128_mn(sm->v[0][0]);
+        constexpr uint64_t Q_TILE = sizeof(sm->q[0]) / 16, Q_BLOCK = sizeof(sm->q[0][0]) / 16, KV_STAGE = sizeof(sm->k[0]) / 16, KV_BLOCK = sizeof(sm->k[0][0]) / 16;
         auto issue_s = [&](int t, int j) {                     // S = Q K_j^T into buffer j & 1 of row tile t
             const int s = j % KV_STAGES;
             if (!__all_sync(0xffffffffu, mbar_wait(&sm->kv_full[s], (j / KV_STAGES) & 1))) { ok = false; return; }
@@ -264,7 +275,7 @@ attn_prefill_q8_sm100_kernel(const Params p) {
             if (leader) {
 #pragma unroll
                 for (int b = 0; b < NB; ++b) {
-                    const uint64_t dq = make_desc_sw128(sm->q[t][b]), dk = make_desc_sw128(sm->k[s][b]);
+                    const uint64_t dq = q_desc + t * Q_TILE + b * Q_BLOCK, dk = k_desc + s * KV_STAGE + b * KV_BLOCK;
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
                         tcgen05_mma_f16(tmem + 128 * t + 64 * (j & 1), dq + (uint64_t)(2 * k), dk + (uint64_t)(2 * k), idesc_s, b > 0 || k > 0);
@@ -289,7 +300,7 @@ attn_prefill_q8_sm100_kernel(const Params p) {
                     if (leader) {
 #pragma unroll
                         for (int b = 0; b < NB; ++b) {
-                            const uint64_t dv = make_desc_sw128_mn(sm->v[s][b]);
+                            const uint64_t dv = v_desc + s * KV_STAGE + b * KV_BLOCK;
 #pragma unroll
                             for (int k = 0; k < BK / 16; ++k)  // 16 keys an MMA: 8 columns of P, 2,048 bytes of V
                                 tcgen05_mma_f16_ts(tm_o(t, j) + 64 * b, tmem + 128 * t + 64 * (j & 1) + 8 * k, dv + (uint64_t)(128 * k),
