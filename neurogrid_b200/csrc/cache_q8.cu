@@ -54,6 +54,23 @@ __device__ __forceinline__ uint2 cw_codes(const float (&x)[8], float f) {
     return make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
 }
 
+// n chunks of eight codes, by a warp: to a scale that is 2^-by times theirs
+template <int KIND>
+__device__ __forceinline__ void cw_requantise(unsigned char* front, int n, int by) {
+    const float g = q8_pow2(max(by, -126));                          // (below that every code becomes 0)
+    for (int i = threadIdx.x & 31; i < n; i += 32) {
+        const uint2 w = *reinterpret_cast<const uint2*>(front + (size_t)i * 8);
+        uint32_t h[4];
+        q8_to_half<KIND>(w.x, h[0], h[1]);
+        q8_to_half<KIND>(w.y, h[2], h[3]);
+        float y[8];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.f32.f16 %0, a;\n\tcvt.f32.f16 %1, b;\n\t}" : "=f"(y[2 * j]), "=f"(y[2 * j + 1]) : "r"(h[j]));
+        *reinterpret_cast<uint2*>(front + (size_t)i * 8) = cw_codes<KIND>(y, g);
+    }
+}
+
 struct CwArgs {
     const void *k, *v;
     long long k_pitch, v_pitch;                     // elements between rows
@@ -136,21 +153,7 @@ cache_write_q8_kernel(const CwArgs a) {
             cw_load8<T, VEC>(src + (i / per_row) * pitch + (i % per_row) * 8, y);
             *reinterpret_cast<uint2*>(dst + (size_t)i * 8) = cw_codes<KIND>(y, f);
         }
-        if (lead && exp > old) {                    // the tokens in front: to the new scale
-            const float g = q8_pow2(max(old - exp, -126));          // (below that every code becomes 0)
-            unsigned char* front = dst - (size_t)lead * a.hd;
-            for (int i = lane; i < lead * per_row; i += 32) {
-                const uint2 w = *reinterpret_cast<const uint2*>(front + (size_t)i * 8);
-                uint32_t h[4];
-                q8_to_half<KIND>(w.x, h[0], h[1]);
-                q8_to_half<KIND>(w.y, h[2], h[3]);
-                float y[8];
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.f32.f16 %0, a;\n\tcvt.f32.f16 %1, b;\n\t}" : "=f"(y[2 * j]), "=f"(y[2 * j + 1]) : "r"(h[j]));
-                *reinterpret_cast<uint2*>(front + (size_t)i * 8) = cw_codes<KIND>(y, g);
-            }
-        }
+        if (lead && exp > old) cw_requantise<KIND>(dst - (size_t)lead * a.hd, lead * per_row, old - exp);
         __syncwarp();
         if (lane == 0 && (!lead || exp > old)) *scale = q8_pow2(exp);
     }
@@ -195,6 +198,138 @@ NG_EXPORT int ng_cache_write_q8(const NgCacheWriteQ8* c, cudaStream_t stream) {
     else if (c->in_bf16) CW_KINDS(__nv_bfloat16, false);
     else if (vec) CW_KINDS(float, true);
     else CW_KINDS(float, false);
+    return ng_launch_status();
+}
+
+// ===================================================================================== rotation and write of single tokens
+// rope_cache.cu's preparation (a head's norm, the rotation, one rounding to bfloat16; the same arithmetic in the same order) and the write above in
+// one launch, for steps whose entries bring one token each: a warp has a head, and so all that is new in its block.  6 layers of LFM2-1.2B a
+// step: a launch of about 2.4 us less each.
+struct NgRopeCacheQ8 {
+    const void* qkv;                                // [rows, (heads + 2 KV heads) head_dim] in bfloat16, or n_part float32 partial sums of it
+    void* q_out;
+    const float *q_weight, *k_weight, *inv_freq;
+    void *k_pages, *v_pages;
+    float *k_scales, *v_scales;
+    const int *table, *positions, *row_entry;
+    int* status;
+    long long part_stride;
+    int n_part, half_pairing, table_stride, n_rows, n_heads, n_kv, head_dim, page_size, block, num_pages, kind;
+    float pos_scale, eps;
+};
+#define RQ_WARPS 4
+template <typename TI, int KIND, int PAIRS>
+__global__ void __launch_bounds__(RQ_WARPS * 32)
+rope_cache_q8_kernel(const NgRopeCacheQ8 c, int ps_log2, int bl_log2) {
+    ng_pdl_trigger();
+    const int row = blockIdx.x, lane = threadIdx.x & 31, head = blockIdx.y * RQ_WARPS + (threadIdx.x >> 5);
+    const int entry = c.row_entry[row], pos = c.positions[row], hd = c.head_dim, half = hd / 2;
+    const bool is_q = head < c.n_heads, is_v = head >= c.n_heads + c.n_kv;
+    const float* w = is_q ? c.q_weight : is_v ? nullptr : c.k_weight;
+    const bool turn = c.inv_freq && !is_v;
+    const float pf = (float)pos / c.pos_scale;
+    int ia[PAIRS], ib[PAIRS];
+    float sn[PAIRS], cs[PAIRS], wa[PAIRS], wb[PAIRS];
+#pragma unroll
+    for (int u = 0; u < PAIRS; ++u) {
+        const int i = min(lane + 32 * u, half - 1);
+        ia[u] = c.half_pairing ? i : 2 * i;
+        ib[u] = c.half_pairing ? i + half : 2 * i + 1;
+        sn[u] = 0.f;
+        cs[u] = 1.f;
+        if (turn && lane + 32 * u < half) sincosf(pf * c.inv_freq[i], &sn[u], &cs[u]);
+        wa[u] = w ? w[ia[u]] : 1.f;
+        wb[u] = w ? w[ib[u]] : 1.f;
+    }
+    ng_pdl_wait();
+    if (head >= c.n_heads + 2 * c.n_kv) return;
+    __nv_bfloat16* q = reinterpret_cast<__nv_bfloat16*>(c.q_out) + ((size_t)row * c.n_heads + head) * hd;
+    if (entry < 0) {                                // padding row: defined output, no cache write
+        if (is_q)
+            for (int j = lane; j < hd; j += 32) q[j] = __float2bfloat16(0.f);
+        return;
+    }
+    const TI* in = ng_after_wait(reinterpret_cast<const TI*>(c.qkv)) + ((size_t)row * (c.n_heads + 2 * c.n_kv) + head) * hd;
+    float x[PAIRS], y[PAIRS], ss = 0.f;
+#pragma unroll
+    for (int u = 0; u < PAIRS; ++u) {
+        x[u] = ng_ld_sum<__nv_bfloat16>(in, ia[u], c.n_part, c.part_stride);
+        y[u] = ng_ld_sum<__nv_bfloat16>(in, ib[u], c.n_part, c.part_stride);
+        if (sizeof(TI) == 4) {                      // (a stack of one part is not rounded yet)
+            x[u] = __bfloat162float(__float2bfloat16(x[u]));
+            y[u] = __bfloat162float(__float2bfloat16(y[u]));
+        }
+        if (lane + 32 * u >= half) x[u] = y[u] = 0.f;
+    }
+    if (w) {
+#pragma unroll
+        for (int u = 0; u < PAIRS; ++u) ss += x[u] * x[u] + y[u] * y[u];
+        const float r = rsqrtf(ng_warp_sum(ss) / (float)hd + c.eps);
+#pragma unroll
+        for (int u = 0; u < PAIRS; ++u) x[u] = x[u] * r * wa[u], y[u] = y[u] * r * wb[u];
+    }
+    float top = 0.f;
+#pragma unroll
+    for (int u = 0; u < PAIRS; ++u) {
+        if (turn) {
+            const float a = x[u] * cs[u] - y[u] * sn[u], b = x[u] * sn[u] + y[u] * cs[u];
+            x[u] = a;
+            y[u] = b;
+        }
+        const __nv_bfloat16 a = __float2bfloat16(x[u]), b = __float2bfloat16(y[u]);
+        if (lane + 32 * u < half) {
+            if (is_q) q[ia[u]] = a, q[ib[u]] = b;
+            x[u] = __bfloat162float(a);
+            y[u] = __bfloat162float(b);
+            top = fabsf(x[u]) < INFINITY ? fmaxf(top, fabsf(x[u])) : top;
+            top = fabsf(y[u]) < INFINITY ? fmaxf(top, fabsf(y[u])) : top;
+        }
+    }
+    if (is_q) return;
+    const int kv = is_v ? head - c.n_heads - c.n_kv : head - c.n_heads, pi = pos >> ps_log2;
+    const int page = pos >= 0 && pi < c.table_stride ? c.table[(size_t)entry * c.table_stride + pi] : -1;
+    if (page < 0 || page >= c.num_pages) {
+        if (lane == 0 && head == c.n_heads) atomicOr(c.status, NG_STATUS_BAD_PAGE);
+        return;
+    }
+    const int slot = pos & ((1 << ps_log2) - 1), lead = pos & ((1 << bl_log2) - 1);
+    const size_t slab = (size_t)page * c.n_kv + kv;
+    unsigned char* dst = reinterpret_cast<unsigned char*>(is_v ? c.v_pages : c.k_pages) + ((slab << ps_log2) + slot) * hd;
+    float* scale = (is_v ? c.v_scales : c.k_scales) + (slab << (ps_log2 - bl_log2)) + (slot >> bl_log2);
+    const int old = lead ? min(max(q8_exponent_of(*scale), NG_Q8_EXP_LOWEST), NG_Q8_EXP_HIGHEST) : NG_Q8_EXP_LOWEST;
+    const int exp = max(q8_exponent<KIND>(ng_warp_max(top)), old);
+    const float f = q8_pow2(-exp);
+#pragma unroll
+    for (int u = 0; u < PAIRS; ++u)
+        if (lane + 32 * u < half) {
+            const uint32_t h = q8_from_float<KIND>(x[u] * f, y[u] * f);
+            dst[ia[u]] = (unsigned char)h;
+            dst[ib[u]] = (unsigned char)(h >> 8);
+        }
+    if (lead && exp > old) cw_requantise<KIND>(dst - (size_t)lead * hd, lead * (hd >> 3), old - exp);
+    __syncwarp();
+    if (lane == 0 && (!lead || exp > old)) *scale = q8_pow2(exp);
+}
+
+NG_EXPORT int ng_rope_cache_q8(const NgRopeCacheQ8* call, cudaStream_t stream) {
+    const NgRopeCacheQ8& c = *call;
+    if (c.n_rows <= 0) return NG_OK;
+    if (c.n_heads <= 0 || c.n_kv <= 0 || c.head_dim <= 0 || c.head_dim % 16 || c.head_dim > 256 || !power_of_two(c.page_size) ||
+        !power_of_two(c.block) || c.block < 8 || c.block > c.page_size || c.num_pages <= 0 || c.table_stride <= 0 || !c.status || c.n_part < 0 ||
+        c.pos_scale == 0.f || (c.kind != NG_Q8_E4M3 && c.kind != NG_Q8_INT8) || (((uintptr_t)c.k_pages | (uintptr_t)c.v_pages) & 7))
+        return NG_BAD_SIZE;
+    const dim3 grid(c.n_rows, (c.n_heads + 2 * c.n_kv + RQ_WARPS - 1) / RQ_WARPS);
+    if (grid.y > 65535) return NG_BAD_SIZE;
+#define RQ_GO(TI, KIND, PAIRS) NG_LAUNCH((rope_cache_q8_kernel<TI, KIND, PAIRS>), grid, RQ_WARPS * 32, 0, stream, c, log2_of(c.page_size), log2_of(c.block))
+#define RQ_PAIRS(TI, KIND)                                                                                                             \
+    do {                                                                                                                               \
+        if (c.head_dim <= 64) RQ_GO(TI, KIND, 1);                                                                                      \
+        else if (c.head_dim <= 128) RQ_GO(TI, KIND, 2);                                                                                \
+        else RQ_GO(TI, KIND, 4);                                                                                                       \
+    } while (0)
+#define RQ_KINDS(TI) do { if (c.kind == NG_Q8_E4M3) RQ_PAIRS(TI, NG_Q8_E4M3); else RQ_PAIRS(TI, NG_Q8_INT8); } while (0)
+    if (c.n_part > 0) RQ_KINDS(float);
+    else RQ_KINDS(__nv_bfloat16);
     return ng_launch_status();
 }
 

@@ -449,8 +449,9 @@ def q8_libraries(head_dim: int):
 
 
 Q8_KINDS = {torch.float8_e4m3fn: 0, torch.int8: 1}
-# the launchers' arguments (NgCacheWriteQ8, NgPool, NgAttnQ8), packed: a ctypes call pays for every argument
+# the launchers' arguments (NgCacheWriteQ8, NgRopeCacheQ8, NgPool, NgAttnQ8), packed: a ctypes call pays for every argument
 _Q8_WRITE = struct.Struct("@11P2q10i")
+_Q8_ROPE = struct.Struct("@13Pq11i2f")
 _Q8_POOL = struct.Struct("@Pq2i")
 _Q8_ATTENTION = struct.Struct("@12P14if")
 _Q8_CALL = [ctypes.c_char_p, _c_void_p]
@@ -528,6 +529,31 @@ def cache_write_q8(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pa
                             table.shape[1], shape[0], n_entries, n_kv, hd, page_size, block, num_pages, kind, act), _stream()), what)
 
 
+def rope_cache_q8(qkv: torch.Tensor, q_out: torch.Tensor, q_weight: Optional[torch.Tensor], k_weight: Optional[torch.Tensor],
+                  inv_freq: Optional[torch.Tensor], half_pairing: bool, pos_scale: float, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                  k_scales: torch.Tensor, v_scales: torch.Tensor, table: torch.Tensor, positions: torch.Tensor, row_entry: torch.Tensor,
+                  n_heads: int, eps: float, status: torch.Tensor) -> None:
+    """``rope_cache`` and ``cache_write_q8`` in one launch, for a step whose entries bring one token each (no entry has two rows):
+    qkv [N, (nH + 2 nKV) * hd] bfloat16 (or a float32 stack [S, N, ...] of partial sums), q -> q_out[N, nH * hd] bfloat16."""
+    what = "rope_cache_q8"
+    kind, num_pages, n_kv, page_size, hd, block = _q8_cache(what, k_pages, v_pages, k_scales, v_scales, table)
+    n = q_out.shape[0]
+    if q_out.dtype is not torch.bfloat16 or q_out.shape != (n, n_heads * hd) or hd > 256:
+        raise KernelError(f"{what}: q is bfloat16 [N, heads * head], heads of at most 256")
+    n_part, stride = _stack(qkv, (n, (n_heads + 2 * n_kv) * hd), q_out.dtype, "rope_cache_q8 input")
+    _f32(q_weight, "q norm weight"), _f32(k_weight, "k norm weight"), _f32(inv_freq, "inv_freq")
+    _i32(positions, "positions"), _i32(row_entry, "row_entry"), _i32(status, "status")
+    if positions.numel() != n or row_entry.numel() != n or (inv_freq is not None and inv_freq.numel() != hd // 2) \
+            or any(w is not None and w.numel() != hd for w in (q_weight, k_weight)):
+        raise KernelError(f"{what}: shapes do not fit {n} rows of heads of {hd}")
+    here = _current(what, qkv)
+    at = [0 if t is None else _on(what, t, here) for t in (qkv, q_out, q_weight, k_weight, inv_freq, k_pages, v_pages, k_scales, v_scales,
+                                                           table, positions, row_entry, status)]
+    f = _fn("cache_q8", "ng_rope_cache_q8", _Q8_CALL)
+    _check(f(_Q8_ROPE.pack(*at, stride, n_part if qkv.dtype is torch.float32 else 0, int(half_pairing), table.shape[1], n, n_heads, n_kv, hd,
+                           page_size, block, num_pages, kind, pos_scale, eps), _stream()), what)
+
+
 def copy_pages(pools, src, dst) -> None:
     """pool[:, dst[i]] = pool[:, src[i]] for every tensor of ``pools``, each [layers, pages, ...] and contiguous (keys, values and
     scales of a group of layers go in one launch).  ``src`` and ``dst`` are page numbers on the host: sequences, numpy arrays or CPU
@@ -580,12 +606,17 @@ def attn_decode_q8_splits(n_single: int, n_heads: int, n_kv_heads: int, head_dim
     group = -(-n_heads // n_kv_heads)
     segments = n_kv_heads * -(-group // (16 if group > 8 and head_dim <= 64 else 8))      # of an entry
     turns = -(-(min(window, max_ctx) if window else max_ctx) // (128 if head_dim <= 128 else 64))
-    if turns <= 4:
-        return 1
     slots = (3 if head_dim <= 64 and group <= 8 else 2) * _sm_count(device)
-    even = -(-turns // -(-n_single * segments * turns // slots)) + 1             # all entries as long as the longest
-    alone = -(-turns // -(-segments * turns // slots)) + 1                       # the longest alone
-    return min(alone, max(2 * even, 16))
+    # One block a segment, or shares and a merge, in turns of a block: the merge, the search for the share and pieces of two segments cost
+    # about seven.  Heads of 64, 32 / 8 heads, us with one run / several: 1 row behind 1,000 tokens 6.6 / 7.4, 16 behind 1,500 13.6 / 11.9,
+    # 32 behind 1,500 14.9 / 17.5, behind 2,000 18.6 / 20.3, behind 4,000 32.9 / 30.2, 64 behind 1,000 20.6 / 20.6, behind 2,000 35.2 / 32.0,
+    # 128 behind 1,000 32.3 / 35.1, 256 behind 2,000 95.9 / 100; heads of 128, 32 rows behind 2,000 25.0 / 29.0
+    whole, share = -(-n_single * segments // slots) * turns, -(-n_single * segments * turns // slots)
+    if whole <= share + 7:
+        return 1
+    even = -(-turns // share) + 1                                                # all entries as long as the longest
+    alone = -(-turns // -(-segments * turns // slots)) + 1                       # the longest alone: no more than the merge is worth
+    return min(alone, max(2 * even, 16, turns // 3))
 
 
 def attn_prefill_q8_splits(q_lens, n_heads: int, n_kv_heads: int, head_dim: int, max_ctx: int, window: Optional[int], device) -> int:

@@ -111,6 +111,11 @@ class Attention:
         a = ctx.ws.buf("attn_out", n, s.n_heads * s.head_dim, self.dtype)
         if cache.k_scales is not None:
             # pages of codes: the rotated keys, and the values, as rows; then a block of tokens' codes and scale at a time
+            if n_kv and ctx.max_q == 1 and not ctx.fixed_launches:         # single tokens: in one launch
+                ops.rope_cache_q8(qkv, q, self.q_norm, self.k_norm, inv_freq, half, pos_scale, cache.k_pages, cache.v_pages,
+                                  cache.k_scales, cache.v_scales, cache.table, ctx.positions, ctx.row_entry, s.n_heads, s.qk_norm_eps, ctx.status)
+                self.attend_q8(q, cache, ctx, a, pa.score_slopes)
+                return ops.linear_to_residual(a, self.w_o, self.b_o, ctx.ws, "mixer_out", residual=ctx.residual)
             rows = [None, None]
             if n_kv:
                 rows = [ctx.ws.buf(name, n, n_kv * s.head_dim, self.dtype) for name in ("attn_k_rows", "attn_v_rows")]

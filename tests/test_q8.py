@@ -50,6 +50,25 @@ def test_write_refuses(kw, why):
         write(**kw)
 
 
+@pytest.mark.parametrize("kw,why", [
+    (dict(), "CUDA"),
+    (dict(q=torch.zeros(3, 64)), "bfloat16"),
+    (dict(q=torch.zeros(3, 65, dtype=torch.bfloat16)), "q is bfloat16"),
+    (dict(qkv=torch.zeros(3, 128, dtype=torch.bfloat16)), "expected"),
+    (dict(qkv=torch.zeros(2, 3, 192, dtype=torch.bfloat16)), "float32"),
+    (dict(positions=i32(0, 0)), "do not fit"),
+    (dict(inv_freq=torch.ones(8)), "do not fit"),
+    (dict(weight=torch.ones(31)), "do not fit"),
+    (dict(weight=torch.ones(32, dtype=torch.float64)), "float32"),
+    (dict(c=cache(kind=torch.bfloat16)), "8 bits"),
+])
+def test_rope_and_write_refuses(kw, why):
+    with pytest.raises(ops.KernelError, match=why):
+        ops.rope_cache_q8(kw.get("qkv", torch.zeros(3, 192, dtype=torch.bfloat16)), kw.get("q", torch.zeros(3, 64, dtype=torch.bfloat16)),
+                          kw.get("weight"), None, kw.get("inv_freq"), True, 1.0, *kw.get("c", cache()), kw.get("positions", i32(0, 5, 9)),
+                          i32(0, 1, 1), 2, 1e-5, i32(0))
+
+
 def attend(fn, q=None, out=None, c=None, heads=4, splits=1, scratch=None, n=2, cu=None, **kw):
     q = torch.zeros(3, 128, dtype=torch.bfloat16) if q is None else q
     out = torch.zeros_like(q) if out is None else out

@@ -169,6 +169,41 @@ def test_write_passes_over_padding_and_pages_that_are_not_there():
     assert same_codes(c.dev[0], values) and int(st) == 2
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("nH,nKV,hd,page,block,norm,turn,half", [(4, 2, 64, 16, 16, True, True, True), (3, 1, 16, 8, 8, False, True, False),
+                                                                (6, 2, 128, 32, 16, True, False, True), (2, 2, 80, 16, 8, True, True, False),
+                                                                (2, 1, 256, 64, 64, False, False, True)])
+@pytest.mark.parametrize("parts", [0, 1, 3])
+def test_rope_and_write_in_one_launch(kind, nH, nKV, hd, page, block, norm, turn, half, parts):
+    """Bit for bit what rope_cache and cache_write_q8 give one after the other; padding rows; a page that is not there."""
+    c = Cache([1] * 6, [0, 1, block - 1, block, 3 * block + 5, 70], nKV, hd, page, block, kind, seed=hd)
+    n, width = 8, (nH + 2 * nKV) * hd
+    qkv = rnd(n, width, seed=1, std=2.0) if parts == 0 else rnd(parts, n, width, dtype=torch.float32, seed=1)
+    w = [1 + 0.1 * rnd(hd, dtype=torch.float32, seed=s) if norm else None for s in (2, 3)]
+    inv = 10000.0 ** (-torch.arange(hd // 2, device=DEV).float() / (hd // 2)) if turn else None
+    row_entry, positions = i32([0, 1, 2, -1, 3, 4, 5, -1]), i32([0, 1, block - 1, 0, block, 3 * block + 5, 70, 0])
+    cu, st = i32([0, 1, 2, 4, 5, 6, 8]), torch.zeros(1, dtype=torch.int32, device=DEV)
+    q1, q2 = (torch.full((n, nH * hd), 9.0, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    k, v = (torch.zeros(n, nKV, 1, hd, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    twin = [t.clone() for t in c.dev]
+    # (rope_cache takes a stack of one part for a bfloat16 tensor: it is given that part, rounded as the stack would be)
+    ops().rope_cache(qkv[0].bfloat16() if parts == 1 else qkv, q1, *w, inv, half, 1.0, k, v, None, positions, row_entry, nH, nKV, hd, 1e-5, st)
+    for r, e in enumerate(row_entry.tolist()):                               # (row by row: the entries' rows do not follow one another here)
+        if e >= 0:
+            ops().cache_write_q8(k[r:r + 1].view(1, -1), v[r:r + 1].view(1, -1), *twin, c.table[e:e + 1].contiguous(), i32([0]), i32([0, 1]),
+                                 c.ctx_d[e:e + 1].contiguous(), st)
+    ops().rope_cache_q8(qkv, q2, *w, inv, half, 1.0, *c.args(), positions, row_entry, nH, 1e-5, st)
+    assert torch.equal(q1, q2) and int(st) == 0
+    for a, b in zip(c.dev, twin):
+        raw = torch.uint8 if a.element_size() == 1 else torch.int32
+        assert torch.equal(a.view(raw), b.view(raw))
+    c.table[1, 0] = -1
+    before = [t.clone() for t in c.dev]
+    ops().rope_cache_q8(qkv, q2, *w, inv, half, 1.0, *c.args(), positions, row_entry, nH, 1e-5, st)
+    page = int(c.table_host[1, 0])
+    assert int(st) == 2 and all(torch.equal(a.view(torch.uint8)[page], b.view(torch.uint8)[page]) for a, b in zip(c.dev, before))
+
+
 # ------------------------------------------------------------------------------------------------ attention
 def check_rows(got, want, bound, rows=None):
     err = (got.cpu().double() - want).abs()
