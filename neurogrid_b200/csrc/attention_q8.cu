@@ -258,10 +258,10 @@ struct DcArgs {
     float scale;
 };
 constexpr int TURN = DC_WARPS * GROUP;                               // keys of a turn of the four warps
-// turns of an entry's segments (0: not a single token, or a row that the buffers do not hold)
+// turns of an entry's segments (0: not a single token, or a row that the buffers, or a position that the table, do not hold)
 __device__ __forceinline__ int dc_turns(const DcArgs& a, int e) {
     const int row = a.cu_q[e], pos = a.ctx_before[e];
-    if (a.cu_q[e + 1] - row != 1 || row < 0 || row >= a.n_rows || pos < 0) return 0;
+    if (a.cu_q[e + 1] - row != 1 || row < 0 || row >= a.n_rows || pos < 0 || pos > a.c.last_key) return 0;
     const int lo = a.window > 0 ? max(0, pos - a.window + 1) & ~(GROUP - 1) : 0;
     return (pos - lo) / TURN + 1;
 }
@@ -584,7 +584,7 @@ attn_prefill_q8_kernel(const PfArgs a) {
     ng_pdl_wait();
     const int G = a.nH / a.c.nKV;
     const int r0 = (gridDim.y - 1 - blockIdx.y) * PF_ROWS;
-    if (q0 < 0 || ctx < 0 || r0 >= qlen * G || (a.skip_single && a.cu_q[e + 1] - q0 == 1)) return;
+    if (q0 < 0 || ctx < 0 || ctx > a.c.last_key || r0 >= qlen * G || (a.skip_single && a.cu_q[e + 1] - q0 == 1)) return;
     const int rows_here = min(PF_ROWS, qlen * G - r0);
     const int pos_first = ctx + r0 / G, pos_last = ctx + (r0 + rows_here - 1) / G;
     const int key_lo = a.window > 0 ? max(0, pos_first - a.window + 1) : 0;
@@ -804,7 +804,7 @@ NG_EXPORT int ng_attn_decode_q8(const NgAttnQ8* call, cudaStream_t stream) {
     else if (nt == 1) DC_KINDS(1, 8);
     else if (block >= 16) DC_KINDS(DC_NT_MAX, 16);
     else DC_KINDS(DC_NT_MAX, 8);
-    if (n_splits > 1) return q8_merge(c.scratch, c.cu_q, c.out, nH, n_splits, c.n_rows, n_entries, 1, 1, 1, stream);
+    if (n_splits > 1) return q8_merge(c, a.c, 1, 1, 1, stream);
     return ng_launch_status();
 }
 
@@ -828,7 +828,6 @@ NG_EXPORT int ng_attn_prefill_q8(const NgAttnQ8* call, cudaStream_t stream) {
     } while (0)
     if (kind == NG_Q8_E4M3) PF_GO(NG_Q8_E4M3);
     else PF_GO(NG_Q8_INT8);
-    if (c.n_splits > 1)
-        return q8_merge(c.scratch, c.cu_q, c.out, c.n_heads, c.n_splits, c.n_rows, c.n_entries, c.skip_single ? 2 : 1, 0x7fffffff, c.max_q, stream);
+    if (c.n_splits > 1) return q8_merge(c, a.c, c.skip_single ? 2 : 1, 0x7fffffff, c.max_q, stream);
     return ng_launch_status();
 }

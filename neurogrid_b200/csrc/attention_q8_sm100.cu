@@ -121,7 +121,7 @@ attn_prefill_q8_sm100_kernel(const Params p) {
     const int q0 = p.cu_q[e], q1 = p.cu_q[e + 1], qlen = min(q1, p.n_rows) - q0, ctx = p.ctx_before[e];
     const int G = p.nH / p.c.nKV;
     const int r0 = (gridDim.y - 1 - blockIdx.y) * BR;
-    if (q0 < 0 || ctx < 0 || r0 >= qlen * G || (p.skip_single && q1 - q0 == 1)) {
+    if (q0 < 0 || ctx < 0 || ctx > p.c.last_key || r0 >= qlen * G || (p.skip_single && q1 - q0 == 1)) {
         ng_pdl_wait();                                         // (a launch none of whose blocks waited would end before the one before it)
         return;
     }
@@ -565,7 +565,6 @@ NG_EXPORT int ng_attn_prefill_q8_sm100(const NgAttnQ8* call, cudaStream_t stream
     } while (0)
     if (kind == NG_Q8_E4M3) Q8P_GO(NG_Q8_E4M3);
     else Q8P_GO(NG_Q8_INT8);
-    if (c.n_splits > 1)
-        return q8_merge(c.scratch, c.cu_q, c.out, c.n_heads, c.n_splits, c.n_rows, c.n_entries, c.skip_single ? 2 : 1, 0x7fffffff, c.max_q, stream);
+    if (c.n_splits > 1) return q8_merge(c, p.c, c.skip_single ? 2 : 1, 0x7fffffff, c.max_q, stream);
     return ng_launch_status();
 }

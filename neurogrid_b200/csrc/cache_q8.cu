@@ -214,7 +214,7 @@ struct NgRopeCacheQ8 {
     const int *table, *positions, *row_entry;
     int* status;
     long long part_stride;
-    int n_part, half_pairing, table_stride, n_rows, n_heads, n_kv, head_dim, page_size, block, num_pages, kind;
+    int n_part, half_pairing, table_stride, n_entries, n_rows, n_heads, n_kv, head_dim, page_size, block, num_pages, kind;
     float pos_scale, eps;
 };
 #define RQ_WARPS 4
@@ -244,7 +244,7 @@ rope_cache_q8_kernel(const NgRopeCacheQ8 c, int ps_log2, int bl_log2) {
     ng_pdl_wait();
     if (head >= c.n_heads + 2 * c.n_kv) return;
     __nv_bfloat16* q = reinterpret_cast<__nv_bfloat16*>(c.q_out) + ((size_t)row * c.n_heads + head) * hd;
-    if (entry < 0) {                                // padding row: defined output, no cache write
+    if (entry < 0 || entry >= c.n_entries) {        // padding row: defined output, no cache write
         if (is_q)
             for (int j = lane; j < hd; j += 32) q[j] = __float2bfloat16(0.f);
         return;

@@ -33,6 +33,7 @@ struct Cache {
     const float *ks, *vs;                // [pages, nKV, page / block]
     const int* table;
     int table_stride, num_pages, nKV, ps_log2, bl_log2;
+    int last_key;                        // the last position that a row of the table has a place for
 };
 
 // BYTES of codes from a page; no line of the first-level cache is taken (they are read once).  Not moved above the wait.
@@ -56,15 +57,15 @@ __device__ __forceinline__ void ld_codes(uint32_t* w, const unsigned char* p) {
 constexpr int MG_EACH = (HD + 63) / 64;                              // pairs of dimensions a lane has
 template <bool WIDE>
 __global__ void __launch_bounds__(MG_WARPS * 32)
-attn_q8_merge_kernel(const float* __restrict__ scratch, const int* __restrict__ cu_q, bf16* __restrict__ out, int nH, int room, int n_rows,
-                     int least, int most) {
+attn_q8_merge_kernel(const float* __restrict__ scratch, const int* __restrict__ cu_q, const int* __restrict__ ctx_before, int last_key,
+                     bf16* __restrict__ out, int nH, int room, int n_rows, int least, int most) {
     __shared__ float part_s[WIDE ? MG_WARPS : 1][HD + 2];
     ng_pdl_trigger();
     const int e = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int head = WIDE ? blockIdx.x : blockIdx.x * MG_WARPS + warp;
-    const int q0 = cu_q[e], n = cu_q[e + 1] - q0;
+    const int q0 = cu_q[e], n = cu_q[e + 1] - q0, ctx = ctx_before[e];
     ng_pdl_wait();
-    if (n < least || n > most || (!WIDE && head >= nH)) return;
+    if (n < least || n > most || q0 < 0 || ctx < 0 || ctx > last_key || (!WIDE && head >= nH)) return;       // (entries that left no records)
     scratch = ng_after_wait(scratch);
     constexpr int STEP = WIDE ? MG_WARPS : 1;
     for (int r = q0 + blockIdx.z; r < min(q0 + n, n_rows); r += gridDim.z) {
@@ -146,17 +147,6 @@ attn_q8_merge_kernel(const float* __restrict__ scratch, const int* __restrict__ 
     }
 }
 
-static int q8_merge(const float* scratch, const int* cu_q, void* out, int nH, int n_splits, int n_rows, int n_entries, int least, int most,
-                 int rows, cudaStream_t stream) {
-    const int z = rows < 1 ? 1 : rows > 65535 ? 65535 : rows;
-    if (n_splits > 8 && (long long)n_entries * nH * z < 1024)        // many runs of few rows
-        NG_LAUNCH((attn_q8_merge_kernel<true>), dim3(nH, n_entries, z), MG_WARPS * 32, 0, stream, scratch, cu_q, (bf16*)out, nH, n_splits, n_rows, least, most);
-    else
-        NG_LAUNCH((attn_q8_merge_kernel<false>), dim3((nH + MG_WARPS - 1) / MG_WARPS, n_entries, z), MG_WARPS * 32, 0, stream, scratch, cu_q, (bf16*)out,
-                  nH, n_splits, n_rows, least, most);
-    return ng_launch_status();
-}
-
 static int log2_exact(int n) {               // -1: not a power of two
     if (n <= 0 || (n & (n - 1))) return -1;
     int l = 0;
@@ -178,9 +168,22 @@ struct NgAttnQ8 {
 // What every entry refuses; fills in the cache.
 static bool attn_q8_args(const NgAttnQ8& c, Cache& to) {
     to = Cache{(const unsigned char*)c.k_pages, (const unsigned char*)c.v_pages, c.k_scales, c.v_scales, c.table, c.table_stride, c.num_pages,
-               c.n_kv, log2_exact(c.page_size), log2_exact(c.block)};
+               c.n_kv, log2_exact(c.page_size), log2_exact(c.block), (int)((long long)c.table_stride * c.page_size - 1)};
     return c.head_dim == HD && c.n_heads > 0 && c.n_kv > 0 && c.n_heads % c.n_kv == 0 && to.ps_log2 >= 3 && to.bl_log2 >= 3 &&
-           to.bl_log2 <= to.ps_log2 && c.table_stride > 0 && c.num_pages > 0 && (long long)c.n_kv * c.page_size * HD <= 0x7fffffff &&
+           to.bl_log2 <= to.ps_log2 && c.table_stride > 0 && (long long)c.table_stride * c.page_size <= 1 << 30 && c.num_pages > 0 &&
+           (long long)c.n_rows * c.n_heads <= 1 << 30 && (long long)c.n_kv * c.page_size * HD <= 0x7fffffff &&
            !(((uintptr_t)c.k_pages | (uintptr_t)c.v_pages) & 15) && (c.kind == NG_Q8_E4M3 || c.kind == NG_Q8_INT8) && c.window >= 0 &&
            c.n_splits >= 1 && (c.n_splits == 1 || (c.scratch && !((uintptr_t)c.scratch & 15)));
+}
+
+// least .. most: the rows that an entry brings to have records
+static int q8_merge(const NgAttnQ8& c, const Cache& cache, int least, int most, int rows, cudaStream_t stream) {
+    const int z = rows < 1 ? 1 : rows > 65535 ? 65535 : rows;
+    if (c.n_splits > 8 && (long long)c.n_entries * c.n_heads * z < 1024)        // many runs of few rows
+        NG_LAUNCH((attn_q8_merge_kernel<true>), dim3(c.n_heads, c.n_entries, z), MG_WARPS * 32, 0, stream, c.scratch, c.cu_q, c.ctx_before,
+                  cache.last_key, (bf16*)c.out, c.n_heads, c.n_splits, c.n_rows, least, most);
+    else
+        NG_LAUNCH((attn_q8_merge_kernel<false>), dim3((c.n_heads + MG_WARPS - 1) / MG_WARPS, c.n_entries, z), MG_WARPS * 32, 0, stream, c.scratch,
+                  c.cu_q, c.ctx_before, cache.last_key, (bf16*)c.out, c.n_heads, c.n_splits, c.n_rows, least, most);
+    return ng_launch_status();
 }

@@ -451,7 +451,7 @@ def q8_libraries(head_dim: int):
 Q8_KINDS = {torch.float8_e4m3fn: 0, torch.int8: 1}
 # the launchers' arguments (NgCacheWriteQ8, NgRopeCacheQ8, NgPool, NgAttnQ8), packed: a ctypes call pays for every argument
 _Q8_WRITE = struct.Struct("@11P2q10i")
-_Q8_ROPE = struct.Struct("@13Pq11i2f")
+_Q8_ROPE = struct.Struct("@13Pq12i2f")
 _Q8_POOL = struct.Struct("@Pq2i")
 _Q8_ATTENTION = struct.Struct("@12P14if")
 _Q8_CALL = [ctypes.c_char_p, _c_void_p]
@@ -550,8 +550,8 @@ def rope_cache_q8(qkv: torch.Tensor, q_out: torch.Tensor, q_weight: Optional[tor
     at = [0 if t is None else _on(what, t, here) for t in (qkv, q_out, q_weight, k_weight, inv_freq, k_pages, v_pages, k_scales, v_scales,
                                                            table, positions, row_entry, status)]
     f = _fn("cache_q8", "ng_rope_cache_q8", _Q8_CALL)
-    _check(f(_Q8_ROPE.pack(*at, stride, n_part if qkv.dtype is torch.float32 else 0, int(half_pairing), table.shape[1], n, n_heads, n_kv, hd,
-                           page_size, block, num_pages, kind, pos_scale, eps), _stream()), what)
+    _check(f(_Q8_ROPE.pack(*at, stride, n_part if qkv.dtype is torch.float32 else 0, int(half_pairing), table.shape[1], table.shape[0], n, n_heads, n_kv,
+                           hd, page_size, block, num_pages, kind, pos_scale, eps), _stream()), what)
 
 
 def copy_pages(pools, src, dst) -> None:

@@ -197,6 +197,13 @@ def test_rope_and_write_in_one_launch(kind, nH, nKV, hd, page, block, norm, turn
     for a, b in zip(c.dev, twin):
         raw = torch.uint8 if a.element_size() == 1 else torch.int32
         assert torch.equal(a.view(raw), b.view(raw))
+    row_entry[6] = len(c.q_lens)                                             # (an entry that the table has no row for counts as padding)
+    twin = [t.clone() for t in c.dev]
+    ops().rope_cache_q8(qkv, q2, *w, inv, half, 1.0, *c.args(), positions, row_entry, nH, 1e-5, st)
+    assert bool((q2[6] == 0).all()) and torch.equal(q1[:6], q2[:6]) and int(st) == 0
+    for t, b in zip(twin, c.dev):
+        page = int(c.table_host[5, 70 // c.page])
+        assert torch.equal(t.view(torch.uint8)[page], b.view(torch.uint8)[page])
     c.table[1, 0] = -1
     before = [t.clone() for t in c.dev]
     ops().rope_cache_q8(qkv, q2, *w, inv, half, 1.0, *c.args(), positions, row_entry, nH, 1e-5, st)
@@ -215,7 +222,7 @@ def check_rows(got, want, bound, rows=None):
 
 def run_decode(c, q, nH, window, scale, splits, slopes=None, max_ctx=None):
     out = torch.full_like(q, 7.0)
-    n = ops().attn_q8_scratch_floats(q.shape[0], nH, c.dev[0].shape[3], splits)
+    n = ops().attn_q8_scratch_floats(len(c.q_lens), nH, c.dev[0].shape[3], splits)
     scratch = torch.full((n,), math.nan, device=DEV) if n else None
     longest = max(a + b for a, b in zip(c.q_lens, c.ctx)) if max_ctx is None else max_ctx
     ops().attn_decode_q8(q, *c.args(), c.cu, c.ctx_d, out, scratch, len(c.q_lens), nH, window, scale, splits, longest, slopes)
@@ -419,6 +426,71 @@ def test_many_entries_and_longer_portions():
     got = run_decode(c, q, 16, None, 0.125, 1)
     check_rows(got, want, bound, list(range(37)))
     check_rows(out, want, bound, list(range(37, c.rows)))
+
+
+@pytest.mark.parametrize("hd", [48, 64])
+@pytest.mark.parametrize("splits", [1, 3])
+def test_entries_behind_their_table_or_in_front_of_it_are_left_alone(hd, splits):
+    """A context that no row of the table holds, or of less than nothing: the rows stay as they were, the others are right."""
+    q = rnd(5, 4 * hd, seed=6)
+    c = Cache([1, 1, 1, 1, 1], [40, 9, 70, 0, 100], 2, hd, 16, 16, E4M3, seed=4)
+    want, bound = ref.attention(q, *c.args(), c.cu_host, c.ctx, 4, None, 0.125)
+    c.ctx_d = i32([40, -1, 70, 2 ** 31 - 1, c.table.shape[1] * 16])
+    got = run_decode(c, q, 4, None, 0.125, splits)
+    check_rows(got, want, bound, [0, 2])
+    assert bool((got[[1, 3, 4]] == 7.0).all())
+    q = rnd(60, 4 * hd, seed=6)
+    c = Cache([20, 7, 30, 3], [40, 9, 70, 5], 2, hd, 16, 16, E4M3, seed=4)
+    want, bound = ref.attention(q, *c.args(), c.cu_host, c.ctx, 4, None, 0.125)
+    c.ctx_d = i32([40, -1, 70, c.table.shape[1] * 16])
+    got = run_prefill(c, q, 4, None, 0.125, splits)
+    check_rows(got, want, bound, [*range(20), *range(27, 57)])
+    assert bool((got[[*range(20, 27), *range(57, 60)]] == 7.0).all())
+
+
+@pytest.mark.parametrize("splits", [2, 9])
+def test_decode_shares_of_many_entries(splits):
+    """More entries than a warp looks over at once, of very different lengths, some with no single token."""
+    lens = [1 if i % 7 else (0, 2)[i % 2] for i in range(100)]
+    ctx = [(i * i * 13) % 900 if i % 5 else 0 for i in range(100)]
+    c = Cache(lens, ctx, 2, 64, 16, 16, E4M3, seed=8)
+    q = rnd(c.rows, 8 * 64, seed=3)
+    single = [c.cu_host[e] for e, n in enumerate(lens) if n == 1]
+    want, bound = ref.attention(q, *c.args(), c.cu_host, c.ctx, 8, None, 0.125)
+    got = run_decode(c, q, 8, None, 0.125, splits)
+    check_rows(got, want, bound, single)
+    assert bool((got[[r for r in range(c.rows) if r not in single]] == 7.0).all())
+
+
+def test_the_integer_that_the_writer_never_stores():
+    """-128 stands for -128 times the scale."""
+    c = Cache([1, 5], [60, 30], 2, 64, 16, 16, INT8, seed=6)
+    for x in (c.k, c.v):
+        x[torch.rand(x.shape, generator=torch.Generator().manual_seed(1)) < 0.1] = -128
+    c.dev[0], c.dev[1] = c.k.to(DEV), c.v.to(DEV)
+    q = rnd(c.rows, 4 * 64, seed=3)
+    want, bound = ref.attention(q, *c.args(), c.cu_host, c.ctx, 4, None, 0.125)
+    check_rows(run_decode(c, q, 4, None, 0.125, 1), want, bound, [0])
+    check_rows(run_prefill(c, q, 4, None, 0.125), want, bound)
+
+
+def test_calls_on_two_streams_at_once():
+    """Each with outputs and scratch of its own: nothing of a call is kept anywhere else."""
+    c = Cache([1] * 8 + [200], [700 + 40 * i for i in range(8)] + [300], 2, 64, 16, 16, E4M3, seed=6)
+    qs = [rnd(c.rows, 8 * 64, seed=10 + i) for i in range(2)]
+    wants = [ref.attention(q, *c.args(), c.cu_host, c.ctx, 8, None, 0.125) for q in qs]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(3):
+        for i, (s, q) in enumerate(zip(streams, qs)):
+            with torch.cuda.stream(s):
+                got[i].append((run_decode(c, q, 8, None, 0.125, 6), run_prefill(c, q, 8, None, 0.125, 2, True)))
+    torch.cuda.synchronize()
+    for i, (want, bound) in enumerate(wants):
+        for single, portion in got[i]:
+            check_rows(single, want, bound, list(range(8)))
+            check_rows(portion, want, bound, list(range(8, c.rows)))
 
 
 # ------------------------------------------------------------------------------------------------ copies
