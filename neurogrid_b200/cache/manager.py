@@ -138,9 +138,10 @@ class CacheManager:
         return [max(0, end_pages - len(t)) for t in r.tables]
 
     def pages_freed_first(self, req_id) -> List[int]:
+        """Per group, pages that become free when the request gives back those its window has passed (not those that a fork still holds)."""
         r = self._req[req_id]
-        return [max(0, min(self._passed(g, r.length), len(r.tables[g])) - max(r.first_live[g], self._kept(g)))
-                for g in range(len(self.pools))]
+        return [sum(pool.holders(p) == 1 for p in r.tables[g][max(r.first_live[g], self._kept(g)):self._passed(g, r.length)])
+                for g, pool in enumerate(self.pools)]
 
     def can_extend(self, req_id, n_new: int) -> bool:
         r = self._req[req_id]

@@ -88,8 +88,8 @@ class Engine:
         if n < 1 or (rng_keys is not None and len(rng_keys) != n):
             raise ValueError("n is at least 1, with a random stream for each sample or for none")
         ids = list(range(self._next_id, self._next_id + n))
-        reqs = [self._request(prompt, params, i, rng_keys[j] if rng_keys is not None else None) for j, i in enumerate(ids)]
         self._next_id += n
+        reqs = [self._request(prompt, params, i, rng_keys[j] if rng_keys is not None else None) for j, i in enumerate(ids)]
         self._requests.update(zip(ids, reqs))
         self.scheduler.add_samples(reqs[0], reqs[1:])
         return ids

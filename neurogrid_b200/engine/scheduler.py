@@ -186,8 +186,7 @@ class Scheduler:
             if stalled is not None:
                 victim = self.running[-1]
                 if len(self.running) == 1:
-                    self._fail(victim, "cache_full")
-                    plan.failed.append(victim)
+                    plan.failed += self._fail(victim, "cache_full")
                 else:
                     self._preempt(victim)
                     plan.preempted.append(victim)
@@ -203,8 +202,7 @@ class Scheduler:
                 if req.pending + len(self.running) * ps > self._room(None, free):
                     if not self.running:                     # the whole pool is free and it still does not fit
                         self.waiting.popleft()
-                        self._fail(req, "cache_full")
-                        plan.failed.append(req)
+                        plan.failed += self._fail(req, "cache_full")
                         continue
                     break
                 n = self._portion(req, budget)
@@ -226,15 +224,16 @@ class Scheduler:
         self.preemptions += 1
         self.waiting.appendleft(req)
 
-    def _fail(self, req: Request, reason: str) -> None:
+    def _fail(self, req: Request, reason: str) -> List[Request]:
+        """The request ends, and with it the samples that wait for its prompt (they would fail for the same reason); returns them all."""
         if req in self.running:
             self.running.remove(req)
         if self.cache.is_live(req.id):
             self.cache.release(req.id)
-        req.state, req.finish_reason = FINISHED, reason
-        for r in req.forks:                                      # (they would fail for the same reason)
+        ended, req.forks = [req] + req.forks, []
+        for r in ended:
             r.state, r.finish_reason = FINISHED, reason
-        req.forks = []
+        return ended
 
     # ------------------------------------------------------------------ one step ahead
     def commit_ahead(self, plan: StepPlan) -> None:

@@ -61,6 +61,20 @@ def test_fork_shares_full_pages_and_copies_the_last():
     m.check()
 
 
+def test_pages_that_a_fork_still_holds_are_not_counted_on():
+    m = mgr(pages=(4,), windows=(8,), page_size=8)
+    m.admit("a")
+    m.extend("a", 24); m.advance("a", 24)                      # three pages, of which the window has passed two
+    m.fork("a", "b")
+    assert m.pages_free() == [1] and m.pages_freed_first("a") == [0]
+    assert m.can_extend("a", 8) and not m.can_extend("a", 9)   # (a page is free; giving back two that b holds frees none)
+    m.extend("a", 8); m.advance("a", 8)
+    m.check()
+    assert m.pages_free() == [0] and m.pages_freed_first("b") == [2] and m.can_extend("b", 9)
+    m.extend("b", 9); m.advance("b", 9)
+    m.check()
+
+
 def test_fork_is_all_or_nothing():
     m = mgr(pages=(4, 3), windows=(None, None), max_requests=3)
     m.admit("a")
@@ -176,7 +190,7 @@ def test_samples_that_find_no_slot_read_the_prompt_themselves():
     t = Scheduler(mgr(pages=(1,)), max_tokens_per_step=64, max_requests=2)
     bad = [Request(i, list(range(30)), SamplingParams()) for i in range(2)]
     t.add_samples(bad[0], bad[1:])
-    assert t.plan().failed == [bad[0]] and all(r.finish_reason == "cache_full" for r in bad) and not t.has_work()
+    assert t.plan().failed == bad and all(r.finish_reason == "cache_full" for r in bad) and not t.has_work()
 
 
 def copy_pages(pools, src, dst):

@@ -210,6 +210,20 @@ def test_samples_read_their_prompt_once(model_dirs):
     assert 44 + 4 * 6 <= eng.runner.tokens_run <= 44 + 4 * 7
 
 
+def test_samples_beside_requests_with_ids_of_their_own(model_dirs):
+    """An id that a caller has taken is in the way once, as it is for a single request; samples of a prompt that cannot be served all end."""
+    cfg, _ = plain_lfm2.load_plain(model_dirs["B"])
+    eng = _engine(model_dirs["B"], "B", dtype="float32", max_requests=4, num_pages=4)
+    eng.add_request([1, 2, 3], SamplingParams(max_new_tokens=2), request_id=1)
+    with pytest.raises(KeyError):
+        eng.add_samples([4, 5, 6], 2)
+    ids = eng.add_samples([4, 5, 6], 2, SamplingParams(max_new_tokens=2))
+    assert sorted(r.id for r in eng.run()) == sorted([1] + ids)
+    ids = eng.add_samples(_tokens(60, cfg["vocab_size"], 1), 3)
+    done = eng.run()
+    assert sorted(r.id for r in done) == ids and all(r.finish_reason == "cache_full" for r in done)
+
+
 @pytest.mark.parametrize("kind", ["e4m3", "int8"])
 def test_samples_over_a_cache_in_8_bits(model_dirs, kind):
     """A fork copies codes and scales: greedy samples of one prompt are one token list."""
