@@ -8,12 +8,14 @@ step, H = model width.
 """
 from __future__ import annotations
 
+import array
 import ctypes
 import functools
 import os
 import struct
 from typing import Optional, Tuple
 
+import numpy as np
 import torch
 
 from . import build
@@ -457,9 +459,16 @@ _Q8_ATTENTION = struct.Struct("@12P14if")
 _Q8_CALL = [ctypes.c_char_p, _c_void_p]
 
 
+def _q8_fn(lib_name: str, symbol: str, head_dim: Optional[int] = None):
+    f = _fn_cache.get((symbol, head_dim))
+    if f is None:
+        f = _fn_cache[symbol, head_dim] = _fn(lib_name, symbol, _Q8_CALL, None if head_dim is None else {"NG_HEAD_DIM": head_dim})
+    return f
+
+
 def _q8_cache(what: str, k_pages, v_pages, k_scales, v_scales, table):
-    """(kind, pages, KV heads, page, head size, block) of a cache in 8 bits, after its checks."""
-    dtype, shape, of_scales = k_pages.dtype, k_pages.shape, k_scales.shape
+    """(kind, pages, KV heads, page, head size, block, rows of the table, pages of a row) of a cache in 8 bits, after its checks."""
+    dtype, shape, of_scales, of_table = k_pages.dtype, k_pages.shape, k_scales.shape, table.shape
     kind = Q8_KINDS.get(dtype)
     if kind is None or v_pages.dtype is not dtype:
         raise KernelError(f"{what}: pages in 8 bits are float8_e4m3fn or int8 (keys and values alike), got {dtype} and {v_pages.dtype}")
@@ -471,13 +480,18 @@ def _q8_cache(what: str, k_pages, v_pages, k_scales, v_scales, table):
         raise KernelError(f"{what}: scales are [pages, KV heads, page / block], keys' and values' alike")
     if k_scales.dtype is not torch.float32 or v_scales.dtype is not torch.float32:
         raise KernelError(f"{what}: scales must be float32")
-    _i32(table, "table")
     block = page_size // of_scales[2]
     if page_size & (page_size - 1) or block & (block - 1) or block < 8:
         raise KernelError(f"{what}: pages and blocks are powers of two, blocks of at least 8 tokens; got {page_size} and {block}")
-    if hd % 16 or table.dim() != 2:
+    if hd % 16 or len(of_table) != 2:
         raise KernelError(f"{what}: head sizes are multiples of 16 and the table is [entries, pages]")
-    return kind, num_pages, n_kv, page_size, hd, block
+    return kind, num_pages, n_kv, page_size, hd, block, *of_table
+
+
+def _i32s(what: str, *tensors) -> None:
+    for t in tensors:
+        if t.dtype is not torch.int32:
+            _i32(t, f"{what}: a table or a description of the batch")
 
 
 def _current(what: str, t: torch.Tensor) -> int:
@@ -487,14 +501,18 @@ def _current(what: str, t: torch.Tensor) -> int:
     return _current_device() if _current_device is not None else torch.cuda.current_device()
 
 
-def _on(what: str, t: torch.Tensor, here: int) -> int:
-    """The address of a contiguous tensor of device ``here``."""
-    if t.get_device() != here:
-        _ptr(t, what)
-        raise KernelError(f"{what}: a tensor is on {t.device}, the current device is cuda:{here}")
-    if not t.is_contiguous():
-        raise KernelError(f"{what}: a tensor must be contiguous")
-    return t.data_ptr()
+def _on(what: str, here: int, *tensors):
+    """The addresses of contiguous tensors of device ``here`` (0 for None)."""
+    at = []
+    for t in tensors:
+        if t is None:
+            at.append(0)
+            continue
+        if t.get_device() != here or not t.is_contiguous():
+            _ptr(t, what)
+            raise KernelError(f"{what}: a tensor is on {t.device}, the current device is cuda:{here}")
+        at.append(t.data_ptr())
+    return at
 
 
 def cache_write_q8(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, k_scales: torch.Tensor,
@@ -510,23 +528,24 @@ def cache_write_q8(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pa
     scale.  Codes are rounded to nearest, ties to even; infinities become the largest code, NaN stays NaN in e4m3 and becomes 0 in
     int8.  Places of a page that no row goes to stay as they were.  A page that is not in the table sets the bad-page bit."""
     what = "cache_write_q8"
-    kind, num_pages, n_kv, page_size, hd, block = _q8_cache(what, k_pages, v_pages, k_scales, v_scales, table)
+    kind, num_pages, n_kv, page_size, hd, block, table_rows, stride = _q8_cache(what, k_pages, v_pages, k_scales, v_scales, table)
     shape = k.shape
     if len(shape) != 2 or v.shape != shape or shape[1] != n_kv * hd or k.dtype is not v.dtype:
-        raise KernelError(f"{what}: keys {tuple(k.shape)} and values {tuple(v.shape)} do not fit the pages")
-    act, n_entries = _act_flag(k, "keys"), ctx_before.numel()
-    _i32(row_entry, "row_entry"), _i32(cu_q, "cu_q"), _i32(ctx_before, "ctx_before"), _i32(status, "status")
-    if row_entry.numel() != shape[0] or cu_q.numel() != n_entries + 1 or table.shape[0] < n_entries:
-        raise KernelError(f"{what}: the batch description does not fit {shape[0]} rows of {n_entries} entries")
+        raise KernelError(f"{what}: keys {tuple(shape)} and values {tuple(v.shape)} do not fit the pages")
+    act, n_entries, n = _act_flag(k, "keys"), ctx_before.numel(), shape[0]
+    _i32s(what, table, row_entry, cu_q, ctx_before, status)
+    if row_entry.numel() != n or cu_q.numel() != n_entries + 1 or table_rows < n_entries:
+        raise KernelError(f"{what}: the batch description does not fit {n} rows of {n_entries} entries")
     here = _current(what, k)
-    for t in (k, v):
-        if t.get_device() != here:
-            _on(what, t, here)
-    f = _fn("cache_q8", "ng_cache_write_q8", _Q8_CALL)
-    _check(f(_Q8_WRITE.pack(k.data_ptr(), v.data_ptr(), _on(what, k_pages, here), _on(what, v_pages, here), _on(what, k_scales, here),
-                            _on(what, v_scales, here), _on(what, table, here), _on(what, row_entry, here), _on(what, cu_q, here),
-                            _on(what, ctx_before, here), _on(what, status, here), _column_block(k, "keys"), _column_block(v, "values"),
-                            table.shape[1], shape[0], n_entries, n_kv, hd, page_size, block, num_pages, kind, act), _stream()), what)
+    at = _on(what, here, k_pages, v_pages, k_scales, v_scales, table, row_entry, cu_q, ctx_before, status)
+    (k_pitch, k_step), (v_pitch, v_step) = k.stride(), v.stride()
+    if k_step != 1 or v_step != 1 or k_pitch < shape[1] or v_pitch < shape[1] or k.get_device() != here or v.get_device() != here:
+        k_pitch, v_pitch = _column_block(k, "keys"), _column_block(v, "values")        # (one row may have any pitch)
+        if k.get_device() != here or v.get_device() != here:
+            raise KernelError(f"{what}: a tensor is on another device than the current one, cuda:{here}")
+    _check(_q8_fn("cache_q8", "ng_cache_write_q8")(
+        _Q8_WRITE.pack(k.data_ptr(), v.data_ptr(), *at, k_pitch, v_pitch, stride, n, n_entries, n_kv, hd, page_size, block, num_pages, kind, act),
+        _stream()), what)
 
 
 def rope_cache_q8(qkv: torch.Tensor, q_out: torch.Tensor, q_weight: Optional[torch.Tensor], k_weight: Optional[torch.Tensor],
@@ -536,22 +555,21 @@ def rope_cache_q8(qkv: torch.Tensor, q_out: torch.Tensor, q_weight: Optional[tor
     """``rope_cache`` and ``cache_write_q8`` in one launch, for a step whose entries bring one token each (no entry has two rows):
     qkv [N, (nH + 2 nKV) * hd] bfloat16 (or a float32 stack [S, N, ...] of partial sums), q -> q_out[N, nH * hd] bfloat16."""
     what = "rope_cache_q8"
-    kind, num_pages, n_kv, page_size, hd, block = _q8_cache(what, k_pages, v_pages, k_scales, v_scales, table)
+    kind, num_pages, n_kv, page_size, hd, block, table_rows, table_pages = _q8_cache(what, k_pages, v_pages, k_scales, v_scales, table)
     n = q_out.shape[0]
     if q_out.dtype is not torch.bfloat16 or q_out.shape != (n, n_heads * hd) or hd > 256:
         raise KernelError(f"{what}: q is bfloat16 [N, heads * head], heads of at most 256")
     n_part, stride = _stack(qkv, (n, (n_heads + 2 * n_kv) * hd), q_out.dtype, "rope_cache_q8 input")
     _f32(q_weight, "q norm weight"), _f32(k_weight, "k norm weight"), _f32(inv_freq, "inv_freq")
-    _i32(positions, "positions"), _i32(row_entry, "row_entry"), _i32(status, "status")
+    _i32s(what, table, positions, row_entry, status)
     if positions.numel() != n or row_entry.numel() != n or (inv_freq is not None and inv_freq.numel() != hd // 2) \
             or any(w is not None and w.numel() != hd for w in (q_weight, k_weight)):
         raise KernelError(f"{what}: shapes do not fit {n} rows of heads of {hd}")
     here = _current(what, qkv)
-    at = [0 if t is None else _on(what, t, here) for t in (qkv, q_out, q_weight, k_weight, inv_freq, k_pages, v_pages, k_scales, v_scales,
-                                                           table, positions, row_entry, status)]
-    f = _fn("cache_q8", "ng_rope_cache_q8", _Q8_CALL)
-    _check(f(_Q8_ROPE.pack(*at, stride, n_part if qkv.dtype is torch.float32 else 0, int(half_pairing), table.shape[1], table.shape[0], n, n_heads, n_kv,
-                           hd, page_size, block, num_pages, kind, pos_scale, eps), _stream()), what)
+    at = _on(what, here, qkv, q_out, q_weight, k_weight, inv_freq, k_pages, v_pages, k_scales, v_scales, table, positions, row_entry, status)
+    _check(_q8_fn("cache_q8", "ng_rope_cache_q8")(
+        _Q8_ROPE.pack(*at, stride, n_part if qkv.dtype is torch.float32 else 0, int(half_pairing), table_pages, table_rows, n, n_heads, n_kv,
+                      hd, page_size, block, num_pages, kind, pos_scale, eps), _stream()), what)
 
 
 def copy_pages(pools, src, dst) -> None:
@@ -559,35 +577,50 @@ def copy_pages(pools, src, dst) -> None:
     scales of a group of layers go in one launch).  ``src`` and ``dst`` are page numbers on the host: sequences, numpy arrays or CPU
     tensors.  No page may be written twice, or be read as well as written; a page may be read several times.  The numbers are checked
     before anything is launched, and travel with the launch: nothing has to be kept for it (a captured graph repeats the same copies)."""
-    import numpy as np
     what = "copy_pages"
-    if any(isinstance(x, torch.Tensor) and x.is_cuda for x in (src, dst)):
-        raise KernelError(f"{what}: page numbers are host values")
-    a, b = np.asarray(src), np.asarray(dst)
-    if a.size == 0 and b.size == 0:
-        return
-    if a.ndim != 1 or a.shape != b.shape or a.dtype.kind not in "iu" or b.dtype.kind not in "iu":
+    a, b = _page_numbers(what, src), _page_numbers(what, dst)
+    n = len(a) // 4
+    if len(a) != len(b):
         raise KernelError(f"{what}: src and dst are whole numbers, as many of one as of the other")
-    if a.dtype != np.int32 or b.dtype != np.int32:
-        if min(a.min(), b.min()) < 0 or max(a.max(), b.max()) > 0x7fffffff:
-            raise KernelError(f"{what}: {_ERR[6]}")
-    a, b = np.ascontiguousarray(a, dtype=np.int32), np.ascontiguousarray(b, dtype=np.int32)
     pools = [t for t in pools if t is not None]
-    if not pools:
+    if not n or not pools:
         return
     shapes = [t.shape for t in pools]
     if any(len(x) < 2 or x[1] != shapes[0][1] for x in shapes):
         raise KernelError(f"{what}: pools are [layers, pages, ...] with the same pages")
-    here, of_page = _current(what, pools[0]), []
-    for t, shape in zip(pools, shapes):
-        at, n = _on(what, t, here), t.numel()
-        if n:
-            of_page.append(_Q8_POOL.pack(at, n // (shape[0] * shape[1]) * t.element_size(), shape[0], shape[1]))
+    at, of_page = _on(what, _current(what, pools[0]), *pools), []
+    for t, x, base in zip(pools, shapes, at):
+        size = t.numel()
+        if size:
+            of_page.append(_Q8_POOL.pack(base, size // (x[0] * x[1]) * t.element_size(), x[0], x[1]))
     f = _fn("cache_q8", "ng_copy_pages", [ctypes.c_char_p, _c_int, ctypes.c_char_p, ctypes.c_char_p, _c_int, _c_void_p])
-    a, b, n = a.tobytes(), b.tobytes(), a.size
     for i in range(0, len(of_page), 8):
         part = of_page[i:i + 8]
         _check(f(b"".join(part), len(part), a, b, n, _stream()), what)
+
+
+def _page_numbers(what: str, x) -> bytes:
+    """Page numbers on the host as int32 values."""
+    if isinstance(x, torch.Tensor):
+        if x.is_cuda:
+            raise KernelError(f"{what}: page numbers are host values")
+        x = x.numpy()
+    try:
+        if isinstance(x, np.ndarray):
+            if x.ndim != 1 or (x.dtype.kind not in "iu" and x.size):
+                raise TypeError
+            if x.dtype == np.int32:
+                return x.tobytes()
+            if x.size > 64:                              # (numpy's reductions cost more than a short list)
+                if x.min() < 0 or x.max() > 0x7fffffff:
+                    raise OverflowError
+                return x.astype(np.int32).tobytes()
+            x = x.tolist()
+        return array.array("i", x).tobytes()
+    except TypeError:
+        raise KernelError(f"{what}: src and dst are whole numbers, as many of one as of the other") from None
+    except OverflowError:
+        raise KernelError(f"{what}: {_ERR[6]}") from None
 
 
 def attn_q8_scratch_floats(n_rows: int, n_heads: int, head_dim: int, n_splits: int) -> int:
@@ -630,8 +663,8 @@ def attn_prefill_q8_splits(q_lens, n_heads: int, n_kv_heads: int, head_dim: int,
 
 def _q8_attention(what, q, k_pages, v_pages, k_scales, v_scales, table, cu_q, ctx_before, out, scratch, n_entries, max_q, n_heads, window,
                   scale, skip_single, n_splits, slopes, n_records):
-    """Checks, and the launcher's arguments but for the status word's address: (head size, a function of that address that packs them)."""
-    kind, num_pages, n_kv, page_size, hd, block = _q8_cache(what, k_pages, v_pages, k_scales, v_scales, table)
+    """Checks, and the launcher's arguments: (head size, addresses but for the status word's, which comes last, the rest)."""
+    kind, num_pages, n_kv, page_size, hd, block, table_rows, stride = _q8_cache(what, k_pages, v_pages, k_scales, v_scales, table)
     shape = q.shape
     if q.dtype is not torch.bfloat16 or out.dtype is not torch.bfloat16:
         raise KernelError(f"{what} takes bfloat16 queries")
@@ -641,19 +674,19 @@ def _q8_attention(what, q, k_pages, v_pages, k_scales, v_scales, table, cu_q, ct
         raise KernelError(f"{what}: shapes do not fit")
     if n_splits < 1:
         raise KernelError(f"{what}: {n_splits} runs")
-    need = attn_q8_scratch_floats(n_records, n_heads, hd, n_splits)
-    if need and (scratch is None or scratch.numel() < need or scratch.dtype is not torch.float32):
-        raise KernelError(f"{what} needs {need} float32 values of scratch")
-    _i32(cu_q, "cu_q"), _i32(ctx_before, "ctx_before")
-    if cu_q.numel() < n_entries + 1 or ctx_before.numel() < n_entries or table.shape[0] < n_entries:
+    if n_splits > 1:
+        need = attn_q8_scratch_floats(n_records, n_heads, hd, n_splits)
+        if scratch is None or scratch.numel() < need or scratch.dtype is not torch.float32:
+            raise KernelError(f"{what} needs {need} float32 values of scratch")
+    else:
+        scratch = None
+    _i32s(what, table, cu_q, ctx_before)
+    if cu_q.numel() < n_entries + 1 or ctx_before.numel() < n_entries or table_rows < n_entries:
         raise KernelError(f"{what}: the batch description does not fit {n_entries} entries")
-    here = _current(what, q)
-    at = (_on(what, q, here), _on(what, k_pages, here), _on(what, v_pages, here), _on(what, k_scales, here), _on(what, v_scales, here),
-          _on(what, table, here), _on(what, cu_q, here), _on(what, ctx_before, here), _on(what, out, here), _on(what, scratch, here) if need else 0,
-          _slopes(slopes, n_heads) or 0)
-    rest = (table.shape[1], shape[0], n_entries, max_q, n_heads, n_kv, hd, page_size, block, num_pages, kind, window or 0, skip_single,
-            n_splits, scale)
-    return hd, lambda status: _Q8_ATTENTION.pack(*at, status, *rest)
+    at = _on(what, _current(what, q), q, k_pages, v_pages, k_scales, v_scales, table, cu_q, ctx_before, out, scratch)
+    at.append(_slopes(slopes, n_heads) or 0)
+    return hd, at, (stride, shape[0], n_entries, max_q, n_heads, n_kv, hd, page_size, block, num_pages, kind, window or 0, skip_single,
+                    n_splits, scale)
 
 
 def attn_decode_q8(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, k_scales: torch.Tensor, v_scales: torch.Tensor,
@@ -664,10 +697,9 @@ def attn_decode_q8(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     number of query heads a KV head.  The rows of other entries stay as they were.  ``n_splits`` (``attn_decode_q8_splits``) runs of
     the keys, planned for contexts of up to ``max_ctx`` (longer ones are right too); ``scratch`` holds ``attn_q8_scratch_floats`` (of
     ``n_entries``) float32 values when there is more than one."""
-    hd, pack = _q8_attention("attn_decode_q8", q, k_pages, v_pages, k_scales, v_scales, table, cu_q, ctx_before, out, scratch, n_entries, 1,
-                             n_heads, window, scale, 0, n_splits, slopes, n_entries)
-    f = _fn("attention_q8", "ng_attn_decode_q8", _Q8_CALL, {"NG_HEAD_DIM": hd})
-    _check(f(pack(0), _stream()), "attn_decode_q8")
+    hd, at, rest = _q8_attention("attn_decode_q8", q, k_pages, v_pages, k_scales, v_scales, table, cu_q, ctx_before, out, scratch, n_entries,
+                                 1, n_heads, window, scale, 0, n_splits, slopes, n_entries)
+    _check(_q8_fn("attention_q8", "ng_attn_decode_q8", hd)(_Q8_ATTENTION.pack(*at, 0, *rest), _stream()), "attn_decode_q8")
 
 
 def attn_prefill_q8(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, k_scales: torch.Tensor, v_scales: torch.Tensor,
@@ -677,15 +709,13 @@ def attn_prefill_q8(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     """Flash attention of the step's portions over a cache in 8 bits (``cache_write_q8``); their own keys are read from the cache too.
     Entries of one token are left to ``attn_decode_q8`` when ``skip_single``.  ``n_splits`` (``attn_prefill_q8_splits``) runs of every
     block's keys, merged through ``scratch`` (``attn_q8_scratch_floats`` of q's rows)."""
-    hd, pack = _q8_attention("attn_prefill_q8", q, k_pages, v_pages, k_scales, v_scales, table, cu_q, ctx_before, out, scratch, n_entries,
-                             max_q, n_heads, window, scale, int(bool(skip_single)), n_splits, slopes, q.shape[0])
-    if ATTN_BACKEND == "sm100" and hd in (64, 128) and scale > 0 and q.data_ptr() % 16 == 0 and out.data_ptr() % 16 == 0:
-        f = _fn("attention_q8_sm100", "ng_attn_prefill_q8_sm100", _Q8_CALL, {"NG_HEAD_DIM": hd})
-        packed = pack(_gemm_status(q.device).data_ptr())
+    hd, at, rest = _q8_attention("attn_prefill_q8", q, k_pages, v_pages, k_scales, v_scales, table, cu_q, ctx_before, out, scratch,
+                                 n_entries, max_q, n_heads, window, scale, int(bool(skip_single)), n_splits, slopes, q.shape[0])
+    if ATTN_BACKEND == "sm100" and hd in (64, 128) and scale > 0 and at[0] % 16 == 0 and at[8] % 16 == 0:
+        f, status = _q8_fn("attention_q8_sm100", "ng_attn_prefill_q8_sm100", hd), _gemm_status(q.device).data_ptr()
     else:
-        f = _fn("attention_q8", "ng_attn_prefill_q8", _Q8_CALL, {"NG_HEAD_DIM": hd})
-        packed = pack(0)
-    _check(f(packed, _stream()), "attn_prefill_q8")
+        f, status = _q8_fn("attention_q8", "ng_attn_prefill_q8", hd), 0
+    _check(f(_Q8_ATTENTION.pack(*at, status, *rest), _stream()), "attn_prefill_q8")
 
 
 # ----------------------------------------------------------------------------- attention with float32 weights
