@@ -16,6 +16,7 @@
 //
 // Keys that no row of the block sees, and keys whose page is not there, are stored as zeros (their codes may be NaN).  Every mbarrier wait
 // is bounded; a waiter that gives up sets a status bit and the block runs to its end.
+#include <cstddef>
 #include <type_traits>
 
 #include "sm100_common.cuh"
@@ -77,14 +78,17 @@ __device__ __forceinline__ void tmem_st16u(uint32_t taddr, const uint32_t (&v)[1
     tmem_st16(taddr, f);
 }
 
+struct Barriers {
+    uint64_t q_full[2], kv_full[KV_STAGES], kv_empty[KV_STAGES], s_full[2][2], p_full[2][2], o_ready[2][2];          // [row tile][tile j & 1]
+    uint64_t joined[2][4];                       // [row tile][warp]: the odd tiles' stream has left its reference point and sum
+};
 struct Smem {
     uint16_t q[2][NB][BQ * 64];                  // K-major, 128-byte swizzle, a block for each 64 of the head
     uint16_t k[KV_STAGES][NB][BK * 64];
     uint16_t v[KV_STAGES][NB][BK * 64];
     float ks[KV_STAGES][8], vl[KV_STAGES][8], vi[KV_STAGES][8];       // of each 8 keys: K's scale, V's log2 and reciprocal
-    uint64_t q_full[2], kv_full[KV_STAGES], kv_empty[KV_STAGES], s_full[2][2], p_full[2][2], o_ready[2][2];          // [row tile][tile j & 1]
-    uint64_t joined[2][4];                       // [row tile][warp]: the odd tiles' stream has left its reference point and sum
-    float odd_m[BR], odd_l[BR];
+    Barriers b;
+    float odd_m[BR], odd_l[BR], row_f[BR];       // row_f: what a row's raw products are multiplied by (base 2)
     uint32_t tmem_base;
 };
 
@@ -125,6 +129,13 @@ attn_prefill_q8_sm100_kernel(const Params p) {
         ng_pdl_wait();                                         // (a launch none of whose blocks waited would end before the one before it)
         return;
     }
+    // A row of the block is of token tb + tr; n rows behind the first one of token tb: (n + 1/2) / G in float32 is exact for n < 2^21
+    const int tb = r0 / G, hb = r0 - tb * G;
+    const float per_head = 1.f / (float)G;
+    auto row_at = [&](int row) {                               // of the block; the row's place in q and out, in rows of heads
+        const int n = hb + row, tr = (int)(((float)n + 0.5f) * per_head);
+        return (size_t)(q0 + tb + tr) * p.nH + kvh * G + n - tr * G;
+    };
     const int rows_here = min(BR, qlen * G - r0), rows_0 = min(BQ, rows_here), rows_1 = max(0, rows_here - BQ);
     const int first = ctx + r0 / G, last = ctx + (r0 + rows_here - 1) / G;          // positions
     const int key_lo = p.window > 0 ? max(0, first - p.window + 1) : 0, kv_end = last + 1;
@@ -140,22 +151,35 @@ attn_prefill_q8_sm100_kernel(const Params p) {
     if (n_tiles <= 0) {                                        // an empty run: records that the merge passes over
         ng_pdl_wait();
         if (threadIdx.x < rows_here) {
-            const int token = (r0 + threadIdx.x) / G, head = kvh * G + (r0 + threadIdx.x) - token * G;
-            float* rec = p.scratch + (((size_t)(q0 + token) * p.nH + head) * p.n_splits + split) * REC;
+            float* rec = p.scratch + (row_at(threadIdx.x) * p.n_splits + split) * REC;
             rec[0] = -INFINITY;
             rec[1] = 0.f;
         }
         return;
     }
-    if (threadIdx.x == 0) {
-        for (int s = 0; s < KV_STAGES; ++s) { mbar_init(&sm->kv_full[s], KV_WARPS); mbar_init(&sm->kv_empty[s], 1); }
-        for (int t = 0; t < 2; ++t) {
-            mbar_init(&sm->q_full[t], 4 * STREAMS);
-            for (int i = 0; i < 4; ++i) mbar_init(&sm->joined[t][i], 1);
-            for (int i = 0; i < 2; ++i) { mbar_init(&sm->s_full[t][i], 1); mbar_init(&sm->p_full[t][i], 4); mbar_init(&sm->o_ready[t][i], 1); }
-        }
+    if (threadIdx.x < sizeof(Barriers) / 8) {                  // a thread a barrier
+        const int i = threadIdx.x;
+        const bool kv = i >= offsetof(Barriers, kv_full) / 8 && i < offsetof(Barriers, kv_empty) / 8, pf = i >= offsetof(Barriers, p_full) / 8 && i < offsetof(Barriers, o_ready) / 8;
+        mbar_init(reinterpret_cast<uint64_t*>(&sm->b) + i, i < 2 ? 4 * STREAMS : kv ? KV_WARPS : pf ? 4 : 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    // Loaders: the page numbers of the first tiles (the batch description: no kernel of this step writes it)
+    constexpr int UNITS = (8 + KV_WARPS - 1) / KV_WARPS, DEPTH = 2;
+    const int loader = __shfl_sync(0xffffffffu, warp - SOFTMAX_WARPS, 0);
+    struct Pages { int unit[UNITS], mine; };                   // of a tile to ask for, as the table has them; mine: lane u's, unit u's (the scales)
+    auto page_of = [&](int key) {                              // (not looked at before the tile is asked for: the load would be waited for here)
+        const int i = key >> p.c.ps_log2;
+        return key + 7 >= key_lo && key < kv_end && i < p.c.table_stride ? p.c.table[(size_t)e * p.c.table_stride + i] : -1;
+    };
+    auto pages = [&](int tile) {
+        Pages to;
+#pragma unroll
+        for (int n = 0; n < UNITS; ++n) to.unit[n] = loader + KV_WARPS * n < 8 ? page_of(tile * BK + 8 * (loader + KV_WARPS * n)) : -1;
+        to.mine = loader == KV_WARPS - 1 && lane < 8 ? page_of(tile * BK + 8 * lane) : -1;
+        return to;
+    };
+    Pages page0{}, page1{};
+    if (loader >= 0 && loader < KV_WARPS) page0 = pages(tile0), page1 = pages(tile0 + 1);
     if (warp == SOFTMAX_WARPS + KV_WARPS) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" :: "r"(smem_u32(&sm->tmem_base)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -172,30 +196,19 @@ attn_prefill_q8_sm100_kernel(const Params p) {
         // ------------------------------------------------------------------ keys and values
         // A unit is eight keys (they lie in one page and one block) of K and of V: UNIT_LOADS requests of 16 bytes a lane each.  A warp has
         // every third unit; page numbers are asked for a tile before the codes, the codes DEPTH tiles before they are stored.
-        constexpr int UNIT_LOADS = HD / 64, UNITS = (8 + KV_WARPS - 1) / KV_WARPS, DEPTH = 2;
-        const int w = __shfl_sync(0xffffffffu, warp - SOFTMAX_WARPS, 0), mask = (1 << p.c.ps_log2) - 1;
-        const int* trow = p.c.table + (size_t)e * p.c.table_stride;
+        constexpr int UNIT_LOADS = HD / 64;
+        const int w = loader, mask = (1 << p.c.ps_log2) - 1;
         const long long page_bytes = (long long)(p.c.nKV << p.c.ps_log2) * HD, head_at = (long long)(kvh << p.c.ps_log2) * HD + lane * 16;
         const unsigned char *k_pages = p.c.k + head_at, *v_pages = p.c.v + head_at;
         uint32_t k[DEPTH][UNITS][UNIT_LOADS][4], v[DEPTH][UNITS][UNIT_LOADS][4];
         float ks[DEPTH], vs[DEPTH];
-        int page[UNITS], my_page;                              // of the next tile to ask for, as the table has them; my_page: lane u's, unit u's (the scales)
-        auto page_of = [&](int key) {                          // (not looked at before the next tile: the load would be waited for here)
-            const int i = key >> p.c.ps_log2;
-            return key + 7 >= key_lo && key < kv_end && i < p.c.table_stride ? trow[i] : -1;
-        };
-        auto pages = [&](int tile) {
-#pragma unroll
-            for (int n = 0; n < UNITS; ++n) page[n] = w + KV_WARPS * n < 8 ? page_of(tile * BK + 8 * (w + KV_WARPS * n)) : -1;
-            my_page = w == KV_WARPS - 1 && lane < 8 ? page_of(tile * BK + 8 * lane) : -1;
-        };
         // (a page that is not there: page 0 is read, and the unit's keys become zeros when they are stored)
         bool bad[DEPTH][UNITS];
-        auto load = [&](int d, int tile) {
+        auto load = [&](int d, int tile, const Pages& page) {
 #pragma unroll
             for (int n = 0; n < UNITS; ++n) {
-                bad[d][n] = (unsigned)page[n] >= (unsigned)p.c.num_pages;
-                const long long at = (long long)(bad[d][n] ? 0 : page[n]) * page_bytes + (tile * BK + 8 * (w + KV_WARPS * n) & mask) * HD;
+                bad[d][n] = (unsigned)page.unit[n] >= (unsigned)p.c.num_pages;
+                const long long at = (long long)(bad[d][n] ? 0 : page.unit[n]) * page_bytes + (tile * BK + 8 * (w + KV_WARPS * n) & mask) * HD;
 #pragma unroll
                 for (int i = 0; i < UNIT_LOADS; ++i) {
                     ld_codes<16>(k[d][n][i], k_pages + at + i * 512);
@@ -203,8 +216,8 @@ attn_prefill_q8_sm100_kernel(const Params p) {
                 }
             }
             ks[d] = vs[d] = 1.f;
-            if ((unsigned)my_page < (unsigned)p.c.num_pages) {
-                const long long sc = ((long long)my_page * p.c.nKV + kvh << (p.c.ps_log2 - p.c.bl_log2)) + ((tile * BK + 8 * lane & mask) >> p.c.bl_log2);
+            if ((unsigned)page.mine < (unsigned)p.c.num_pages) {
+                const long long sc = ((long long)page.mine * p.c.nKV + kvh << (p.c.ps_log2 - p.c.bl_log2)) + ((tile * BK + 8 * lane & mask) >> p.c.bl_log2);
                 ld_codes<4>(reinterpret_cast<uint32_t*>(&ks[d]), reinterpret_cast<const unsigned char*>(p.c.ks + sc));
                 ld_codes<4>(reinterpret_cast<uint32_t*>(&vs[d]), reinterpret_cast<const unsigned char*>(p.c.vs + sc));
             }
@@ -216,18 +229,16 @@ attn_prefill_q8_sm100_kernel(const Params p) {
             *reinterpret_cast<uint4*>(tile + sw128(row, c)) = make_uint4(h[0], h[1], h[2], h[3]);
             *reinterpret_cast<uint4*>(tile + sw128(row, c + 1)) = make_uint4(h[4], h[5], h[6], h[7]);
         };
-        pages(tile0);
-#pragma unroll
-        for (int d = 0; d < DEPTH; ++d) {
-            load(d, tile0 + d);
-            pages(tile0 + d + 1);
-        }
+        static_assert(DEPTH == 2, "two tiles are asked for here");
+        load(0, tile0, page0);
+        load(1, tile0 + 1, page1);
+        page0 = pages(tile0 + DEPTH);
         for (int j0 = 0; j0 < n_tiles && ok; j0 += DEPTH)
 #pragma unroll
             for (int d = 0; d < DEPTH; ++d) {
                 const int j = j0 + d, s = j % KV_STAGES;
                 if (j >= n_tiles || !ok) break;
-                ok = __all_sync(0xffffffffu, mbar_wait(&sm->kv_empty[s], ((j / KV_STAGES) & 1) ^ 1));
+                ok = __all_sync(0xffffffffu, mbar_wait(&sm->b.kv_empty[s], ((j / KV_STAGES) & 1) ^ 1));
                 if (!ok) break;
 #pragma unroll
                 for (int n = 0; n < UNITS; ++n)
@@ -255,22 +266,22 @@ attn_prefill_q8_sm100_kernel(const Params p) {
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&sm->kv_full[s]);
-                load(d, tile0 + j + DEPTH);                    // (behind the last tile: zeros, from no page)
-                pages(tile0 + j + DEPTH + 1);
+                if (lane == 0) mbar_arrive(&sm->b.kv_full[s]);
+                load(d, tile0 + j + DEPTH, page0);             // (behind the last tile: zeros, from no page)
+                page0 = pages(tile0 + j + DEPTH + 1);
             }
         if (!ok && lane == 0) atomicOr(p.status, NG_STATUS_ATTN_TIMEOUT);
     } else if (warp == SOFTMAX_WARPS + KV_WARPS) {
         // ------------------------------------------------------------------ MMA issuer: all lanes run the loop, one issues
         constexpr uint32_t idesc_s = idesc_f16(BK, 0), idesc_o = idesc_f16(64, 1);
         for (int t = 0; t < 2 && ok; ++t)
-            if ((t ? n_1 : n_0) > 0) ok = __all_sync(0xffffffffu, mbar_wait(&sm->q_full[t], 0));
+            if ((t ? n_1 : n_0) > 0) ok = __all_sync(0xffffffffu, mbar_wait(&sm->b.q_full[t], 0));
         // descriptors of the first stage; addresses are in units of 16 bytes, and so are the distances added to them
         const uint64_t q_desc = make_desc_sw128(sm->q[0][0]), k_desc = make_desc_sw128(sm->k[0][0]), v_desc = make_desc_sw128_mn(sm->v[0][0]);
         constexpr uint64_t Q_TILE = sizeof(sm->q[0]) / 16, Q_BLOCK = sizeof(sm->q[0][0]) / 16, KV_STAGE = sizeof(sm->k[0]) / 16, KV_BLOCK = sizeof(sm->k[0][0]) / 16;
         auto issue_s = [&](int t, int j) {                     // S = Q K_j^T into buffer j & 1 of row tile t
             const int s = j % KV_STAGES;
-            if (!__all_sync(0xffffffffu, mbar_wait(&sm->kv_full[s], (j / KV_STAGES) & 1))) { ok = false; return; }
+            if (!__all_sync(0xffffffffu, mbar_wait(&sm->b.kv_full[s], (j / KV_STAGES) & 1))) { ok = false; return; }
             tcgen05_fence_after();
             if (leader) {
 #pragma unroll
@@ -280,7 +291,7 @@ attn_prefill_q8_sm100_kernel(const Params p) {
                     for (int k = 0; k < 4; ++k)
                         tcgen05_mma_f16(tmem + 128 * t + 64 * (j & 1), dq + (uint64_t)(2 * k), dk + (uint64_t)(2 * k), idesc_s, b > 0 || k > 0);
                 }
-                tcgen05_commit(&sm->s_full[t][j & 1]);
+                tcgen05_commit(&sm->b.s_full[t][j & 1]);
             }
             __syncwarp();
         };
@@ -294,7 +305,7 @@ attn_prefill_q8_sm100_kernel(const Params p) {
                 const int n = t ? n_1 : n_0;
                 if (!ok) break;
                 if (j < n) {
-                    ok = __all_sync(0xffffffffu, mbar_wait(&sm->p_full[t][j & 1], (j >> 1) & 1));          // P_j in tensor memory, O rescaled
+                    ok = __all_sync(0xffffffffu, mbar_wait(&sm->b.p_full[t][j & 1], (j >> 1) & 1));          // P_j in tensor memory, O rescaled
                     if (!ok) break;
                     tcgen05_fence_after();
                     if (leader) {
@@ -306,10 +317,10 @@ attn_prefill_q8_sm100_kernel(const Params p) {
                                 tcgen05_mma_f16_ts(tm_o(t, j) + 64 * b, tmem + 128 * t + 64 * (j & 1) + 8 * k, dv + (uint64_t)(128 * k),
                                                    idesc_o, j >= STREAMS || k > 0);
                         }
-                        tcgen05_commit(&sm->o_ready[t][j & 1]);                // O holds tiles 0..j
+                        tcgen05_commit(&sm->b.o_ready[t][j & 1]);                // O holds tiles 0..j
                     }
                 }
-                if (t == 1 && leader) tcgen05_commit(&sm->kv_empty[s]);        // K_j and V_j may be overwritten
+                if (t == 1 && leader) tcgen05_commit(&sm->b.kv_empty[s]);        // K_j and V_j may be overwritten
                 __syncwarp();
                 if (j + 2 < n) issue_s(t, j + 2);
             }
@@ -325,35 +336,44 @@ attn_prefill_q8_sm100_kernel(const Params p) {
         const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
         float f = 0.f;
         if (n_mine > 0) {
-            // the row of q, divided by a power of two, as float16 (of two streams, each writes half)
-            const bf16* q = ng_after_wait(p.q) + ((size_t)(q0 + token) * p.nH + head) * HD;
-            float top = 0.f;
+            // The warp's rows of q (of two streams, each brings 16 of the 32), each divided by a power of two, as float16: LANES lanes a row, so
+            // that a request is whole lines, all in flight.  (A thread a row: 4 us at the start of every block, heads of 128 7 us.)
+            constexpr int LANES = HD / 8, ROWS = 32 / LANES, MINE = 32 / STREAMS;
+            const bf16* q = ng_after_wait(p.q);
+            const int c = lane % LANES;
+            const int at = 32 * (warp & 3) + MINE * odd + lane / LANES;                  // row of the row tile
 #pragma unroll 4
-            for (int c = 0; c < HD / 8; ++c) {
-                const uint4 w = *reinterpret_cast<const uint4*>(q + 8 * c);
+            for (int i = 0; i < MINE; i += ROWS)               // (rows past the last read that one)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" :: "r"(smem_u32(sm->q[t][c / 8] + sw128(at + i, c % 8))),
+                             "l"(q + row_at(BQ * t + min(at + i, rows_mine - 1)) * HD + 8 * c) : "memory");
+            asm volatile("cp.async.wait_all;" ::: "memory");   // (a lane reads what it asked for itself)
+#pragma unroll 2
+            for (int i = 0; i < MINE; i += ROWS) {
+                uint4* mine = reinterpret_cast<uint4*>(sm->q[t][c / 8] + sw128(at + i, c % 8));
+                const uint4 w = *mine;
                 const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+                float top = 0.f;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float a = fabsf(__uint_as_float(x[i] << 16)), b = fabsf(__uint_as_float(x[i] & 0xffff0000u));
+                for (int j = 0; j < 4; ++j) {
+                    const float a = fabsf(__uint_as_float(x[j] << 16)), b = fabsf(__uint_as_float(x[j] & 0xffff0000u));
                     if (a < INFINITY) top = fmaxf(top, a);
                     if (b < INFINITY) top = fmaxf(top, b);
                 }
-            }
-            const int ex = q_exponent(top);
-            const float div = pow2_any(-ex);
-            f = p.scale * LOG2E * pow2_any(ex);
-#pragma unroll 4
-            for (int c = odd * (HD / 16); c < (odd || STREAMS == 1 ? HD / 8 : HD / 16); ++c) {
-                const uint4 w = *reinterpret_cast<const uint4*>(q + 8 * c);
-                const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                for (int o = 1; o < LANES; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                const int ex = q_exponent(top);
+                const float div = pow2_any(-ex);
                 uint32_t h[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) h[i] = pack_f16(__uint_as_float(x[i] << 16) * div, __uint_as_float(x[i] & 0xffff0000u) * div);
-                *reinterpret_cast<uint4*>(sm->q[t][c / 8] + sw128(r, c % 8)) = make_uint4(h[0], h[1], h[2], h[3]);
+                for (int j = 0; j < 4; ++j) h[j] = pack_f16(__uint_as_float(x[j] << 16) * div, __uint_as_float(x[j] & 0xffff0000u) * div);
+                *mine = make_uint4(h[0], h[1], h[2], h[3]);
+                if (c == 0) sm->row_f[BQ * t + at + i] = p.scale * LOG2E * pow2_any(ex);
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
-            if (lane == 0) mbar_arrive(&sm->q_full[t]);
+            if (lane == 0) mbar_arrive(&sm->b.q_full[t]);
+            if constexpr (STREAMS == 2) asm volatile("bar.sync %0, 64;" :: "r"(1 + 4 * t + (warp & 3)) : "memory");        // the two warps of these rows
+            f = sm->row_f[BQ * t + r];
         }
         // m is the reference point of the exponentials; it moves to the first tile's maximum and then follows lazily: only when a tile exceeds
         // it by more than 2^8 is O in TMEM rescaled (which has to wait for the product before).
@@ -362,7 +382,7 @@ attn_prefill_q8_sm100_kernel(const Params p) {
         const float slope = p.slopes ? p.slopes[head] * LOG2E : 0.f;
         for (int j = odd; j < n_mine && ok; j += STREAMS) {
             const int s = j % KV_STAGES, key0 = (tile0 + j) * BK;
-            ok = mbar_wait(&sm->kv_full[s], (j / KV_STAGES) & 1) && mbar_wait(&sm->s_full[t][j & 1], (j >> 1) & 1);
+            ok = mbar_wait(&sm->b.kv_full[s], (j / KV_STAGES) & 1) && mbar_wait(&sm->b.s_full[t][j & 1], (j >> 1) & 1);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             tcgen05_fence_after();
@@ -372,25 +392,28 @@ attn_prefill_q8_sm100_kernel(const Params p) {
             // largest sc (f and the scales are positive), or with a bias the largest sc fk + slope i.  The first pass finds the maximum, the
             // second the weights: the last 32 scores are still there, the first are read again.
             auto weigh = [&](auto kind) {
-                constexpr int MODE = decltype(kind)::value;                // 0: plain, 1: a bias, 2: hidden keys (and a bias)
+                constexpr int MODE = decltype(kind)::value;                // 0: plain, 1: a bias, 2: hidden keys (and a bias, if only of 0)
                 const float far = slope * (float)(key0 - pos);
                 const int rel = pos - key0, out_of = p.window > 0 ? rel - p.window : -1;
+                uint32_t vis[2];                                           // a bit for each key that the row sees: out_of < key - key0 <= rel
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int n = min(max(rel + 1 - 32 * h, 0), 32), n0 = min(max(out_of + 1 - 32 * h, 0), 32);
+                    vis[h] = (uint32_t)((1ull << n) - (1ull << min(n0, n)));
+                }
                 float sc[32];
-                auto formed = [&](int b, float ks, float vl) {             // the eight scores at 8 b (of the half h) become z (2), or z less lg and far (1)
-                    if constexpr (MODE == 1) {
+                auto formed = [&](int b, float ks) {                       // the eight scores at 8 b become z less lg and far (1, 2)
+                    if constexpr (MODE >= 1) {
                         const float fk = f * ks;
                         const u64 fk2 = pack2(fk, fk);
 #pragma unroll
                         for (int i = 0; i < 8; i += 2)
                             unpack2(ffma2(pack2(sc[8 * (b & 3) + i], sc[8 * (b & 3) + i + 1]), fk2, pack2(slope * i, slope * (i + 1))),
                                     sc[8 * (b & 3) + i], sc[8 * (b & 3) + i + 1]);
-                    } else if constexpr (MODE == 2) {
-                        const float fk = f * ks;
+                        if constexpr (MODE == 2)
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            float& x = sc[8 * (b & 3) + i];
-                            x = 8 * b + i <= rel && 8 * b + i > out_of ? fmaf(slope, (float)(8 * b + i), fmaf(x, fk, vl + far)) : -INFINITY;
-                        }
+                            for (int i = 0; i < 8; ++i)
+                                if (!(vis[b >> 2] >> (8 * (b & 3) + i) & 1)) sc[8 * (b & 3) + i] = -INFINITY;
                     }
                 };
                 float mx = -INFINITY;
@@ -402,10 +425,10 @@ attn_prefill_q8_sm100_kernel(const Params p) {
                     float mz[4];
 #pragma unroll
                     for (int u = 0; u < 4; ++u) {
-                        formed(4 * h + u, ks[u], vl[u]);
+                        formed(4 * h + u, ks[u]);
                         const float* x = sc + 8 * u;
                         const float y = fmaxf(fmax3(fmax3(x[0], x[1], x[2]), fmax3(x[3], x[4], x[5]), x[6]), x[7]);
-                        mz[u] = MODE == 0 ? fmaf(y, f * ks[u], vl[u]) : MODE == 1 ? y + (vl[u] + fmaf(8.f * slope, (float)(4 * h + u), far)) : y;
+                        mz[u] = MODE == 0 ? fmaf(y, f * ks[u], vl[u]) : y + (vl[u] + fmaf(8.f * slope, (float)(4 * h + u), far));
                     }
                     mx = fmax3(mx, fmaxf(mz[0], mz[1]), fmaxf(mz[2], mz[3]));
                 }
@@ -428,8 +451,8 @@ attn_prefill_q8_sm100_kernel(const Params p) {
                     const float ks[4] = {k4.x, k4.y, k4.z, k4.w}, vl[4] = {v4.x, v4.y, v4.z, v4.w}, vi[4] = {i4.x, i4.y, i4.z, i4.w};
 #pragma unroll
                     for (int u = 0; u < 4; ++u) {
-                        if (h == 0) formed(u, ks[u], vl[u]);
-                        const float fk = f * ks[u], lg = (MODE == 0 ? vl[u] : MODE == 1 ? vl[u] + fmaf(8.f * slope, (float)(4 * h + u), far) : 0.f) - m;
+                        if (h == 0) formed(u, ks[u]);
+                        const float fk = f * ks[u], lg = (MODE == 0 ? vl[u] : vl[u] + fmaf(8.f * slope, (float)(4 * h + u), far)) - m;
                         const u64 fk2 = pack2(fk, fk), lg2 = pack2(lg, lg);
                         u64 sum2 = pack2(0.f, 0.f);
 #pragma unroll
@@ -455,7 +478,7 @@ attn_prefill_q8_sm100_kernel(const Params p) {
             else if (p.slopes) weigh(std::integral_constant<int, 1>{});
             else weigh(std::integral_constant<int, 0>{});
             if (j >= STREAMS && __any_sync(0xffffffffu, corr != 1.f)) {    // rescale this warp's rows of O
-                ok = mbar_wait(&sm->o_ready[t][(j - STREAMS) & 1], ((j - STREAMS) >> 1) & 1);
+                ok = mbar_wait(&sm->b.o_ready[t][(j - STREAMS) & 1], ((j - STREAMS) >> 1) & 1);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 tcgen05_fence_after();
@@ -472,12 +495,12 @@ attn_prefill_q8_sm100_kernel(const Params p) {
             tmem_st_wait();
             tcgen05_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&sm->p_full[t][j & 1]);
+            if (lane == 0) mbar_arrive(&sm->b.p_full[t][j & 1]);
         }
         // what the odd tiles' stream found goes to the even tiles', which writes the rows
         const int last_j = n_mine - 1 - (STREAMS == 2 && (n_mine - 1 & 1) != odd ? 1 : 0);             // the stream's last tile (< 0: none)
         if (ok && n_mine > 0 && last_j >= 0) {
-            ok = mbar_wait(&sm->o_ready[t][last_j & 1], (last_j >> 1) & 1);
+            ok = mbar_wait(&sm->b.o_ready[t][last_j & 1], (last_j >> 1) & 1);
             ok = __all_sync(0xffffffffu, ok);
         }
         float m_odd = -INFINITY, l_odd = 0.f;
@@ -487,9 +510,9 @@ attn_prefill_q8_sm100_kernel(const Params p) {
                 sm->odd_m[BQ * t + r] = seen ? m : -INFINITY;
                 sm->odd_l[BQ * t + r] = l;
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&sm->joined[t][warp & 3]);
+                if (lane == 0) mbar_arrive(&sm->b.joined[t][warp & 3]);
             } else {
-                ok = __all_sync(0xffffffffu, mbar_wait(&sm->joined[t][warp & 3], 0));
+                ok = __all_sync(0xffffffffu, mbar_wait(&sm->b.joined[t][warp & 3], 0));
                 m_odd = sm->odd_m[BQ * t + r];
                 l_odd = sm->odd_l[BQ * t + r];
             }
@@ -497,8 +520,7 @@ attn_prefill_q8_sm100_kernel(const Params p) {
         if (!ok) {
             if (lane == 0) atomicOr(p.status, NG_STATUS_ATTN_TIMEOUT);
         } else if (!odd) {
-            const size_t at = (size_t)(q0 + token) * p.nH + head;
-            float* rec = p.scratch + (at * p.n_splits + split) * REC;
+            float* rec = p.scratch + (row_at(BQ * t + r) * p.n_splits + split) * REC;
             const bool two = STREAMS == 2 && n_mine > 1, live = r < rows_mine;
             const float m_even = seen ? m : -INFINITY, top = fmaxf(m_even, m_odd);
             // (a stream that met only NaN has no reference point and keeps its sums)
@@ -511,27 +533,39 @@ attn_prefill_q8_sm100_kernel(const Params p) {
             if (p.n_splits == 1) a *= inv, b *= inv;
             if (n_mine > 0) {
                 tcgen05_fence_after();
-#pragma unroll
+#pragma unroll 1
                 for (int c = 0; c < HD; c += 16) {
                     float x[16], y[16];
                     tmem_ld16(tm_o(t, 0) + lane_base + c, x);
                     if (two) tmem_ld16(tm_o(t, 1) + lane_base + c, y);
 #pragma unroll
                     for (int i = 0; i < 16; ++i) x[i] = two ? fmaf(x[i], a, y[i] * b) : x[i] * a;
-                    if (live && p.n_splits > 1) {
+                    if (p.n_splits > 1) {
+                        if (live)
 #pragma unroll
-                        for (int i = 0; i < 16; i += 4) *reinterpret_cast<float4*>(rec + 4 + c + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
-                    } else if (live) {
-                        uint32_t w[8];
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
-                            w[i] = *reinterpret_cast<const uint32_t*>(&h);
-                        }
-                        *reinterpret_cast<uint4*>(p.out + at * HD + c) = make_uint4(w[0], w[1], w[2], w[3]);
-                        *reinterpret_cast<uint4*>(p.out + at * HD + c + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+                            for (int i = 0; i < 16; i += 4) *reinterpret_cast<float4*>(rec + 4 + c + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+                        continue;
                     }
+#pragma unroll
+                    for (int i = 0; i < 16; i += 8) {          // over the rows of q, which no product reads any more
+                        uint32_t w[4];
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) {
+                            const __nv_bfloat162 h = __floats2bfloat162_rn(x[i + 2 * u], x[i + 2 * u + 1]);
+                            w[u] = *reinterpret_cast<const uint32_t*>(&h);
+                        }
+                        *reinterpret_cast<uint4*>(sm->q[t][(c + i) / 64] + sw128(r, (c + i) / 8 % 8)) = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                }
+                if (p.n_splits == 1) {                         // whole lines again
                     __syncwarp();
+                    constexpr int LANES = HD / 8, ROWS = 32 / LANES;
+                    const int c = lane % LANES, at = 32 * (warp & 3) + lane / LANES;
+#pragma unroll 4
+                    for (int i = 0; i < 32; i += ROWS)
+                        if (at + i < rows_mine)
+                            *reinterpret_cast<uint4*>(p.out + row_at(BQ * t + at + i) * HD + 8 * c) =
+                                *reinterpret_cast<const uint4*>(sm->q[t][c / 8] + sw128(at + i, c % 8));
                 }
             }
         }

@@ -169,7 +169,7 @@ struct NgAttnQ8 {
 static bool attn_q8_args(const NgAttnQ8& c, Cache& to) {
     to = Cache{(const unsigned char*)c.k_pages, (const unsigned char*)c.v_pages, c.k_scales, c.v_scales, c.table, c.table_stride, c.num_pages,
                c.n_kv, log2_exact(c.page_size), log2_exact(c.block), (int)((long long)c.table_stride * c.page_size - 1)};
-    return c.head_dim == HD && c.n_heads > 0 && c.n_kv > 0 && c.n_heads % c.n_kv == 0 && to.ps_log2 >= 3 && to.bl_log2 >= 3 &&
+    return c.head_dim == HD && c.n_heads > 0 && c.n_heads <= 1 << 20 && c.n_kv > 0 && c.n_heads % c.n_kv == 0 && to.ps_log2 >= 3 && to.bl_log2 >= 3 &&
            to.bl_log2 <= to.ps_log2 && c.table_stride > 0 && (long long)c.table_stride * c.page_size <= 1 << 30 && c.num_pages > 0 &&
            (long long)c.n_rows * c.n_heads <= 1 << 30 && (long long)c.n_kv * c.page_size * HD <= 0x7fffffff &&
            !(((uintptr_t)c.k_pages | (uintptr_t)c.v_pages) & 15) && (c.kind == NG_Q8_E4M3 || c.kind == NG_Q8_INT8) && c.window >= 0 &&
