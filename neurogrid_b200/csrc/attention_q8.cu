@@ -8,7 +8,10 @@
 // score.  t_j goes into the exponent: with z_j = x_j log2(e) + log2(t_j) and the reference point m near max z_j, the weights
 // w_j = 2^(z_j - m) are what meets the codes d_j, in float16 (half a step 2^-12 of the weight, smallest step 2^-24 of the
 // largest), and the denominator is sum_j w_j / t_j in 32 bits: t_j is a power of two, both forms are exact.  So a block
-// whose values are small has small weights, not small values, and the sum over the codes never leaves float16's range.
+// whose values are small has small weights, not small values, and the sum over the codes never leaves float16's range.  (A key is lost to the
+// denominator where its weight times t_j is less than 2^-126 of the largest such product: blocks of zeros, whose scale is 2^-100, keep
+// theirs down to 2^-26 of the largest weight times the largest scale.)
+// Entries whose context is below zero or behind the table's last place are passed over, their rows left as they were.
 #include "ng_q8_attention.cuh"
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -24,13 +27,20 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], u
 // permuted so that a lane reads contiguous bytes.  K and V come from memory into the registers they are used from, the next group's requested
 // before this group is computed and the page numbers a group earlier still; nothing passes through shared memory but the four warps' results.
 //
-// Bound by the codes' bytes and by the issue of instructions.  A lane's words of V hold one key's codes each; a byte permutation puts a pair of
-// keys beside each other, as the MMA wants them, and a movmatrix turns a tile of weights from keys x heads to heads x keys.
+// A lane's words of V hold one key's codes each; a byte permutation puts a pair of keys beside each other, as the MMA wants them, and a movmatrix
+// turns a tile of weights from keys x heads to heads x keys.
 //
-// Who does what: with one run, a block has a segment.  With more, the launch has as many blocks as the GPU holds at once and every block finds, from
-// the entries' lengths on the device, its equal share of the turns of all segments laid end to end: pieces of one segment or several.  A piece that
-// is a whole segment writes its output rows; others write records for the merge, the piece's number within the segment as the run's.  So
-// batches of unequal lengths, and segments a little more than the blocks, fill the GPU evenly.
+// Who does what: with one run, a block has a segment.  With more, the launch has as many blocks as the GPU holds at once, in teams of a block for
+// each segment of an entry, and every team finds, from the entries' lengths on the device, its equal share of the turns of all entries
+// laid end to end: pieces of one entry or several.  A piece that is a whole segment writes its output rows; others write records for the
+// merge, the piece's number within the segment as the run's.  So batches of unequal lengths, and segments a little more than the blocks, fill
+// the GPU evenly.
+//
+// Bound by the codes' bytes where there are many (2 requests behind 131,072 tokens, 32 / 8 heads of 128: 86 us, 6.2 TB/s = 0.95 of a plain copy's rate) and else by
+// the chain of a group: page numbers -> codes -> products -> maximum -> weights -> products, three blocks an SM wide (64 requests of
+// up to 4,096 tokens, 32 / 8 heads of 64, integers: 39 us, 4.3 TB/s; the loads alone take 33, the arithmetic alone 34).  8 requests behind
+// 2,100 tokens 10.5 us, 1 behind 300 4.2 us.  Codes through a ring in shared memory (cp.async, 2 to 4 stages) took 43 to 48 us for the 64 requests
+// (more work for the load and store unit), groups of 16 keys or of 64 were slower with heads of 64, conversions cost nothing that could be seen.
 #define DC_WARPS 4
 #define DC_THREADS (DC_WARPS * 32)
 constexpr int W = HD % 64 == 0 ? 16 : HD % 32 == 0 ? 8 : 4;        // bytes of a key that a lane takes at once (of a value row: half of it)
@@ -483,6 +493,8 @@ attn_decode_q8_kernel(const DcArgs a) {
 // portion fills the block's PF_ROWS rows with the heads that share its keys, and a key tile is read and turned into float16 once for
 // all of them.  64-key tiles: the codes of the next tile are requested into registers while this one is computed, then written to shared
 // memory as float16 (two stages, one barrier a tile); scores, weights and sums as for single tokens, 16 rows a warp.
+// For the heads that attention_q8_sm100.cu does not take, and what it refuses.  Bound by `mma.sync` and its ldmatrix loads (2,048 tokens, 32 / 8
+// heads of 64: 91 us, there 41; 512 behind 32,768 1,313 and 178).
 #define PF_WARPS 8
 #define PF_THREADS (PF_WARPS * 32)
 #define PF_ROWS (PF_WARPS * 16)

@@ -179,7 +179,11 @@ static bool attn_q8_args(const NgAttnQ8& c, Cache& to) {
 // least .. most: the rows that an entry brings to have records
 static int q8_merge(const NgAttnQ8& c, const Cache& cache, int least, int most, int rows, cudaStream_t stream) {
     const int z = rows < 1 ? 1 : rows > 65535 ? 65535 : rows;
-    if (c.n_splits > 8 && (long long)c.n_entries * c.n_heads * z < 1024)        // many runs of few rows
+    // A block a (row, head), or a warp: until the rows fill the GPU by themselves the wide form is the faster.  Heads of 64, with the attention in
+    // front of it, wide / narrow, us: 1 row of 32 heads, 17 runs 8.3 / 11.9, 48 runs 15.5 / 24.6; 8 rows, 16 runs 11.2 / 11.9; 64 rows, 2 to
+    // 16 runs 32.6 / 33.0 and 52.1 / 52.6; 256 rows, 8 runs 66.1 / 60.4; portions of 16 rows, 18 runs 34.7 / 38.4, 64 rows 41.2 / 45.6,
+    // 128 rows, 9 runs 42.4 / 42.3, 512 rows, 2 runs 266 / 254
+    if ((long long)c.n_entries * c.n_heads * z <= 4096)
         NG_LAUNCH((attn_q8_merge_kernel<true>), dim3(c.n_heads, c.n_entries, z), MG_WARPS * 32, 0, stream, c.scratch, c.cu_q, c.ctx_before,
                   cache.last_key, (bf16*)c.out, c.n_heads, c.n_splits, c.n_rows, least, most);
     else

@@ -653,12 +653,21 @@ def attn_decode_q8_splits(n_single: int, n_heads: int, n_kv_heads: int, head_dim
 
 
 def attn_prefill_q8_splits(q_lens, n_heads: int, n_kv_heads: int, head_dim: int, max_ctx: int, window: Optional[int], device) -> int:
-    """Runs ``attn_prefill_q8`` should cut the keys into: where its blocks (128 rows of a KV head's query heads) leave SMs idle and see
-    keys enough to share."""
+    """Runs ``attn_prefill_q8`` should cut the keys into, where its blocks (256 or 128 rows of a KV head's query heads) leave SMs idle."""
     group, rows = n_heads // n_kv_heads, 256 if head_dim in (64, 128) else 128
     blocks = sum(-(-n * group // rows) for n in q_lens) * n_kv_heads
     span = min(window + max(q_lens), max_ctx) if window else max_ctx
-    return max(1, min(_sm_count(device) // max(1, blocks), span // 512, 65535 // max(1, len(q_lens))))
+    slots, tiles, records = _sm_count(device) * (2 if head_dim < 64 else 1), -(-span // 64), sum(q_lens) * n_heads
+
+    # In tiles of 64 keys (0.93 us; heads of 128 1.2): a round of blocks takes its tiles and nine more to start and end, the merge three and a
+    # tile for 8,000 records.  32 / 8 heads of 64, us by runs, the chosen in brackets: 2,048 tokens [1: 41] 2: 81; 2,048 behind 16,384 [1: 525]
+    # 2: 560, 4: 535; 1,000 behind 8,000 [1: 139] 2: 151; 700 behind 16,000 1: 257, 3: 186, [5: 180] 8: 213; 64 behind 32,000 8: 75,
+    # [18: 41] 32: 55; 16 behind 4,000 7: 15, 12: 14, [15: 14]; heads of 128, 300 behind 16,000 1: 306, 2: 167, [3: 119] 4: 177; heads of
+    # 80, 100 behind 16,000 1: 488, 3: 176, [4: 137] 6: 184; 8 heads of 256, 40 behind 20,000 1: 1,724, 8: 254, [18: 125] 32: 145
+    def cost(s):
+        return -(-blocks * s // slots) * (tiles / s + 9) + (3 + records * s / 8000 if s > 1 else 0)
+
+    return min(range(1, max(1, min(tiles // 4, slots // n_kv_heads, 65535 // max(1, len(q_lens)))) + 1), key=cost)
 
 
 def _q8_attention(what, q, k_pages, v_pages, k_scales, v_scales, table, cu_q, ctx_before, out, scratch, n_entries, max_q, n_heads, window,
