@@ -20,7 +20,7 @@
 //
 // Bound by the softmax warps' instructions and by the handshakes of a tile (tensor pipe 28 %, exponential unit 57 %, issue slots 61 %
 // busy): 0.93 us for 64 keys of 256 rows, and about 7 us for a block's start and end.  512 tokens behind 32,768 (24 / 8 heads of 64)
-// 178 us = 582 TFLOP/s; 2,048 tokens, 32 / 8 heads of 64: 41 us; 6 requests of up to 611 tokens, 16 / 4 heads of 128, 67 us.  One row tile a block, two blocks an SM
+// 178 us = 582 TFLOP/s; 2,048 tokens, 32 / 8 heads of 64: 41 us; 6 requests of up to 611 tokens, 16 / 4 heads of 128, 65 us.  One row tile a block, two blocks an SM
 // 221 us instead of 178; one stream a row tile 214; registers moved from loaders to softmax warps, exponentials of two streams in turn, two
 // issuers, scores of 128 keys at once, 6 or 8 stages: no gain or slower.
 #include <cstddef>
@@ -343,37 +343,46 @@ attn_prefill_q8_sm100_kernel(const Params p) {
         const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
         float f = 0.f;
         if (n_mine > 0) {
-            // The warp's rows of q (of two streams, each brings 16 of the 32), each divided by a power of two, as float16: LANES lanes a row, so
+            // The warp's rows of q (of two streams, each brings 16 of the 32), each divided by a power of two, as float16: eight lanes a row, so
             // that a request is whole lines, all in flight.  (A thread a row: 4 us at the start of every block, heads of 128 7 us.)
-            constexpr int LANES = HD / 8, ROWS = 32 / LANES, MINE = 32 / STREAMS;
+            constexpr int ROWS = 4, MINE = 32 / STREAMS;
             const bf16* q = ng_after_wait(p.q);
-            const int c = lane % LANES;
-            const int at = 32 * (warp & 3) + MINE * odd + lane / LANES;                  // row of the row tile
+            const int c = lane & 7, at = 32 * (warp & 3) + MINE * odd + (lane >> 3);     // 16-byte chunk of 64 dimensions; row of the row tile
 #pragma unroll 4
-            for (int i = 0; i < MINE; i += ROWS)               // (rows past the last read that one)
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" :: "r"(smem_u32(sm->q[t][c / 8] + sw128(at + i, c % 8))),
-                             "l"(q + row_at(BQ * t + min(at + i, rows_mine - 1)) * HD + 8 * c) : "memory");
+            for (int i = 0; i < MINE; i += ROWS) {             // (rows past the last read that one)
+                const bf16* from = q + row_at(BQ * t + min(at + i, rows_mine - 1)) * HD + 8 * c;
+#pragma unroll
+                for (int n = 0; n < NB; ++n)
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" :: "r"(smem_u32(sm->q[t][n] + sw128(at + i, c))), "l"(from + 64 * n) : "memory");
+            }
             asm volatile("cp.async.wait_all;" ::: "memory");   // (a lane reads what it asked for itself)
 #pragma unroll 2
             for (int i = 0; i < MINE; i += ROWS) {
-                uint4* mine = reinterpret_cast<uint4*>(sm->q[t][c / 8] + sw128(at + i, c % 8));
-                const uint4 w = *mine;
-                const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+                uint4 w[NB];
                 float top = 0.f;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float a = fabsf(__uint_as_float(x[j] << 16)), b = fabsf(__uint_as_float(x[j] & 0xffff0000u));
-                    if (a < INFINITY) top = fmaxf(top, a);
-                    if (b < INFINITY) top = fmaxf(top, b);
+                for (int n = 0; n < NB; ++n) {
+                    w[n] = *reinterpret_cast<const uint4*>(sm->q[t][n] + sw128(at + i, c));
+                    const uint32_t x[4] = {w[n].x, w[n].y, w[n].z, w[n].w};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float a = fabsf(__uint_as_float(x[j] << 16)), b = fabsf(__uint_as_float(x[j] & 0xffff0000u));
+                        if (a < INFINITY) top = fmaxf(top, a);
+                        if (b < INFINITY) top = fmaxf(top, b);
+                    }
                 }
 #pragma unroll
-                for (int o = 1; o < LANES; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                for (int o = 1; o < 8; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
                 const int ex = q_exponent(top);
                 const float div = pow2_any(-ex);
-                uint32_t h[4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) h[j] = pack_f16(__uint_as_float(x[j] << 16) * div, __uint_as_float(x[j] & 0xffff0000u) * div);
-                *mine = make_uint4(h[0], h[1], h[2], h[3]);
+                for (int n = 0; n < NB; ++n) {
+                    const uint32_t x[4] = {w[n].x, w[n].y, w[n].z, w[n].w};
+                    uint32_t h[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) h[j] = pack_f16(__uint_as_float(x[j] << 16) * div, __uint_as_float(x[j] & 0xffff0000u) * div);
+                    *reinterpret_cast<uint4*>(sm->q[t][n] + sw128(at + i, c)) = make_uint4(h[0], h[1], h[2], h[3]);
+                }
                 if (c == 0) sm->row_f[BQ * t + at + i] = p.scale * LOG2E * pow2_any(ex);
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -540,21 +549,24 @@ attn_prefill_q8_sm100_kernel(const Params p) {
             if (p.n_splits == 1) a *= inv, b *= inv;
             if (n_mine > 0) {
                 tcgen05_fence_after();
+                constexpr int CH = STREAMS == 1 ? 32 : 16;     // dimensions at a time
 #pragma unroll 1
-                for (int c = 0; c < HD; c += 16) {
-                    float x[16], y[16];
-                    tmem_ld16(tm_o(t, 0) + lane_base + c, x);
-                    if (two) tmem_ld16(tm_o(t, 1) + lane_base + c, y);
+                for (int c = 0; c < HD; c += CH) {
+                    float x[CH], y[CH];
+                    if constexpr (STREAMS == 1) tmem_ld32(tm_o(t, 0) + lane_base + c, x);
+                    else tmem_ld16(tm_o(t, 0) + lane_base + c, x);
+                    if constexpr (STREAMS == 2)
+                        if (two) tmem_ld16(tm_o(t, 1) + lane_base + c, y);
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) x[i] = two ? fmaf(x[i], a, y[i] * b) : x[i] * a;
+                    for (int i = 0; i < CH; ++i) x[i] = two ? fmaf(x[i], a, y[i] * b) : x[i] * a;
                     if (p.n_splits > 1) {
                         if (live)
 #pragma unroll
-                            for (int i = 0; i < 16; i += 4) *reinterpret_cast<float4*>(rec + 4 + c + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+                            for (int i = 0; i < CH; i += 4) *reinterpret_cast<float4*>(rec + 4 + c + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
                         continue;
                     }
 #pragma unroll
-                    for (int i = 0; i < 16; i += 8) {          // over the rows of q, which no product reads any more
+                    for (int i = 0; i < CH; i += 8) {          // over the rows of q, which no product reads any more
                         uint32_t w[4];
 #pragma unroll
                         for (int u = 0; u < 4; ++u) {

@@ -488,9 +488,12 @@ def _q8_cache(what: str, k_pages, v_pages, k_scales, v_scales, table):
     return kind, num_pages, n_kv, page_size, hd, block, *of_table
 
 
+_INT32 = torch.int32
+
+
 def _i32s(what: str, *tensors) -> None:
     for t in tensors:
-        if t.dtype is not torch.int32:
+        if t.dtype is not _INT32:
             _i32(t, f"{what}: a table or a description of the batch")
 
 
@@ -499,6 +502,10 @@ def _current(what: str, t: torch.Tensor) -> int:
     if not t.is_cuda:
         _ptr(t, what)
     return _current_device() if _current_device is not None else torch.cuda.current_device()
+
+
+def _stream_of(here: int) -> int:
+    return _raw_stream(here) if _raw_stream is not None else _stream()
 
 
 def _on(what: str, here: int, *tensors):
@@ -545,7 +552,7 @@ def cache_write_q8(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pa
             raise KernelError(f"{what}: a tensor is on another device than the current one, cuda:{here}")
     _check(_q8_fn("cache_q8", "ng_cache_write_q8")(
         _Q8_WRITE.pack(k.data_ptr(), v.data_ptr(), *at, k_pitch, v_pitch, stride, n, n_entries, n_kv, hd, page_size, block, num_pages, kind, act),
-        _stream()), what)
+        _stream_of(here)), what)
 
 
 def rope_cache_q8(qkv: torch.Tensor, q_out: torch.Tensor, q_weight: Optional[torch.Tensor], k_weight: Optional[torch.Tensor],
@@ -569,7 +576,7 @@ def rope_cache_q8(qkv: torch.Tensor, q_out: torch.Tensor, q_weight: Optional[tor
     at = _on(what, here, qkv, q_out, q_weight, k_weight, inv_freq, k_pages, v_pages, k_scales, v_scales, table, positions, row_entry, status)
     _check(_q8_fn("cache_q8", "ng_rope_cache_q8")(
         _Q8_ROPE.pack(*at, stride, n_part if qkv.dtype is torch.float32 else 0, int(half_pairing), table_pages, table_rows, n, n_heads, n_kv,
-                      hd, page_size, block, num_pages, kind, pos_scale, eps), _stream()), what)
+                      hd, page_size, block, num_pages, kind, pos_scale, eps), _stream_of(here)), what)
 
 
 def copy_pages(pools, src, dst) -> None:
@@ -588,7 +595,8 @@ def copy_pages(pools, src, dst) -> None:
     shapes = [t.shape for t in pools]
     if any(len(x) < 2 or x[1] != shapes[0][1] for x in shapes):
         raise KernelError(f"{what}: pools are [layers, pages, ...] with the same pages")
-    at, of_page = _on(what, _current(what, pools[0]), *pools), []
+    here = _current(what, pools[0])
+    at, of_page = _on(what, here, *pools), []
     for t, x, base in zip(pools, shapes, at):
         size = t.numel()
         if size:
@@ -596,7 +604,7 @@ def copy_pages(pools, src, dst) -> None:
     f = _fn("cache_q8", "ng_copy_pages", [ctypes.c_char_p, _c_int, ctypes.c_char_p, ctypes.c_char_p, _c_int, _c_void_p])
     for i in range(0, len(of_page), 8):
         part = of_page[i:i + 8]
-        _check(f(b"".join(part), len(part), a, b, n, _stream()), what)
+        _check(f(b"".join(part), len(part), a, b, n, _stream_of(here)), what)
 
 
 def _page_numbers(what: str, x) -> bytes:
@@ -672,7 +680,7 @@ def attn_prefill_q8_splits(q_lens, n_heads: int, n_kv_heads: int, head_dim: int,
 
 def _q8_attention(what, q, k_pages, v_pages, k_scales, v_scales, table, cu_q, ctx_before, out, scratch, n_entries, max_q, n_heads, window,
                   scale, skip_single, n_splits, slopes, n_records):
-    """Checks, and the launcher's arguments: (head size, addresses but for the status word's, which comes last, the rest)."""
+    """Checks, and the launcher's arguments: (head size, stream, addresses but for the status word's, which comes last, the rest)."""
     kind, num_pages, n_kv, page_size, hd, block, table_rows, stride = _q8_cache(what, k_pages, v_pages, k_scales, v_scales, table)
     shape = q.shape
     if q.dtype is not torch.bfloat16 or out.dtype is not torch.bfloat16:
@@ -692,9 +700,10 @@ def _q8_attention(what, q, k_pages, v_pages, k_scales, v_scales, table, cu_q, ct
     _i32s(what, table, cu_q, ctx_before)
     if cu_q.numel() < n_entries + 1 or ctx_before.numel() < n_entries or table_rows < n_entries:
         raise KernelError(f"{what}: the batch description does not fit {n_entries} entries")
-    at = _on(what, _current(what, q), q, k_pages, v_pages, k_scales, v_scales, table, cu_q, ctx_before, out, scratch)
+    here = _current(what, q)
+    at = _on(what, here, q, k_pages, v_pages, k_scales, v_scales, table, cu_q, ctx_before, out, scratch)
     at.append(_slopes(slopes, n_heads) or 0)
-    return hd, at, (stride, shape[0], n_entries, max_q, n_heads, n_kv, hd, page_size, block, num_pages, kind, window or 0, skip_single,
+    return hd, _stream_of(here), at, (stride, shape[0], n_entries, max_q, n_heads, n_kv, hd, page_size, block, num_pages, kind, window or 0, skip_single,
                     n_splits, scale)
 
 
@@ -706,9 +715,9 @@ def attn_decode_q8(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     number of query heads a KV head.  The rows of other entries stay as they were.  ``n_splits`` (``attn_decode_q8_splits``) runs of
     the keys, planned for contexts of up to ``max_ctx`` (longer ones are right too); ``scratch`` holds ``attn_q8_scratch_floats`` (of
     ``n_entries``) float32 values when there is more than one."""
-    hd, at, rest = _q8_attention("attn_decode_q8", q, k_pages, v_pages, k_scales, v_scales, table, cu_q, ctx_before, out, scratch, n_entries,
+    hd, stream, at, rest = _q8_attention("attn_decode_q8", q, k_pages, v_pages, k_scales, v_scales, table, cu_q, ctx_before, out, scratch, n_entries,
                                  1, n_heads, window, scale, 0, n_splits, slopes, n_entries)
-    _check(_q8_fn("attention_q8", "ng_attn_decode_q8", hd)(_Q8_ATTENTION.pack(*at, 0, *rest), _stream()), "attn_decode_q8")
+    _check(_q8_fn("attention_q8", "ng_attn_decode_q8", hd)(_Q8_ATTENTION.pack(*at, 0, *rest), stream), "attn_decode_q8")
 
 
 def attn_prefill_q8(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, k_scales: torch.Tensor, v_scales: torch.Tensor,
@@ -718,13 +727,13 @@ def attn_prefill_q8(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     """Flash attention of the step's portions over a cache in 8 bits (``cache_write_q8``); their own keys are read from the cache too.
     Entries of one token are left to ``attn_decode_q8`` when ``skip_single``.  ``n_splits`` (``attn_prefill_q8_splits``) runs of every
     block's keys, merged through ``scratch`` (``attn_q8_scratch_floats`` of q's rows)."""
-    hd, at, rest = _q8_attention("attn_prefill_q8", q, k_pages, v_pages, k_scales, v_scales, table, cu_q, ctx_before, out, scratch,
+    hd, stream, at, rest = _q8_attention("attn_prefill_q8", q, k_pages, v_pages, k_scales, v_scales, table, cu_q, ctx_before, out, scratch,
                                  n_entries, max_q, n_heads, window, scale, int(bool(skip_single)), n_splits, slopes, q.shape[0])
     if ATTN_BACKEND == "sm100" and hd in (64, 128) and scale > 0 and at[0] % 16 == 0 and at[8] % 16 == 0:
         f, status = _q8_fn("attention_q8_sm100", "ng_attn_prefill_q8_sm100", hd), _gemm_status(q.device).data_ptr()
     else:
         f, status = _q8_fn("attention_q8", "ng_attn_prefill_q8", hd), 0
-    _check(f(_Q8_ATTENTION.pack(*at, status, *rest), _stream()), "attn_prefill_q8")
+    _check(f(_Q8_ATTENTION.pack(*at, status, *rest), stream), "attn_prefill_q8")
 
 
 # ----------------------------------------------------------------------------- attention with float32 weights
