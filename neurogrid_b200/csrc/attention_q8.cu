@@ -525,7 +525,8 @@ struct PfArgs {
     bf16* out;
     float* scratch;
     const float* slopes;
-    int n_rows, nH, window, n_splits, skip_single;
+    int n_rows, n_entries, nH, window, skip_single;
+    int n_splits;
     float scale;
 };
 struct PfTile {
@@ -590,13 +591,12 @@ attn_prefill_q8_kernel(const PfArgs a) {
     extern __shared__ __align__(16) unsigned char smem_raw[];
     PfSmem* sm = reinterpret_cast<PfSmem*>(smem_raw);
     ng_pdl_trigger();
-    // heads fastest, row tiles from the last down: the blocks with the most keys start first
-    const int e = blockIdx.z / a.n_splits, split = blockIdx.z - e * a.n_splits, kvh = blockIdx.x;
+    const int split = blockIdx.z, kvh = blockIdx.x, G = a.nH / a.c.nKV;
+    const RowTile mine = row_tile(a.cu_q, a.n_entries, a.n_rows, G, PF_ROWS, a.skip_single, blockIdx.y);
+    const int e = max(mine.e, 0), r0 = mine.first;
     const int q0 = a.cu_q[e], qlen = min(a.cu_q[e + 1], a.n_rows) - q0, ctx = a.ctx_before[e];
     ng_pdl_wait();
-    const int G = a.nH / a.c.nKV;
-    const int r0 = (gridDim.y - 1 - blockIdx.y) * PF_ROWS;
-    if (q0 < 0 || ctx < 0 || ctx > a.c.last_key || r0 >= qlen * G || (a.skip_single && a.cu_q[e + 1] - q0 == 1)) return;
+    if (mine.e < 0 || ctx < 0 || ctx > a.c.last_key) return;
     const int rows_here = min(PF_ROWS, qlen * G - r0);
     const int pos_first = ctx + r0 / G, pos_last = ctx + (r0 + rows_here - 1) / G;
     const int key_lo = a.window > 0 ? max(0, pos_first - a.window + 1) : 0;
@@ -816,7 +816,7 @@ NG_EXPORT int ng_attn_decode_q8(const NgAttnQ8* call, cudaStream_t stream) {
     else if (nt == 1) DC_KINDS(1, 8);
     else if (block >= 16) DC_KINDS(DC_NT_MAX, 16);
     else DC_KINDS(DC_NT_MAX, 8);
-    if (n_splits > 1) return q8_merge(c, a.c, 1, 1, 1, stream);
+    if (n_splits > 1) return q8_merge(c, a.c, true, 1, stream);
     return ng_launch_status();
 }
 
@@ -826,12 +826,14 @@ NG_EXPORT int ng_attn_prefill_q8(const NgAttnQ8* call, cudaStream_t stream) {
     const int kind = c.kind;
     if (c.n_entries <= 0 || c.n_rows <= 0 || c.max_q <= 0) return NG_OK;
     PfArgs a;
-    if (!attn_q8_args(c, a.c) || (long long)c.n_entries * c.n_splits > 65535 || (((uintptr_t)c.q | (uintptr_t)c.out) & 3)) return NG_BAD_SIZE;
-    const long long tiles = ((long long)c.max_q * (c.n_heads / c.n_kv) + PF_ROWS - 1) / PF_ROWS;
+    if (!attn_q8_args(c, a.c) || c.n_splits > 65535 || (((uintptr_t)c.q | (uintptr_t)c.out) & 3)) return NG_BAD_SIZE;
+    const long long tiles = q8_row_tiles(c, PF_ROWS);
     if (tiles > 65535) return NG_BAD_SIZE;
+    if (tiles <= 0) return NG_OK;                              // (one row, and single tokens are left out)
     a.q = (const bf16*)c.q; a.cu_q = c.cu_q; a.ctx_before = c.ctx_before; a.out = (bf16*)c.out; a.scratch = c.scratch; a.slopes = c.slopes;
-    a.n_rows = c.n_rows; a.nH = c.n_heads; a.window = c.window; a.n_splits = c.n_splits; a.skip_single = c.skip_single; a.scale = c.scale;
-    const dim3 grid(c.n_kv, (unsigned)tiles, c.n_entries * c.n_splits);
+    a.n_rows = c.n_rows; a.n_entries = c.n_entries; a.nH = c.n_heads; a.window = c.window; a.n_splits = c.n_splits; a.skip_single = c.skip_single;
+    a.scale = c.scale;
+    const dim3 grid(c.n_kv, (unsigned)tiles, c.n_splits);
 #define PF_GO(KIND)                                                                                                  \
     do {                                                                                                             \
         static std::atomic<unsigned long long> once{0};                                                              \
@@ -840,6 +842,6 @@ NG_EXPORT int ng_attn_prefill_q8(const NgAttnQ8* call, cudaStream_t stream) {
     } while (0)
     if (kind == NG_Q8_E4M3) PF_GO(NG_Q8_E4M3);
     else PF_GO(NG_Q8_INT8);
-    if (c.n_splits > 1) return q8_merge(c, a.c, c.skip_single ? 2 : 1, 0x7fffffff, c.max_q, stream);
+    if (c.n_splits > 1) return q8_merge(c, a.c, false, c.skip_single ? 2 : 1, stream);
     return ng_launch_status();
 }

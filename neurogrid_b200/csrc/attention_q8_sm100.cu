@@ -105,7 +105,7 @@ struct Params {
     bf16* out;
     const int *cu_q, *ctx_before;
     int* status;
-    int n_rows, nH, window, skip_single, n_splits;
+    int n_rows, n_entries, nH, window, skip_single, n_splits;
     float scale;
     const float* slopes;
     float* scratch;
@@ -127,12 +127,11 @@ attn_prefill_q8_sm100_kernel(const Params p) {
     uint32_t elected;
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(elected));
     const bool leader = elected != 0;
-    // heads run fastest and the row tiles from the last one down: the blocks with the most keys start first
-    const int e = blockIdx.z / p.n_splits, split = blockIdx.z - e * p.n_splits, kvh = blockIdx.x;
-    const int q0 = p.cu_q[e], q1 = p.cu_q[e + 1], qlen = min(q1, p.n_rows) - q0, ctx = p.ctx_before[e];
-    const int G = p.nH / p.c.nKV;
-    const int r0 = (gridDim.y - 1 - blockIdx.y) * BR;
-    if (q0 < 0 || ctx < 0 || ctx > p.c.last_key || r0 >= qlen * G || (p.skip_single && q1 - q0 == 1)) {
+    const int split = blockIdx.z, kvh = blockIdx.x, G = p.nH / p.c.nKV;
+    const RowTile mine = row_tile(p.cu_q, p.n_entries, p.n_rows, G, BR, p.skip_single, blockIdx.y);
+    const int e = max(mine.e, 0), r0 = mine.first;
+    const int q0 = p.cu_q[e], qlen = min(p.cu_q[e + 1], p.n_rows) - q0, ctx = p.ctx_before[e];
+    if (mine.e < 0 || ctx < 0 || ctx > p.c.last_key) {
         ng_pdl_wait();                                         // (a launch none of whose blocks waited would end before the one before it)
         return;
     }
@@ -600,15 +599,16 @@ NG_EXPORT int ng_attn_prefill_q8_sm100(const NgAttnQ8* call, cudaStream_t stream
     const int kind = c.kind;
     if (c.n_entries <= 0 || c.n_rows <= 0 || c.max_q <= 0) return NG_OK;
     Params p;
-    if (!attn_q8_args(c, p.c) || (long long)c.n_entries * c.n_splits > 65535 || !(c.scale > 0.f) || !c.status ||
+    if (!attn_q8_args(c, p.c) || c.n_splits > 65535 || !(c.scale > 0.f) || !c.status ||
         (((uintptr_t)c.q | (uintptr_t)c.out) & 15))
         return NG_BAD_SIZE;
-    const long long tiles = ((long long)c.max_q * (c.n_heads / c.n_kv) + BR - 1) / BR;
+    const long long tiles = q8_row_tiles(c, BR);
     if (tiles > 65535) return NG_BAD_SIZE;
-    p.q = (const bf16*)c.q; p.out = (bf16*)c.out; p.cu_q = c.cu_q; p.ctx_before = c.ctx_before; p.status = c.status; p.n_rows = c.n_rows;
+    if (tiles <= 0) return NG_OK;                              // (one row, and single tokens are left out)
+    p.q = (const bf16*)c.q; p.out = (bf16*)c.out; p.cu_q = c.cu_q; p.ctx_before = c.ctx_before; p.status = c.status; p.n_rows = c.n_rows; p.n_entries = c.n_entries;
     p.nH = c.n_heads; p.window = c.window; p.skip_single = c.skip_single; p.n_splits = c.n_splits; p.scale = c.scale; p.slopes = c.slopes;
     p.scratch = c.scratch;
-    const dim3 grid(c.n_kv, (unsigned)tiles, c.n_entries * c.n_splits);
+    const dim3 grid(c.n_kv, (unsigned)tiles, c.n_splits);
     constexpr int smem = (int)sizeof(Smem) + 1024;
 #define Q8P_GO(KIND)                                                                                                     \
     do {                                                                                                                 \
@@ -618,6 +618,6 @@ NG_EXPORT int ng_attn_prefill_q8_sm100(const NgAttnQ8* call, cudaStream_t stream
     } while (0)
     if (kind == NG_Q8_E4M3) Q8P_GO(NG_Q8_E4M3);
     else Q8P_GO(NG_Q8_INT8);
-    if (c.n_splits > 1) return q8_merge(c, p.c, c.skip_single ? 2 : 1, 0x7fffffff, c.max_q, stream);
+    if (c.n_splits > 1) return q8_merge(c, p.c, false, c.skip_single ? 2 : 1, stream);
     return ng_launch_status();
 }

@@ -49,32 +49,77 @@ __device__ __forceinline__ void ld_codes(uint32_t* w, const unsigned char* p) {
         asm volatile("{\n\t.reg .u16 h;\n\tld.global.L1::no_allocate.u16 h, [%1];\n\tcvt.u32.u16 %0, h;\n\t}" : "=r"(w[0]) : "l"(p) : "memory");
 }
 
+// Which rows a block of a portion's launch has: tiles of `rows` (token, head) rows of each entry, entry by entry, an entry's from the last down (the
+// blocks with the most keys start first); `index` counts them all.  Entries without rows, and single tokens where they are left out,
+// have none, so that a launch beside many single tokens is not mostly blocks that find nothing to do (a portion of 512 tokens behind 2,000 beside 64
+// single tokens 44 us; with a grid of entries x their longest's tiles 70, and cut into two runs 46 and, merged over that grid too, 356).  By
+// a warp, 32 entries at a time.
+struct RowTile { int e, first; };                                    // e < 0: behind the last tile
+__device__ __forceinline__ RowTile row_tile(const int* cu_q, int n_entries, int n_rows, int group, int rows, bool skip_single, int index) {
+    const int lane = threadIdx.x & 31;
+    for (int e0 = 0; e0 < n_entries; e0 += 32) {
+        int n = 0;
+        if (e0 + lane < n_entries) {
+            const int q0 = cu_q[e0 + lane], q1 = cu_q[e0 + lane + 1];
+            if (q0 >= 0 && min(q1, n_rows) > q0 && !(skip_single && q1 - q0 == 1)) n = ((min(q1, n_rows) - q0) * group + rows - 1) / rows;
+        }
+        int upto = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += x;
+        }
+        const uint32_t in = __ballot_sync(0xffffffffu, index < upto);
+        if (in) {
+            const int l = __ffs(in) - 1;
+            return RowTile{e0 + l, (__shfl_sync(0xffffffffu, upto, l) - 1 - index) * rows};
+        }
+        index -= __shfl_sync(0xffffffffu, upto, 31);
+    }
+    return RowTile{-1, 0};
+}
+// the entry of a row (the last whose rows do not begin behind it), by a warp: 32 probes at a time; -1: none
+__device__ __forceinline__ int entry_of_row(const int* cu_q, int n_entries, int row) {
+    const int lane = threadIdx.x & 31;
+    int lo = 0, hi = n_entries;
+    if (cu_q[0] > row || cu_q[n_entries] <= row) return -1;
+    while (hi - lo > 1) {
+        const int step = (hi - lo + 31) / 32, at = lo + lane * step;
+        const int ahead = __popc(__ballot_sync(0xffffffffu, at < hi && cu_q[min(at, n_entries)] <= row));       // (lane 0's is)
+        lo += (max(ahead, 1) - 1) * step;
+        hi = min(lo + step, hi);
+    }
+    return lo;
+}
+
 // out[row, head] = sum_s o_s 2^(m_s - m) / sum_s l_s 2^(m_s - m) over the runs s.  A warp has a (row, head) (WIDE: all four warps of a block, every
 // fourth run each, joined in order): lane s looks after run s's reference point and sum, then the lanes share the dimensions and walk the
-// runs in ascending order.  Rows are the entries' single tokens, whose first record says how many runs there are, or (portions) all rows of
-// the entries that bring more.
+// runs in ascending order.  SINGLE: rows are the entries' single tokens, with records by entry, of which the first says how many there are;
+// else all rows of the entries that bring at least `least`.
 #define MG_WARPS 4
 constexpr int MG_EACH = (HD + 63) / 64;                              // pairs of dimensions a lane has
-template <bool WIDE>
+template <bool WIDE, bool SINGLE>
 __global__ void __launch_bounds__(MG_WARPS * 32)
 attn_q8_merge_kernel(const float* __restrict__ scratch, const int* __restrict__ cu_q, const int* __restrict__ ctx_before, int last_key,
-                     bf16* __restrict__ out, int nH, int room, int n_rows, int least, int most) {
+                     bf16* __restrict__ out, int nH, int room, int n_rows, int n_entries, int least) {
     __shared__ float part_s[WIDE ? MG_WARPS : 1][HD + 2];
     ng_pdl_trigger();
-    const int e = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int head = WIDE ? blockIdx.x : blockIdx.x * MG_WARPS + warp;
-    const int q0 = cu_q[e], n = cu_q[e + 1] - q0, ctx = ctx_before[e];
     ng_pdl_wait();
-    if (n < least || n > most || q0 < 0 || ctx < 0 || ctx > last_key || (!WIDE && head >= nH)) return;       // (entries that left no records)
     scratch = ng_after_wait(scratch);
     constexpr int STEP = WIDE ? MG_WARPS : 1;
-    for (int r = q0 + blockIdx.z; r < min(q0 + n, n_rows); r += gridDim.z) {
-        const float* rec = scratch + ((size_t)(most == 1 ? e : r) * nH + head) * room * REC;      // (single tokens': by entry)
+    for (int i = blockIdx.y; i < (SINGLE ? n_entries : n_rows); i += gridDim.y) {
+        const int e = SINGLE ? i : entry_of_row(cu_q, n_entries, i);
+        if (e < 0) continue;
+        const int q0 = cu_q[e], n = cu_q[e + 1] - q0, ctx = ctx_before[e], r = SINGLE ? q0 : i;
+        if ((SINGLE ? n != 1 : n < least) || q0 < 0 || r >= n_rows || ctx < 0 || ctx > last_key || (!WIDE && head >= nH)) continue;      // (no records)
+        const float* rec = scratch + ((size_t)i * nH + head) * room * REC;
         // (the first 32 runs' are asked for before it is known how many there are)
         const int s0 = lane * STEP + (WIDE ? warp : 0);
         float m0 = s0 < room ? rec[(size_t)s0 * REC] : -INFINITY, l0 = s0 < room ? rec[(size_t)s0 * REC + 1] : 0.f;
         int runs = room;
-        if (most == 1) {
+        if constexpr (SINGLE) {
             runs = (int)rec[2];
             if (runs <= 1) continue;
         }
@@ -176,18 +221,28 @@ static bool attn_q8_args(const NgAttnQ8& c, Cache& to) {
            c.n_splits >= 1 && (c.n_splits == 1 || (c.scratch && !((uintptr_t)c.scratch & 15)));
 }
 
-// least .. most: the rows that an entry brings to have records
-static int q8_merge(const NgAttnQ8& c, const Cache& cache, int least, int most, int rows, cudaStream_t stream) {
-    const int z = rows < 1 ? 1 : rows > 65535 ? 65535 : rows;
+// single: the entries' single tokens; else the rows of entries that bring at least `least`
+static int q8_merge(const NgAttnQ8& c, const Cache& cache, bool single, int least, cudaStream_t stream) {
+    const int count = single ? c.n_entries : c.n_rows;
     // A block a (row, head), or a warp: until the rows fill the GPU by themselves the wide form is the faster.  Heads of 64, with the attention in
     // front of it, wide / narrow, us: 1 row of 32 heads, 17 runs 8.3 / 11.9, 48 runs 15.5 / 24.6; 8 rows, 16 runs 11.2 / 11.9; 64 rows, 2 to
     // 16 runs 32.6 / 33.0 and 52.1 / 52.6; 256 rows, 8 runs 66.1 / 60.4; portions of 16 rows, 18 runs 34.7 / 38.4, 64 rows 41.2 / 45.6,
     // 128 rows, 9 runs 42.4 / 42.3, 512 rows, 2 runs 266 / 254
-    if ((long long)c.n_entries * c.n_heads * z <= 4096)
-        NG_LAUNCH((attn_q8_merge_kernel<true>), dim3(c.n_heads, c.n_entries, z), MG_WARPS * 32, 0, stream, c.scratch, c.cu_q, c.ctx_before,
-                  cache.last_key, (bf16*)c.out, c.n_heads, c.n_splits, c.n_rows, least, most);
-    else
-        NG_LAUNCH((attn_q8_merge_kernel<false>), dim3((c.n_heads + MG_WARPS - 1) / MG_WARPS, c.n_entries, z), MG_WARPS * 32, 0, stream, c.scratch,
-                  c.cu_q, c.ctx_before, cache.last_key, (bf16*)c.out, c.n_heads, c.n_splits, c.n_rows, least, most);
+    const bool wide = (long long)count * c.n_heads <= 4096;
+    const dim3 grid(wide ? c.n_heads : (c.n_heads + MG_WARPS - 1) / MG_WARPS, count < 65535 ? count : 65535);
+#define MG_GO(WIDE, SINGLE)                                                                                                          \
+    NG_LAUNCH((attn_q8_merge_kernel<WIDE, SINGLE>), grid, MG_WARPS * 32, 0, stream, c.scratch, c.cu_q, c.ctx_before, cache.last_key, \
+              (bf16*)c.out, c.n_heads, c.n_splits, c.n_rows, c.n_entries, least)
+    if (single && wide) MG_GO(true, true);
+    else if (single) MG_GO(false, true);
+    else if (wide) MG_GO(true, false);
+    else MG_GO(false, false);
     return ng_launch_status();
+}
+// Row tiles that the portions' launch has to have room for: whole ones, and for each entry that may bring rows one that is not.
+static long long q8_row_tiles(const NgAttnQ8& c, int rows) {
+    const int group = c.n_heads / c.n_kv, least = c.skip_single ? 2 : 1;
+    const long long whole = (long long)c.n_rows * group / rows, some = c.n_entries < c.n_rows / least ? c.n_entries : c.n_rows / least;
+    const long long all = c.n_entries * (((long long)c.max_q * group + rows - 1) / rows);
+    return all < whole + some ? all : whole + some;
 }

@@ -675,7 +675,7 @@ def attn_prefill_q8_splits(q_lens, n_heads: int, n_kv_heads: int, head_dim: int,
     def cost(s):
         return -(-blocks * s // slots) * (tiles / s + 9) + (3 + records * s / 8000 if s > 1 else 0)
 
-    return min(range(1, max(1, min(tiles // 4, slots // n_kv_heads, 65535 // max(1, len(q_lens)))) + 1), key=cost)
+    return min(range(1, max(1, min(tiles // 4, slots // n_kv_heads)) + 1), key=cost)
 
 
 def _q8_attention(what, q, k_pages, v_pages, k_scales, v_scales, table, cu_q, ctx_before, out, scratch, n_entries, max_q, n_heads, window,

@@ -217,6 +217,8 @@ def check_rows(got, want, bound, rows=None):
     ok = err <= bound
     if rows is not None:
         ok, err = ok[rows], err[rows]
+    if ok.numel() == 0:
+        return
     assert bool(ok.all()), f"worst {float(err.max()):.3e}, over the bound at {int((~ok).sum())} of {ok.numel()}"
 
 
@@ -460,6 +462,22 @@ def test_decode_shares_of_many_entries(splits):
     got = run_decode(c, q, 8, None, 0.125, splits)
     check_rows(got, want, bound, single)
     assert bool((got[[r for r in range(c.rows) if r not in single]] == 7.0).all())
+
+
+@pytest.mark.parametrize("hd", [32, 64])
+@pytest.mark.parametrize("splits", [1, 2])
+@pytest.mark.parametrize("lens", [[1] * 70 + [90] + [0, 1, 2] * 20 + [65], [1], [3, 1], [1] * 40 + [0] * 40, [0, 0, 5, 0]])
+def test_portions_beside_many_single_tokens(hd, splits, lens):
+    """Row tiles are counted over the entries that have any, wherever they lie."""
+    ctx = [(37 * i) % 150 for i in range(len(lens))]
+    c = Cache(lens, ctx, 2, hd, 16, 16, INT8, seed=3)
+    q = rnd(c.rows, 6 * hd, seed=7)
+    want, bound = ref.attention(q, *c.args(), c.cu_host, c.ctx, 6, None, 0.125)
+    many = [r for e, n in enumerate(lens) for r in range(c.cu_host[e], c.cu_host[e + 1]) if n > 1]
+    got = run_prefill(c, q, 6, None, 0.125, splits, True)
+    check_rows(got[many], want[many], bound[many])
+    assert bool((got[[r for r in range(c.rows) if r not in many]] == 7.0).all())
+    check_rows(run_prefill(c, q, 6, None, 0.125, splits, False), want, bound)
 
 
 def test_the_integer_that_the_writer_never_stores():
