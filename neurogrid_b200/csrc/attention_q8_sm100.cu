@@ -122,7 +122,6 @@ attn_prefill_q8_sm100_kernel(const Params p) {
     extern __shared__ unsigned char smem_raw[];
     // (an offset, not a rounded address: the compiler then knows that what it points to is shared memory)
     Smem* sm = reinterpret_cast<Smem*>(smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u));
-    ng_pdl_trigger();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     uint32_t elected;
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(elected));
@@ -186,14 +185,18 @@ attn_prefill_q8_sm100_kernel(const Params p) {
     };
     Pages page0{}, page1{};
     if (loader >= 0 && loader < KV_WARPS) page0 = pages(tile0), page1 = pages(tile0 + 1);
+    ng_pdl_wait();                                             // q and the pages are this step's data
+    // All of the SM's tensor memory: asked for behind the wait, and the next kernel let in behind the allocation.  A block of a tcgen05 product of few
+    // rows fits on the SM beside this one (its 4,096 registers and 110 KB are what is left): had it tensor memory before this block did, this
+    // block would wait for it, and it for this kernel (or, in front of this kernel, this block for it and it for the tensor memory).
     if (warp == SOFTMAX_WARPS + KV_WARPS) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" :: "r"(smem_u32(&sm->tmem_base)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    ng_pdl_wait();                                             // q and the pages are this step's data
     tcgen05_fence_before();
     __syncthreads();
     tcgen05_fence_after();
+    ng_pdl_trigger();
     const uint32_t tmem = sm->tmem_base;                       // S of row tile t, tile j: 128 t + 64 (j & 1); O: tm_o(t, j)
     auto tm_o = [&](int t, int j) { return tmem + 256 + HD * (STREAMS == 2 ? 2 * t + (j & 1) : t); };
     bool ok = true;

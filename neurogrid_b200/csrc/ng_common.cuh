@@ -66,7 +66,7 @@ __device__ __forceinline__ float ng_block_sum(float v, float* smem32) {
 // ---- programmatic dependent launch ---------------------------------------------------------
 // Every kernel of the package is launched with the "programmatic stream serialization"
 // attribute, signals at its top that the next kernel of the stream may be scheduled
-// (ng_pdl_trigger), and waits (ng_pdl_wait) before it first reads what earlier kernels wrote or
+// (ng_pdl_trigger; one that takes all of an SM's tensor memory: behind that allocation), and waits (ng_pdl_wait) before it first reads what earlier kernels wrote or
 // writes anything to global memory.  The next kernel's launch latency and prologue then overlap
 // this kernel's tail.  Without the attribute both instructions do nothing.
 // NEUROGRID_B200_PDL=0 in the environment switches the attribute off.
