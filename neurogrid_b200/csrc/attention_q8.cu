@@ -114,7 +114,7 @@ __device__ __forceinline__ void dc_load(DcGroup<GRAN>& r, const DcBase& b, const
 template <int NT>
 struct DcState {
     float o[NT][HD / 16][4], m[NT][2], l[NT][2];
-    uint32_t seen;                           // a bit for each tile of heads: a key has been met
+    uint32_t seen;                           // a bit for each (tile of heads, of the lane's two): a finite score has been met
 };
 __device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
     uint32_t y;
@@ -182,31 +182,28 @@ __device__ __forceinline__ void dc_compute(DcState<NT>& st, DcGroup<GRAN>& r, co
         for (int s = 0; s < SUB; ++s)
 #pragma unroll
             for (int j = 0; j < 4; ++j) mx[n][j & 1] = fmaxf(mx[n][j & 1], sc[n][s][j]);
-        up |= fmaxf(mx[n][0], mx[n][1]) > 8.f || !(st.seen >> n & 1);
+        up |= fmaxf(mx[n][0], mx[n][1]) > 8.f || (st.seen >> 2 * n & 3) != 3;
     }
     // the reference point follows the maximum lazily: weights may reach 2^8 before the sums are rescaled.  It starts at 0 and moves to a head's
-    // first maximum, up or down, with sums that are zero.
+    // first maximum, up or down, with sums that are zero.  Each head has its own bit for that: one whose scores are all NaN never gets it.
     if (__any_sync(0xffffffffu, up)) {
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            bool any = true;
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                float x = mx[n][j];
+                float x = mx[n][j];                                  // (the same in every lane that has the head: so is the bit)
 #pragma unroll
                 for (int o = 4; o <= 16; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
-                const bool first = !(st.seen >> n & 1);
-                const float by = x == -INFINITY ? 0.f : first ? x : fmaxf(x, 0.f), c = q8_ex2(-by);
-                any = any && x != -INFINITY;
+                const bool first = !(st.seen >> (2 * n + j) & 1);
+                const float by = x == -INFINITY ? 0.f : first ? x : fmaxf(x, 0.f), c = first ? 1.f : q8_ex2(-by);
                 st.m[n][j] += by;
-                st.l[n][j] *= first ? 1.f : c;
+                st.l[n][j] *= c;
 #pragma unroll
-                for (int i = 0; i < HD / 16; ++i)
-                    if (!first) { st.o[n][i][j] *= c; st.o[n][i][2 + j] *= c; }
+                for (int i = 0; i < HD / 16; ++i) { st.o[n][i][j] *= c; st.o[n][i][2 + j] *= c; }
+                if (x != -INFINITY) st.seen |= 1u << (2 * n + j);
 #pragma unroll
                 for (int s = 0; s < SUB; ++s) { sc[n][s][j] -= by; sc[n][s][2 + j] -= by; }
             }
-            if (__any_sync(0xffffffffu, any)) st.seen |= 1u << n;     // (a key is seen by all heads or by none)
         }
     }
     uint32_t pb[NT][SUB][2];
@@ -429,7 +426,7 @@ __device__ __forceinline__ void dc_piece(const DcArgs& a, float* red_s, int e, i
             const int h = 8 * n + 2 * t + j;
             if (h >= heads) continue;
             float* mine = red_s + (size_t)(warp * heads + h) * REC;
-            if (g == 0) mine[0] = st.seen >> n & 1 ? st.m[n][j] : -INFINITY, mine[1] = l;
+            if (g == 0) mine[0] = st.seen >> (2 * n + j) & 1 ? st.m[n][j] : -INFINITY, mine[1] = l;
 #pragma unroll
             for (int i = 0; i < HD / 16; ++i)
                 *reinterpret_cast<float2*>(mine + 4 + dc_dim(i, g, 0)) = make_float2(st.o[n][i][j], st.o[n][i][2 + j]);

@@ -41,3 +41,23 @@ def test_portions_between_products_that_use_tensor_memory(rows, hd):
         y.zero_()
         graph.replay()
         assert torch.equal(y, want)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("nH,nKV,hd", [(8, 1, 64), (7, 1, 64), (16, 1, 64), (16, 2, 128), (15, 1, 32), (8, 1, 48), (24, 3, 256)])
+@pytest.mark.parametrize("splits", [1, 5])
+def test_heads_of_nan_leave_the_other_heads_of_their_tile_alone(kind, nH, nKV, hd, splits):
+    """NaN in one head of every pair that a lane looks after, over many groups of keys."""
+    c = Cache([1, 1, 1], [700, 3, 1500], nKV, hd, 16, 16, kind, seed=nH)
+    q = rnd(3, nH * hd, seed=9, std=1.5)
+    sick = torch.zeros(nH, dtype=torch.bool)
+    sick[0::2] = True
+    q.view(3, nH, hd)[:2, sick.to(DEV), hd // 2] = math.nan
+    q.view(3, nH, hd)[2, (~sick).to(DEV), 0] = math.nan
+    got = run_decode(c, q, nH, None, hd ** -0.5, splits)
+    want, bound = ref.attention(torch.nan_to_num(q), *c.args(), c.cu_host, c.ctx, nH, None, hd ** -0.5)
+    for r in range(3):
+        ill = sick if r < 2 else ~sick
+        of_row = [t[r].view(nH, hd) for t in (got, want, bound)]
+        assert bool(torch.isnan(of_row[0][ill.to(DEV)]).all())
+        check_rows(of_row[0][(~ill).to(DEV)], of_row[1][~ill], of_row[2][~ill])
