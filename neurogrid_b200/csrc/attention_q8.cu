@@ -11,7 +11,8 @@
 // whose values are small has small weights, not small values, and the sum over the codes never leaves float16's range.  (A key is lost to the
 // denominator where its weight times t_j is less than 2^-126 of the largest such product: blocks of zeros, whose scale is 2^-100, keep
 // theirs down to 2^-26 of the largest weight times the largest scale.)
-// Entries whose context is below zero or behind the table's last place are passed over, their rows left as they were.
+// Entries whose context is below zero or behind the table's last place are passed over, their rows left as they were.  Keys whose page is not there
+// (below zero, or beyond the pool) are hidden from every row.
 #include "ng_q8_attention.cuh"
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -528,7 +529,7 @@ struct PfArgs {
 };
 struct PfTile {
     uint32_t k[PF_EACH][4], v[PF_EACH][4];
-    float ks, vs;                                                    // threads 0 .. 7: of their 8 keys
+    float ks, vs;                                                    // threads 0 .. 7: of their 8 keys; vs -1: they have no page
 };
 __device__ __forceinline__ void pf_load(PfTile& r, const Cache& c, const int* trow, int key0, int key_lo, int k_end, int kvh) {
     const int mask = (1 << c.ps_log2) - 1;
@@ -546,7 +547,8 @@ __device__ __forceinline__ void pf_load(PfTile& r, const Cache& c, const int* tr
             ld_codes<16>(r.v[n], c.v + at);
         }
     }
-    r.ks = r.vs = 1.f;
+    r.ks = 1.f;
+    r.vs = -1.f;
     if (threadIdx.x < PF_KEYS / 8) {
         const int key = key0 + 8 * threadIdx.x;
         int page = -1;
@@ -577,8 +579,8 @@ __device__ __forceinline__ void pf_store(PfSmem* sm, int s, const PfTile& r) {
     }
     if (threadIdx.x < PF_KEYS / 8) {
         sm->ks[s][threadIdx.x] = r.ks;
-        sm->vl[s][threadIdx.x] = q8_log2(r.vs);
-        sm->vi[s][threadIdx.x] = q8_recip(r.vs);
+        sm->vl[s][threadIdx.x] = r.vs < 0.f ? -INFINITY : q8_log2(r.vs);         // hidden
+        sm->vi[s][threadIdx.x] = q8_recip(r.vs);                     // (1, times weights of 0)
     }
 }
 

@@ -14,7 +14,8 @@
 // A row tile has two S buffers, for even and odd key tiles.  The tensor pipe runs the issuer's MMAs in order and a commit covers all
 // before it, so "S of tile j + 2 is complete" also says that P V of tile j has read its P.
 //
-// Keys that no row of the block sees, and keys whose page is not there, are stored as zeros (their codes may be NaN).  A NaN among the values of
+// Keys that no row of the block sees, and keys whose page is not there, are stored as zeros (their codes may be NaN).  The latter are hidden: the
+// logarithm of their scale is minus infinity, and so is their z.  A NaN among the values of
 // a key that some rows of the block see reaches the others of its tile as well (0 NaN), as it does in a plain product with masked weights.
 // Every mbarrier wait is bounded; a waiter that gives up sets a status bit and the block runs to its end.
 //
@@ -210,7 +211,7 @@ attn_prefill_q8_sm100_kernel(const Params p) {
         const long long page_bytes = (long long)(p.c.nKV << p.c.ps_log2) * HD, head_at = (long long)(kvh << p.c.ps_log2) * HD + lane * 16;
         const unsigned char *k_pages = p.c.k + head_at, *v_pages = p.c.v + head_at;
         uint32_t k[DEPTH][UNITS][UNIT_LOADS][4], v[DEPTH][UNITS][UNIT_LOADS][4];
-        float ks[DEPTH], vs[DEPTH];
+        float ks[DEPTH], vs[DEPTH];                            // (vs: -1 for a unit that has no page)
         // (a page that is not there: page 0 is read, and the unit's keys become zeros when they are stored)
         bool bad[DEPTH][UNITS];
         auto load = [&](int d, int tile, const Pages& page) {
@@ -224,7 +225,8 @@ attn_prefill_q8_sm100_kernel(const Params p) {
                     ld_codes<16>(v[d][n][i], v_pages + at + i * 512);
                 }
             }
-            ks[d] = vs[d] = 1.f;
+            ks[d] = 1.f;
+            vs[d] = -1.f;
             if ((unsigned)page.mine < (unsigned)p.c.num_pages) {
                 const long long sc = ((long long)page.mine * p.c.nKV + kvh << (p.c.ps_log2 - p.c.bl_log2)) + ((tile * BK + 8 * lane & mask) >> p.c.bl_log2);
                 ld_codes<4>(reinterpret_cast<uint32_t*>(&ks[d]), reinterpret_cast<const unsigned char*>(p.c.ks + sc));
@@ -270,8 +272,8 @@ attn_prefill_q8_sm100_kernel(const Params p) {
                     }
                 if (w == KV_WARPS - 1 && lane < 8) {
                     sm->ks[s][lane] = ks[d];
-                    sm->vl[s][lane] = q8_log2(vs[d]);
-                    sm->vi[s][lane] = q8_recip(vs[d]);
+                    sm->vl[s][lane] = vs[d] < 0.f ? -INFINITY : q8_log2(vs[d]);
+                    sm->vi[s][lane] = q8_recip(vs[d]);         // (of a unit without a page: 1, times weights of 0)
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();

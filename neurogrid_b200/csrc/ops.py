@@ -712,7 +712,8 @@ def attn_decode_q8(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
                    n_entries: int, n_heads: int, window: Optional[int], scale: float, n_splits: int, max_ctx: int,
                    slopes: Optional[torch.Tensor] = None) -> None:
     """``attn_decode_bf16`` over a cache in 8 bits (``cache_write_q8``): split-context attention of the entries that bring one token, any
-    number of query heads a KV head.  The rows of other entries stay as they were.  ``n_splits`` (``attn_decode_q8_splits``) runs of
+    number of query heads a KV head.  The rows of other entries stay as they were.  Keys whose page the table does not have (-1, or a
+    number beyond the pool) are hidden; a row that sees no key is zero.  ``n_splits`` (``attn_decode_q8_splits``) runs of
     the keys, planned for contexts of up to ``max_ctx`` (longer ones are right too); ``scratch`` holds ``attn_q8_scratch_floats`` (of
     ``n_entries``) float32 values when there is more than one."""
     hd, stream, at, rest = _q8_attention("attn_decode_q8", q, k_pages, v_pages, k_scales, v_scales, table, cu_q, ctx_before, out, scratch, n_entries,
@@ -725,6 +726,7 @@ def attn_prefill_q8(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
                     n_heads: int, window: Optional[int], scale: float, skip_single: bool, slopes: Optional[torch.Tensor] = None,
                     scratch: Optional[torch.Tensor] = None, n_splits: int = 1) -> None:
     """Flash attention of the step's portions over a cache in 8 bits (``cache_write_q8``); their own keys are read from the cache too.
+    Keys without a page are hidden, as they are from single tokens.
     Entries of one token are left to ``attn_decode_q8`` when ``skip_single``.  ``n_splits`` (``attn_prefill_q8_splits``) runs of every
     block's keys, merged through ``scratch`` (``attn_q8_scratch_floats`` of q's rows)."""
     hd, stream, at, rest = _q8_attention("attn_prefill_q8", q, k_pages, v_pages, k_scales, v_scales, table, cu_q, ctx_before, out, scratch,

@@ -61,3 +61,66 @@ def test_heads_of_nan_leave_the_other_heads_of_their_tile_alone(kind, nH, nKV, h
         of_row = [t[r].view(nH, hd) for t in (got, want, bound)]
         assert bool(torch.isnan(of_row[0][ill.to(DEV)]).all())
         check_rows(of_row[0][(~ill).to(DEV)], of_row[1][~ill], of_row[2][~ill])
+
+
+def attention_with_holes(q, c, n_heads, window, scale, slopes, hidden):
+    """ref.attention's 64-bit values where keys in ``hidden`` [entry][key] are not there, and sum_j weight_j |v_j|."""
+    k_pages, v_pages, ks, vs = (t.cpu() for t in c.dev)
+    n_kv, hd = k_pages.shape[1], k_pages.shape[3]
+    out = torch.zeros(q.shape, dtype=torch.float64)
+    size = torch.zeros(q.shape, dtype=torch.float64)
+    for e in range(len(c.ctx)):
+        ctx, q0, n = c.ctx[e], c.cu_host[e], c.q_lens[e]
+        j = torch.arange(ctx + n)
+        p, at = c.table_host[e][j // c.page].long(), j % c.page
+        pos = torch.arange(ctx, ctx + n)[:, None]
+        for h in range(n_heads):
+            g = h // (n_heads // n_kv)
+            k, v = ((t[:, g].view(torch.uint8)[p, at].view(t.dtype).double() * s[p, g, at // c.block].double()[:, None])
+                    for t, s in ((k_pages, ks), (v_pages, vs)))
+            k[hidden[e][:ctx + n]], v[hidden[e][:ctx + n]] = 0.0, 0.0
+            s = q[q0:q0 + n, h * hd:(h + 1) * hd].cpu().double() @ k.T * scale
+            if slopes is not None:
+                s = s - float(slopes[h]) * (pos - j).double()
+            seen = (j <= pos) & ~hidden[e][:ctx + n]
+            if window:
+                seen = seen & (j > pos - window)
+            w = torch.softmax(s.masked_fill(~seen, -math.inf), -1)
+            w = torch.where(seen.any(-1, keepdim=True), w, 0.0)
+            out[q0:q0 + n, h * hd:(h + 1) * hd] = w @ v
+            size[q0:q0 + n, h * hd:(h + 1) * hd] = w @ v.abs()
+    return out, size
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("hd", [48, 64, 128])
+@pytest.mark.parametrize("page,block", [(8, 8), (32, 16), (64, 64)])
+@pytest.mark.parametrize("window,bias", [(None, False), (None, True), (150, False)])
+@pytest.mark.parametrize("splits", [1, 3])
+def test_keys_without_a_page_are_hidden_from_portions_and_single_tokens_alike(kind, hd, page, block, window, bias, splits):
+    """A table with holes, of no page and of a page beyond the pool, behind the tokens and among them; an entry none of whose pages is there."""
+    lens, ctx = [40, 1, 70, 1, 9], [300, 300, 5, 200, 30]
+    c = Cache(lens, ctx, 2, hd, page, block, kind, seed=hd + page)
+    q = rnd(c.rows, 8 * hd, seed=3, std=1.5)
+    slopes = torch.pow(2.0, -torch.arange(1, 9).float() / 2).to(DEV) if bias else None
+    hidden = [torch.zeros(400, dtype=torch.bool) for _ in lens]
+    table = c.table_host.clone()
+    for e in range(len(lens)):
+        held = -(-(lens[e] + ctx[e]) // page)
+        for i in (range(held) if e == 4 else {1, held // 2, held - 2} - {held - 1}):
+            if 0 <= i < held:
+                table[e, i] = -1 if (i + e) % 2 else c.k.shape[0] + 1000 * i
+                hidden[e][i * page:(i + 1) * page] = True
+    c.table = table.to(DEV)
+    want, size = attention_with_holes(q, c, 8, window, hd ** -0.5, slopes, hidden)
+    # q8_refs' terms: the output's rounding, weights in float16 and their smallest step, the scores' roundings (together below 2^-12 here)
+    largest = ref.LARGEST[kind] * 2.0 ** -4
+    bound = 2.0 ** -8 * want.abs() + (2.0 ** -11 + 2.0 ** -12) * size + 2.0 ** -25 * 400 * largest
+    single = [c.cu_host[e] for e, n in enumerate(lens) if n == 1]
+    many = [r for r in range(c.rows) if r not in single]
+    portions = run_prefill(c, q, 8, window, hd ** -0.5, splits, False, slopes)
+    check_rows(portions, want, bound)
+    check_rows(run_decode(c, q, 8, window, hd ** -0.5, splits, slopes), want, bound, single)
+    check_rows(run_prefill(c, q, 8, window, hd ** -0.5, splits, True, slopes), want, bound, many)
+    none = list(range(c.cu_host[4], c.cu_host[5]))
+    assert bool((portions[none] == 0).all())
