@@ -8,9 +8,9 @@
 // score.  t_j goes into the exponent: with z_j = x_j log2(e) + log2(t_j) and the reference point m near max z_j, the weights
 // w_j = 2^(z_j - m) are what meets the codes d_j, in float16 (half a step 2^-12 of the weight, smallest step 2^-24 of the
 // largest), and the denominator is sum_j w_j / t_j in 32 bits: t_j is a power of two, both forms are exact.  So a block
-// whose values are small has small weights, not small values, and the sum over the codes never leaves float16's range.  (A key is lost to the
-// denominator where its weight times t_j is less than 2^-126 of the largest such product: blocks of zeros, whose scale is 2^-100, keep
-// theirs down to 2^-26 of the largest weight times the largest scale.)
+// whose values are small has small weights, not small values, and the sum over the codes never leaves float16's range.  Where scales lie so far
+// apart (Q8_LOW) that a w_j may be lost which counts in the denominator, the denominator takes 2^(x_j log2(e) - m) by an exponential of
+// its own, and its sums are moved in two steps where one factor would be lost.
 // Entries whose context is below zero or behind the table's last place are passed over, their rows left as they were.  Keys whose page is not there
 // (below zero, or beyond the pool) are hidden from every row.
 #include "ng_q8_attention.cuh"
@@ -115,7 +115,7 @@ __device__ __forceinline__ void dc_load(DcGroup<GRAN>& r, const DcBase& b, const
 template <int NT>
 struct DcState {
     float o[NT][HD / 16][4], m[NT][2], l[NT][2];
-    uint32_t seen;                           // a bit for each (tile of heads, of the lane's two): a finite score has been met
+    uint32_t seen;                           // a bit for each (tile of heads, of the lane's two): a finite score has been met; the highest: Q8_HIGH
 };
 __device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
     uint32_t y;
@@ -153,6 +153,11 @@ __device__ __forceinline__ void dc_compute(DcState<NT>& st, DcGroup<GRAN>& r, co
                 const int key = key0 + 16 * s + GRAN * u;
                 if (key >= k_end || key + GRAN <= key_lo || (r.missing >> (s * UNITS + u) & 1)) r.ks[s][u] = r.vs[s][u] = 1.f;
             }
+    bool wide = false;                                               // (Q8_LOW)
+#pragma unroll
+    for (int s = 0; s < SUB; ++s)
+#pragma unroll
+        for (int u = 0; u < UNITS; ++u) wide = wide || r.vs[s][u] < q8_pow2(Q8_LOW);
     // z less the reference point as it stands: what 2^ is taken of, unless the point has to move
     float mx[NT][2];
     bool up = false;
@@ -189,6 +194,11 @@ __device__ __forceinline__ void dc_compute(DcState<NT>& st, DcGroup<GRAN>& r, co
     // first maximum, up or down, with sums that are zero.  Each head has its own bit for that: one whose scores are all NaN never gets it.
     if (__any_sync(0xffffffffu, up)) {
 #pragma unroll
+        for (int s = 0; s < SUB; ++s)
+#pragma unroll
+            for (int u = 0; u < UNITS; ++u)
+                if (r.vs[s][u] > q8_pow2(Q8_HIGH)) st.seen |= 1u << 31;
+#pragma unroll
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
@@ -198,7 +208,7 @@ __device__ __forceinline__ void dc_compute(DcState<NT>& st, DcGroup<GRAN>& r, co
                 const bool first = !(st.seen >> (2 * n + j) & 1);
                 const float by = x == -INFINITY ? 0.f : first ? x : fmaxf(x, 0.f), c = first ? 1.f : q8_ex2(-by);
                 st.m[n][j] += by;
-                st.l[n][j] *= c;
+                if (!first) st.l[n][j] = q8_add_scaled(st.l[n][j], -by, 0.f);
 #pragma unroll
                 for (int i = 0; i < HD / 16; ++i) { st.o[n][i][j] *= c; st.o[n][i][2 + j] *= c; }
                 if (x != -INFINITY) st.seen |= 1u << (2 * n + j);
@@ -207,6 +217,16 @@ __device__ __forceinline__ void dc_compute(DcState<NT>& st, DcGroup<GRAN>& r, co
             }
         }
     }
+    if (wide || st.seen >> 31)                                       // in place of what is added below
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int s = 0; s < SUB; ++s)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float vs = r.vs[s][UNITS == 1 ? 0 : j >> 1];
+                    st.l[n][j & 1] += q8_ex2(sc[n][s][j] - q8_log2(vs)) - q8_ex2(sc[n][s][j]) * q8_recip(vs);
+                }
     uint32_t pb[NT][SUB][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -441,9 +461,8 @@ __device__ __forceinline__ void dc_piece(const DcArgs& a, float* red_s, int e, i
 #pragma unroll
         for (int w = 0; w < DC_WARPS; ++w) {
             const float* rec = red_s + (size_t)(w * heads + h) * REC;
-            const float c = rec[0] == -INFINITY ? (m == -INFINITY ? 1.f : 0.f) : q8_ex2(rec[0] - m);       // (a warp that met only NaN kept its sums)
-            l = fmaf(rec[1], c, l);
-            acc = fmaf(rec[4 + d], c, acc);
+            l = q8_add_scaled(rec[1], q8_below(rec[0], m), l);
+            acc = fmaf(rec[4 + d], q8_ex2(q8_below(rec[0], m)), acc);
         }
         const size_t at = (size_t)row * a.nH + head0 + h;
         float* rec = a.scratch + (((size_t)e * a.nH + head0 + h) * a.n_splits + run) * REC;
@@ -651,6 +670,7 @@ attn_prefill_q8_kernel(const PfArgs a) {
 #pragma unroll
     for (int i = 0; i < HD / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
     float m_lo = -INFINITY, m_hi = -INFINITY, l_lo = 0.f, l_hi = 0.f;
+    bool high = false;                                               // (Q8_HIGH)
     constexpr bool Q_HELD = HD <= 64;
     uint32_t qa[Q_HELD ? HD / 16 : 1][4];
     if constexpr (Q_HELD)
@@ -707,22 +727,31 @@ attn_prefill_q8_kernel(const PfArgs a) {
             }
             const float n_lo = fmaxf(m_lo, mx_lo), n_hi = fmaxf(m_hi, mx_hi);
             const float c_lo = n_lo == -INFINITY ? 1.f : q8_ex2(m_lo - n_lo), c_hi = n_hi == -INFINITY ? 1.f : q8_ex2(m_hi - n_hi);
+            l_lo = q8_add_scaled(l_lo, q8_below(m_lo, n_lo), 0.f);
+            l_hi = q8_add_scaled(l_hi, q8_below(m_hi, n_hi), 0.f);
             m_lo = n_lo;
             m_hi = n_hi;
-            l_lo *= c_lo;
-            l_hi *= c_hi;
 #pragma unroll
             for (int i = 0; i < HD / 8; ++i) { o[i][0] *= c_lo; o[i][1] *= c_lo; o[i][2] *= c_hi; o[i][3] *= c_hi; }
         }
         const float ref_lo = m_lo == -INFINITY ? 0.f : m_lo, ref_hi = m_hi == -INFINITY ? 0.f : m_hi;
         uint32_t p[PF_KEYS / 16][4];
+        const float lg8 = sm->vl[s][lane & 7];                       // (minus infinity for keys that are hidden)
+        high = high || __any_sync(0xffffffffu, lg8 > Q8_HIGH);
+        const bool wide = __any_sync(0xffffffffu, lg8 < Q8_LOW && lg8 != -INFINITY) || high;
 #pragma unroll
         for (int nt = 0; nt < PF_KEYS / 8; ++nt) {
             const float p0 = q8_ex2(sc[nt][0] - ref_lo), p1 = q8_ex2(sc[nt][1] - ref_lo);
             const float p2 = q8_ex2(sc[nt][2] - ref_hi), p3 = q8_ex2(sc[nt][3] - ref_hi);
-            const float inv = sm->vi[s][nt];
-            l_lo = fmaf(p0 + p1, inv, l_lo);
-            l_hi = fmaf(p2 + p3, inv, l_hi);
+            if (wide) {
+                const float lg = sm->vl[s][nt] == -INFINITY ? 0.f : sm->vl[s][nt];
+                l_lo += q8_ex2(sc[nt][0] - ref_lo - lg) + q8_ex2(sc[nt][1] - ref_lo - lg);
+                l_hi += q8_ex2(sc[nt][2] - ref_hi - lg) + q8_ex2(sc[nt][3] - ref_hi - lg);
+            } else {
+                const float inv = sm->vi[s][nt];
+                l_lo = fmaf(p0 + p1, inv, l_lo);
+                l_hi = fmaf(p2 + p3, inv, l_hi);
+            }
             p[nt >> 1][(nt & 1) * 2 + 0] = pack_f16(p0, p1);
             p[nt >> 1][(nt & 1) * 2 + 1] = pack_f16(p2, p3);
         }

@@ -17,6 +17,10 @@
 // Keys that no row of the block sees, and keys whose page is not there, are stored as zeros (their codes may be NaN).  The latter are hidden: the
 // logarithm of their scale is minus infinity, and so is their z.  A NaN among the values of
 // a key that some rows of the block see reaches the others of its tile as well (0 NaN), as it does in a plain product with masked weights.
+// Denominators: a loader looks over the scales of the values as well.  If they lie so far apart that keys may have been lost to the denominator (Q8_LOW;
+// this kernel's bound is FAR_SCALES), the rows' denominators are formed again at the end, key by key.  Exponentials of their own in such tiles, as in the
+// other kernels, or the look at the scales in other warps, cost every cache 4 to 7 %: 2,048 tokens 41 -> 44 us, 512 behind 32,768 176 -> 184
+// (so 42 and 180).  The same two over a cache of such values: 0.9 and 4.7 ms.
 // Every mbarrier wait is bounded; a waiter that gives up sets a status bit and the block runs to its end.
 //
 // Bound by the softmax warps' instructions and by the handshakes of a tile (tensor pipe 28 %, exponential unit 57 %, issue slots 61 %
@@ -42,6 +46,7 @@ static_assert(HD == 64 || HD == 128, "head sizes 64 and 128");
 #define Q8P_THREADS (32 * (SOFTMAX_WARPS + 4))
 #define KV_WARPS 3
 #define MIN_RUN 4                    // a run of keys is at least this many tiles
+#define FAR_SCALES 100               // exponents' distance of scales up to which a key lost to the denominator counts less than 2^-26 of it
 static_assert(BQ == BLOCK_W, "a row tile is the 128 rows of the MMA");
 
 __device__ __forceinline__ float fmax3(float a, float b, float c) {
@@ -89,6 +94,7 @@ __device__ __forceinline__ void tmem_st16u(uint32_t taddr, const uint32_t (&v)[1
 struct Barriers {
     uint64_t q_full[2], kv_full[KV_STAGES], kv_empty[KV_STAGES], s_full[2][2], p_full[2][2], o_ready[2][2];          // [row tile][tile j & 1]
     uint64_t joined[2][4];                       // [row tile][warp]: the odd tiles' stream has left its reference point and sum
+    uint64_t scales_seen;                        // `far` is known
 };
 struct Smem {
     uint16_t q[2][NB][BQ * 64];                  // K-major, 128-byte swizzle, a block for each 64 of the head
@@ -97,7 +103,7 @@ struct Smem {
     float ks[KV_STAGES][8], vl[KV_STAGES][8], vi[KV_STAGES][8];       // of each 8 keys: K's scale, V's log2 and reciprocal
     Barriers b;
     float odd_m[BR], odd_l[BR], row_f[BR];       // row_f: what a row's raw products are multiplied by (base 2)
-    uint32_t tmem_base;
+    uint32_t tmem_base, far;                     // far: scales of values lie more than FAR_SCALES apart
 };
 
 struct Params {
@@ -114,12 +120,53 @@ struct Params {
 
 // half of a tile row's swizzled bytes: 16-byte chunk c (8 float16) of row r
 __device__ __forceinline__ int sw128(int r, int c) { return (r >> 3) * 512 + (r & 7) * 64 + ((c ^ (r & 7)) << 3); }
+// sum of 2^(x - top) over keys k0 .. k1 for row r of a row tile of q (float16, in shared memory), x = f * scale * (q . code) + slope (key - pos);
+// eight keys at a time (they lie in one page and one block)
+template <int KIND>
+__device__ __noinline__ float denominator(const Cache& c, const int* trow, int kvh, const uint16_t* q, int r, float f, float slope, float top,
+                                          int pos, int k0, int k1) {
+    const int mask = (1 << c.ps_log2) - 1;
+    float sum = 0.f;
+#pragma unroll 1
+    for (int key = k0 & ~7; key <= k1; key += 8) {
+        const int i = key >> c.ps_log2, page = i < c.table_stride ? trow[i] : -1;
+        if ((unsigned)page >= (unsigned)c.num_pages) continue;
+        const long long slab = (long long)page * c.nKV + kvh;
+        const unsigned char* codes = c.k + ((slab << c.ps_log2) + (key & mask)) * HD;
+        const float fk = f * c.ks[(slab << (c.ps_log2 - c.bl_log2)) + ((key & mask) >> c.bl_log2)];
+        float raw[8] = {};
+#pragma unroll 1
+        for (int ch = 0; ch < HD / 8; ++ch) {                  // eight dimensions
+            uint32_t w[8][2];
+#pragma unroll
+            for (int n = 0; n < 8; ++n) ld_codes<8>(w[n], codes + n * HD + ch * 8);
+            const uint4 x = *reinterpret_cast<const uint4*>(q + ch / 8 * (BQ * 64) + sw128(r, ch % 8));
+            const uint32_t qs[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+            for (int n = 0; n < 8; ++n)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    uint32_t h[2];
+                    q8_to_half<KIND>(w[n][j], h[0], h[1]);
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&qs[2 * j + u])), b = __half22float2(*reinterpret_cast<const __half2*>(&h[u]));
+                        raw[n] = fmaf(a.x, b.x, fmaf(a.y, b.y, raw[n]));
+                    }
+                }
+        }
+#pragma unroll
+        for (int n = 0; n < 8; ++n)
+            if (key + n >= k0 && key + n <= k1) sum += q8_ex2(fmaf(raw[n], fk, slope * (float)(key + n - pos)) - top);
+    }
+    return sum;
+}
 // kind::f16, float16 operands: as make_idesc without its bfloat16 bits
 __host__ __device__ constexpr uint32_t idesc_f16(int n, int b_mn) { return make_idesc(n, b_mn) & ~((1u << 7) | (1u << 10)); }
 
 template <int KIND>
 __global__ void __launch_bounds__(Q8P_THREADS, 1)
-attn_prefill_q8_sm100_kernel(const Params p) {
+attn_prefill_q8_sm100_kernel(const __grid_constant__ Params p) {
     extern __shared__ unsigned char smem_raw[];
     // (an offset, not a rounded address: the compiler then knows that what it points to is shared memory)
     Smem* sm = reinterpret_cast<Smem*>(smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u));
@@ -212,6 +259,7 @@ attn_prefill_q8_sm100_kernel(const Params p) {
         const unsigned char *k_pages = p.c.k + head_at, *v_pages = p.c.v + head_at;
         uint32_t k[DEPTH][UNITS][UNIT_LOADS][4], v[DEPTH][UNITS][UNIT_LOADS][4];
         float ks[DEPTH], vs[DEPTH];                            // (vs: -1 for a unit that has no page)
+        float low = INFINITY, high = 0.f;                      // the last loader's lanes: scales of values so far
         // (a page that is not there: page 0 is read, and the unit's keys become zeros when they are stored)
         bool bad[DEPTH][UNITS];
         auto load = [&](int d, int tile, const Pages& page) {
@@ -273,6 +321,7 @@ attn_prefill_q8_sm100_kernel(const Params p) {
                 if (w == KV_WARPS - 1 && lane < 8) {
                     sm->ks[s][lane] = ks[d];
                     sm->vl[s][lane] = vs[d] < 0.f ? -INFINITY : q8_log2(vs[d]);
+                    low = fminf(low, vs[d] < 0.f ? INFINITY : vs[d]), high = fmaxf(high, vs[d]);
                     sm->vi[s][lane] = q8_recip(vs[d]);         // (of a unit without a page: 1, times weights of 0)
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -281,6 +330,13 @@ attn_prefill_q8_sm100_kernel(const Params p) {
                 load(d, tile0 + j + DEPTH, page0);             // (behind the last tile: zeros, from no page)
                 page0 = pages(tile0 + j + DEPTH + 1);
             }
+        if (w == KV_WARPS - 1) {
+            const bool far = __any_sync(0xffffffffu, q8_log2(ng_warp_max(high)) - q8_log2(low) > FAR_SCALES);
+            if (lane == 0) {
+                sm->far = far;
+                mbar_arrive(&sm->b.scales_seen);
+            }
+        }
         if (!ok && lane == 0) atomicOr(p.status, NG_STATUS_ATTN_TIMEOUT);
     } else if (warp == SOFTMAX_WARPS + KV_WARPS) {
         // ------------------------------------------------------------------ MMA issuer: all lanes run the loop, one issues
@@ -453,7 +509,7 @@ attn_prefill_q8_sm100_kernel(const Params p) {
                     mx = fmax3(mx, fmaxf(mz[0], mz[1]), fmaxf(mz[2], mz[3]));
                 }
                 if (mx > m + 8.f || (!seen && mx > -INFINITY)) {           // move the reference point
-                    corr = seen ? q8_ex2(m - mx) : 0.f;
+                    corr = seen ? q8_ex2(m - mx) : 0.f;        // (sums that this loses: FAR_SCALES)
                     seen = true;
                     m = mx;
                     l *= corr;
@@ -523,6 +579,7 @@ attn_prefill_q8_sm100_kernel(const Params p) {
             ok = mbar_wait(&sm->b.o_ready[t][last_j & 1], (last_j >> 1) & 1);
             ok = __all_sync(0xffffffffu, ok);
         }
+        if (!odd && ok && n_mine > 0) ok = __all_sync(0xffffffffu, mbar_wait(&sm->b.scales_seen, 0));
         float m_odd = -INFINITY, l_odd = 0.f;
         if (STREAMS == 2 && n_mine > 1 && ok) {
             if (odd) {
@@ -544,10 +601,13 @@ attn_prefill_q8_sm100_kernel(const Params p) {
             const bool two = STREAMS == 2 && n_mine > 1, live = r < rows_mine;
             const float m_even = seen ? m : -INFINITY, top = fmaxf(m_even, m_odd);
             // (a stream that met only NaN has no reference point and keeps its sums)
-            float a = m_even == -INFINITY ? (top == -INFINITY ? 1.f : 0.f) : q8_ex2(m_even - top);
-            float b = m_odd == -INFINITY ? (top == -INFINITY ? 1.f : 0.f) : q8_ex2(m_odd - top);
+            float a = q8_ex2(q8_below(m_even, top)), b = q8_ex2(q8_below(m_odd, top));
             l = fmaf(l, a, l_odd * b);
             if (n_mine <= 0) l = 0.f;
+            else if (sm->far && live && top > -INFINITY) {
+                l = denominator<KIND>(p.c, p.c.table + (size_t)e * p.c.table_stride, kvh, sm->q[t][0], r, f, slope, top, pos,
+                                      max(tile0 * BK, p.window > 0 ? pos - p.window + 1 : 0), min((tile0 + n_mine) * BK - 1, pos));
+            }
             if (p.n_splits > 1 && live) rec[0] = n_mine > 0 ? top : -INFINITY, rec[1] = l;
             const float inv = l == 0.f ? 0.f : 1.f / l;
             if (p.n_splits == 1) a *= inv, b *= inv;

@@ -18,6 +18,21 @@ __device__ __forceinline__ float q8_ex2(float x) {       // 2^x, 2 ulp; -inf -> 
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// l 2^d + to, also where 2^d alone lies below the smallest normal number: a sum of 2^x over keys whose values have small scales is large (up to
+// 2^100 a key) beside a reference point that contains the scales, and is still there when keys with the largest scales have moved that point by 2^200.
+__device__ __forceinline__ float q8_add_scaled(float l, float d, float to) {
+    const bool far = d < -125.f;
+    const float c = q8_ex2(far ? 0.5f * d : d);
+    return fmaf(far ? l * c : l, c, to);
+}
+// how far a run's reference point lies below the highest of several; runs that met only NaN have none, and keep their sums
+__device__ __forceinline__ float q8_below(float ms, float m) { return m == -INFINITY ? 0.f : ms - m; }
+// The denominator takes a key's weight 2^(z - m) divided by its scale, and the weight is lost below 2^-126.  m is the z of a key that counts 2^-(its log2
+// scale) in the denominator, so what a lost key counts there is less than 2^-(126 - the distance of both scales' exponents) of it.  Keys
+// whose scale's log2 is below Q8_LOW, and all once a scale above Q8_HIGH has moved m, are added by exponentials of their own: what others
+// lose is below 2^-46.
+#define Q8_LOW (-40)
+#define Q8_HIGH 40
 // The power of two that a row of q is divided by (its largest value becomes 1 to 2): exponent of the row's largest finite value.
 __device__ __forceinline__ int q_exponent(float top) { return min(max((int)(__float_as_uint(top) >> 23) - 127, -100), 127); }
 __device__ __forceinline__ float pow2_any(int e) { return q8_pow2(min(max(e, -126), 127)); }
@@ -132,10 +147,9 @@ attn_q8_merge_kernel(const float* __restrict__ scratch, const int* __restrict__ 
                 ls = s1 < runs ? rec[(size_t)s1 * REC + 1] : 0.f;
             }
             if (s1 >= runs) ms = -INFINITY, ls = 0.f;
-            const float mb = fmaxf(m, ng_warp_max(ms)), c = m == -INFINITY ? (mb == -INFINITY ? 1.f : 0.f) : q8_ex2(m - mb);
-            const float f = ms == -INFINITY ? (mb == -INFINITY ? 1.f : 0.f) : q8_ex2(ms - mb);          // (a run that met only NaN kept its sums)
+            const float mb = fmaxf(m, ng_warp_max(ms)), c = q8_ex2(q8_below(m, mb)), f = q8_ex2(q8_below(ms, mb));
+            l = q8_add_scaled(l, q8_below(m, mb), ng_warp_sum(q8_add_scaled(ls, q8_below(ms, mb), 0.f)));
             m = mb;
-            l = fmaf(l, c, ng_warp_sum(ls * f));
 #pragma unroll
             for (int i = 0; i < MG_EACH; ++i) acc[i][0] *= c, acc[i][1] *= c;
             const uint32_t some = __ballot_sync(0xffffffffu, ls != 0.f);                               // (an empty run wrote no row)
@@ -173,8 +187,8 @@ attn_q8_merge_kernel(const float* __restrict__ scratch, const int* __restrict__ 
             for (int i = 0; i < MG_EACH; ++i) acc[i][0] = acc[i][1] = 0.f;
 #pragma unroll
             for (int w = 0; w < MG_WARPS; ++w) {
-                const float f = part_s[w][0] == -INFINITY ? (top == -INFINITY ? 1.f : 0.f) : q8_ex2(part_s[w][0] - top);
-                l = fmaf(part_s[w][1], f, l);
+                const float f = q8_ex2(q8_below(part_s[w][0], top));
+                l = q8_add_scaled(part_s[w][1], q8_below(part_s[w][0], top), l);
 #pragma unroll
                 for (int i = 0; i < MG_EACH; ++i) {
                     const int d = 2 * lane + 64 * i;

@@ -124,3 +124,36 @@ def test_keys_without_a_page_are_hidden_from_portions_and_single_tokens_alike(ki
     check_rows(run_prefill(c, q, 8, window, hd ** -0.5, splits, True, slopes), want, bound, many)
     none = list(range(c.cu_host[4], c.cu_host[5]))
     assert bool((portions[none] == 0).all())
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("hd", [48, 64, 128])
+@pytest.mark.parametrize("how", ["zeros", "any", "rising", "falling"])
+@pytest.mark.parametrize("portion", [False, True])
+def test_every_key_counts_whatever_the_scale_of_its_values(kind, hd, how, portion):
+    """Scales of values over their whole range, 2^-100 to 2^100: a key's weight in the denominator has nothing to do with them.  Rows of q of zero (all
+    keys alike) and others; the far scales in one warp's keys, in different ones, in different runs."""
+    c = Cache([5, 3, 2] if portion else [1, 1, 1], [30, 700, 1500], 2, hd, 16, 16, kind, seed=hd)
+    g = torch.Generator().manual_seed(8)
+    shape = c.vs.shape
+    if how == "zeros":                                       # blocks of zeros, at the least scale, beside blocks of large values
+        zero = torch.rand(shape, generator=g) < 0.5
+        exps = torch.full(shape, 27.0).masked_fill(zero, -100.0)
+        c.v.view(shape + (16, hd)).view(torch.uint8).masked_fill_(zero[..., None, None], 0)
+    elif how == "any":
+        exps = torch.randint(-100, 101, shape, generator=g).float()
+    else:                                                    # along each entry's keys, in a few steps
+        exps = torch.zeros(shape)
+        for e in range(3):
+            held = [p for p in c.table_host[e].tolist() if p >= 0]
+            for i, p in enumerate(held):
+                x = -100 + 50 * (4 * i // max(1, len(held) - 1))
+                exps[p] = x if how == "rising" else -x
+    c.dev[1], c.dev[3] = c.v.to(DEV), torch.pow(2.0, exps).to(DEV)
+    q = rnd(c.rows, 8 * hd, seed=1, std=1.5)
+    q.view(c.rows, 8, hd)[:, ::2] = 0.0
+    want, bound = ref.attention(q, *c.args(), c.cu_host, c.ctx, 8, None, hd ** -0.5)
+    assert bool(torch.isfinite(want).all())
+    for splits in (1, 2, 7):
+        got = (run_prefill if portion else run_decode)(c, q, 8, None, hd ** -0.5, splits)
+        check_rows(got, want, bound)
