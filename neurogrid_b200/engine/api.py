@@ -83,8 +83,9 @@ class Engine:
 
     def add_samples(self, prompt: Sequence[int], n: int, params: Optional[SamplingParams] = None,
                     rng_keys: Optional[Sequence[int]] = None) -> List[Hashable]:
-        """Queue ``n`` requests for the same prompt, each with a random stream of its own.  The prompt is read once; the others start
-        from copies of its state and share the pages that it has filled."""
+        """Queue ``n`` requests for the same prompt, each with a random stream of its own.  The first reads it; the others start from copies of its
+        state and share the pages that it has filled.  Those that find no slot (of ``max_requests``), or no page beside one for each running
+        request, at that moment wait as requests of their own and read the prompt again."""
         if n < 1 or (rng_keys is not None and len(rng_keys) != n):
             raise ValueError("n is at least 1, with a random stream for each sample or for none")
         ids = list(range(self._next_id, self._next_id + n))
@@ -182,7 +183,7 @@ class Engine:
                  top_p: float = 1.0, seed: int = DEFAULT_SEED, stop_token_ids: Sequence[int] = (),
                  ignore_eos: bool = False, n: int = 1) -> List[List[int]]:
         """Generated token ids for each prompt (prompt not included), in the order given.  ``n`` > 1: a list of that many
-        samples for each prompt, which is read once for all of them."""
+        samples for each prompt, which is read once for those that find room beside the first (``add_samples``)."""
         params = SamplingParams(temperature=temperature, top_p=top_p, max_new_tokens=max_new_tokens, seed=seed,
                                 stop_token_ids=tuple(stop_token_ids), ignore_eos=ignore_eos)
         ids = [i for k, p in enumerate(prompts) for i in self.add_samples(p, n, params, range(k * n, k * n + n))]

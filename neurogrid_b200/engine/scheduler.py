@@ -99,8 +99,8 @@ class Scheduler:
         self.waiting.append(req)
 
     def add_samples(self, req: Request, more: Sequence[Request]) -> None:
-        """Queue ``req`` and further samples of its prompt.  The prompt is read once, up to its last token; then the others are forked
-        off, each with the pages of what was read (they read the prompt themselves where no slot or page is free for that)."""
+        """Queue ``req`` and further samples of its prompt.  The prompt is read up to its last token; then the others are forked off, each with the
+        pages of what was read.  Those for which there is no slot, or no page beside one for each running request, read the prompt themselves."""
         self.add(req)
         for r in more:
             if len(req.prompt) < 2:
@@ -112,13 +112,19 @@ class Scheduler:
             r.state = WAITING
             req.forks.append(r)
 
+    def _room_to_fork(self, req: Request) -> bool:
+        """A slot, and in every group a page for the fork (a copy of the last page or, where that is full, its next token's) with one page of headroom
+        for each running request, as for an admission."""
+        return len(self.running) < self.max_requests and self.cache.can_fork(req.id) \
+            and all(free > len(self.running) for free in self.cache.pages_free())
+
     def _fork(self, plan: StepPlan) -> None:
         """Fork the requests whose prompt has been read up to its last token."""
         for req in list(self.running):
             if not req.forks or req.fed < len(req.prompt) - 1:
                 continue
             for r in req.forks:
-                if len(self.running) < self.max_requests and self.cache.can_fork(req.id):
+                if self._room_to_fork(req):
                     plan.forks.append(self.cache.fork(req.id, r.id))
                     r.fed, r.state = req.fed, RUNNING
                     self.running.append(r)
@@ -188,6 +194,9 @@ class Scheduler:
                 if len(self.running) == 1:
                     plan.failed += self._fail(victim, "cache_full")
                 else:
+                    if self.cache.is_live(victim.id):            # (a fork of this plan: its copies are not made)
+                        slot = self.cache.slot(victim.id)
+                        plan.forks = [f for f in plan.forks if f[1] != slot]
                     self._preempt(victim)
                     plan.preempted.append(victim)
                 continue
