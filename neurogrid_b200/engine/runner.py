@@ -23,6 +23,7 @@ import torch
 from ..cache.manager import CacheManager, PagedNeed
 from ..cache.pages import OutOfPages
 from ..cache.storage import CacheStorage, page_bytes, parse_cache_dtype
+from ..parts.attention import Q8_SCRATCH_FLOATS
 from ..parts.base import PagedView, SlotView, StepContext, Workspace
 
 
@@ -135,6 +136,15 @@ class ModelRunner:
         """Device bytes one page id costs over all paged layers (keys and values)."""
         cache_dtype = parse_cache_dtype(cache_dtype)
         return sum(page_bytes(n, page_size, model.dtype, cache_dtype) for n in cls._paged(model.cache_needs()))
+
+    @classmethod
+    def workspace_reserve(cls, model, max_tokens_per_step: int, cache_dtype: Optional[str] = None) -> int:
+        """Device bytes to leave beside the page pool: the eager workspace and the one the portion graphs keep are allocated at the first steps, after
+        the pool, and over a cache in 8 bits each workspace (the eager one, and those of the graphs of single tokens, portions and mixed steps) holds
+        records of runs."""
+        rows = max_tokens_per_step + min(max_tokens_per_step, cls.MAX_PORTION_ROWS)
+        records = 4 * 4 * Q8_SCRATCH_FLOATS if cache_dtype is not None else 0
+        return rows * model.activation_bytes_per_row() + 2 * cls.MAX_PORTION_LOGITS_BYTES + records
 
     # ------------------------------------------------------------------ requests
     def admit(self, req_id: Hashable) -> int:

@@ -21,3 +21,14 @@ def test_tensor_memory_is_taken_after_the_kernels_before_and_before_the_kernels_
     assert body.rindex("ng_pdl_wait()", 0, alloc) < alloc < body.index("__syncthreads()", alloc) < signal
     # between the last wait in front of the allocation and the allocation nothing returns
     assert "return" not in body[body.rindex("ng_pdl_wait()", 0, alloc):alloc]
+
+
+def test_room_is_left_for_the_records_of_every_workspace(model_dirs):
+    """The page pool is sized from what the workspaces leave: over a cache in 8 bits each of the four holds records of its own."""
+    from neurogrid_b200.engine import ModelRunner
+    from neurogrid_b200.engine.loading import model_from_dir
+    from neurogrid_b200.parts.attention import Q8_SCRATCH_FLOATS
+    _, model = model_from_dir(model_dirs["D"], dtype="bfloat16", device="cpu")
+    plain = ModelRunner.workspace_reserve(model, 256)
+    assert plain == 2 * 256 * model.activation_bytes_per_row() + 2 * ModelRunner.MAX_PORTION_LOGITS_BYTES
+    assert ModelRunner.workspace_reserve(model, 256, "e4m3") == plain + 4 * 4 * Q8_SCRATCH_FLOATS
