@@ -713,9 +713,10 @@ def attn_decode_q8(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
                    slopes: Optional[torch.Tensor] = None) -> None:
     """``attn_decode_bf16`` over a cache in 8 bits (``cache_write_q8``): split-context attention of the entries that bring one token, any
     number of query heads a KV head.  The rows of other entries stay as they were.  Keys whose page the table does not have (-1, or a
-    number beyond the pool) are hidden; a row that sees no key is zero.  ``n_splits`` (``attn_decode_q8_splits``) runs of
-    the keys, planned for contexts of up to ``max_ctx`` (longer ones are right too); ``scratch`` holds ``attn_q8_scratch_floats`` (of
-    ``n_entries``) float32 values when there is more than one."""
+    number beyond the pool) are hidden; a row that sees no key is zero.  ``n_splits`` is how many runs an
+    entry's keys may be cut into (``attn_decode_q8_splits`` plans it for contexts of some length; longer ones are right too), and ``scratch`` holds
+    ``attn_q8_scratch_floats`` (of ``n_entries``) float32 values when it is more than one.  The runs are found on the device:
+    ``max_ctx`` stands here as it does in ``attn_decode_bf16`` and changes nothing."""
     hd, stream, at, rest = _q8_attention("attn_decode_q8", q, k_pages, v_pages, k_scales, v_scales, table, cu_q, ctx_before, out, scratch, n_entries,
                                  1, n_heads, window, scale, 0, n_splits, slopes, n_entries)
     _check(_q8_fn("attention_q8", "ng_attn_decode_q8", hd)(_Q8_ATTENTION.pack(*at, 0, *rest), stream), "attn_decode_q8")

@@ -157,3 +157,28 @@ def test_every_key_counts_whatever_the_scale_of_its_values(kind, hd, how, portio
     for splits in (1, 2, 7):
         got = (run_prefill if portion else run_decode)(c, q, 8, None, hd ** -0.5, splits)
         check_rows(got, want, bound)
+
+
+def test_decode_planned_for_short_contexts_serves_long_ones():
+    """The number of runs comes from a plan for 1,400 tokens, and stays in a captured graph, while contexts grow to more than four times that."""
+    nH, nKV, hd, page, n = 8, 2, 64, 16, 3
+    splits = ops().attn_decode_q8_splits(n, nH, nKV, hd, 1400, None, torch.device(DEV, 0))
+    assert splits > 1
+    c = Cache([1] * n, [6399, 4000, 1], nKV, hd, page, 16, INT8, stride=400, dirty=False)
+    q = rnd(n, nH * hd, seed=1)
+    out = torch.empty_like(q)
+    scratch = torch.full((ops().attn_q8_scratch_floats(n, nH, hd, splits),), math.nan, device=DEV)
+
+    def call():
+        ops().attn_decode_q8(q, *c.args(), c.cu, c.ctx_d, out, scratch, n, nH, None, 0.125, splits, 1400)
+
+    call()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        call()
+    for ctx in ([899, 20, 1], [2000, 899, 0], [6399, 4000, 1]):
+        c.ctx = ctx
+        c.ctx_d.copy_(torch.tensor(ctx, dtype=torch.int32))
+        graph.replay()
+        check_rows(out, *ref.attention(q, *c.args(), c.cu_host, ctx, nH, None, 0.125))
