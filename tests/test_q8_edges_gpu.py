@@ -182,3 +182,14 @@ def test_decode_planned_for_short_contexts_serves_long_ones():
         c.ctx_d.copy_(torch.tensor(ctx, dtype=torch.int32))
         graph.replay()
         check_rows(out, *ref.attention(q, *c.args(), c.cu_host, ctx, nH, None, 0.125))
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("lens,ctx,window,splits", [([256], [0], None, 2), ([256], [70], None, 5), ([200, 256], [40, 130], None, 6), ([256], [600], 100, 3),
+                                                   ([129], [60], None, 4), ([300], [1], None, 7), ([200], [120], None, 2), ([256], [100], None, 3)])
+def test_runs_of_keys_that_only_the_second_row_tile_sees(hd, lens, ctx, window, splits):
+    """One query head a KV head: a block's first 128 tokens end two key tiles before its last 128 do, so runs begin behind what they see."""
+    c = Cache(lens, ctx, 2, hd, 16, 16, E4M3, seed=hd)
+    q = rnd(c.rows, 2 * hd, seed=4, std=1.5)
+    want, bound = ref.attention(q, *c.args(), c.cu_host, c.ctx, 2, window, hd ** -0.5)
+    check_rows(run_prefill(c, q, 2, window, hd ** -0.5, splits), want, bound)
