@@ -31,8 +31,10 @@ class Engine:
         reference's flag does).  ``num_pages`` defaults to room for ``max_requests`` full
         contexts, limited to ``cache_memory_fraction`` of the free device memory (the reference
         sizes its pool to 25% of free VRAM, pkg/inference/engine_gpu.go:224-243).  ``cache_dtype``: "e4m3" or "int8" holds the
-        keys and values of grouped-query attention in 8 bits (half the memory and, in decoding, half the traffic of bfloat16;
-        a value is off by at most 2^-4 of itself (e4m3) or half a step of its block's scale (int8))."""
+        keys and values of grouped-query attention in 8 bits (half the memory and, in decoding, half the traffic of bfloat16).
+        With s the scale of a value's block of 16 tokens and head, it is off by at most 2^-4 of itself or, if that is more, 2^-10 s (e4m3),
+        or by s / 2 (int8), where the block was written at once; where it filled over several steps and s grew, by less than 2^-4 of
+        itself + 2^-9 s (e4m3), or s (int8)."""
         self.device = require_cuda(f"cuda:{gpu}")
         self.dtype = parse_dtype(dtype)
         if model is not None:
