@@ -727,6 +727,7 @@ attn_prefill_q8_kernel(const PfArgs a) {
             }
             const float n_lo = fmaxf(m_lo, mx_lo), n_hi = fmaxf(m_hi, mx_hi);
             const float c_lo = n_lo == -INFINITY ? 1.f : q8_ex2(m_lo - n_lo), c_hi = n_hi == -INFINITY ? 1.f : q8_ex2(m_hi - n_hi);
+            high = high || __any_sync(0xffffffffu, sm->vl[s][lane & 7] > Q8_HIGH);
             l_lo = q8_add_scaled(l_lo, q8_below(m_lo, n_lo), 0.f);
             l_hi = q8_add_scaled(l_hi, q8_below(m_hi, n_hi), 0.f);
             m_lo = n_lo;
@@ -737,21 +738,23 @@ attn_prefill_q8_kernel(const PfArgs a) {
         const float ref_lo = m_lo == -INFINITY ? 0.f : m_lo, ref_hi = m_hi == -INFINITY ? 0.f : m_hi;
         uint32_t p[PF_KEYS / 16][4];
         const float lg8 = sm->vl[s][lane & 7];                       // (minus infinity for keys that are hidden)
-        high = high || __any_sync(0xffffffffu, lg8 > Q8_HIGH);
-        const bool wide = __any_sync(0xffffffffu, lg8 < Q8_LOW && lg8 != -INFINITY) || high;
+        if (__any_sync(0xffffffffu, (lg8 < Q8_LOW && lg8 != -INFINITY) || high))
+#pragma unroll
+            for (int nt = 0; nt < PF_KEYS / 8; ++nt) {               // in place of what is added below
+                const float lg = sm->vl[s][nt] == -INFINITY ? 0.f : sm->vl[s][nt], inv = sm->vi[s][nt];
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    l_lo += q8_ex2(sc[nt][j] - ref_lo - lg) - q8_ex2(sc[nt][j] - ref_lo) * inv;
+                    l_hi += q8_ex2(sc[nt][2 + j] - ref_hi - lg) - q8_ex2(sc[nt][2 + j] - ref_hi) * inv;
+                }
+            }
 #pragma unroll
         for (int nt = 0; nt < PF_KEYS / 8; ++nt) {
             const float p0 = q8_ex2(sc[nt][0] - ref_lo), p1 = q8_ex2(sc[nt][1] - ref_lo);
             const float p2 = q8_ex2(sc[nt][2] - ref_hi), p3 = q8_ex2(sc[nt][3] - ref_hi);
-            if (wide) {
-                const float lg = sm->vl[s][nt] == -INFINITY ? 0.f : sm->vl[s][nt];
-                l_lo += q8_ex2(sc[nt][0] - ref_lo - lg) + q8_ex2(sc[nt][1] - ref_lo - lg);
-                l_hi += q8_ex2(sc[nt][2] - ref_hi - lg) + q8_ex2(sc[nt][3] - ref_hi - lg);
-            } else {
-                const float inv = sm->vi[s][nt];
-                l_lo = fmaf(p0 + p1, inv, l_lo);
-                l_hi = fmaf(p2 + p3, inv, l_hi);
-            }
+            const float inv = sm->vi[s][nt];
+            l_lo = fmaf(p0 + p1, inv, l_lo);
+            l_hi = fmaf(p2 + p3, inv, l_hi);
             p[nt >> 1][(nt & 1) * 2 + 0] = pack_f16(p0, p1);
             p[nt >> 1][(nt & 1) * 2 + 1] = pack_f16(p2, p3);
         }
