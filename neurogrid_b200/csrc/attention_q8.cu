@@ -37,10 +37,10 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], u
 // merge, the piece's number within the segment as the run's.  So batches of unequal lengths, and segments a little more than the blocks, fill
 // the GPU evenly.
 //
-// Bound by the codes' bytes where there are many (2 requests behind 131,072 tokens, 32 / 8 heads of 128: 86 us, 6.2 TB/s = 0.95 of a plain copy's rate) and else by
+// Bound by the codes' bytes where there are many (2 requests behind 131,072 tokens, 32 / 8 heads of 128: 87.5 us, 6.1 TB/s = 0.94 of a plain copy's rate) and else by
 // the chain of a group: page numbers -> codes -> products -> maximum -> weights -> products, three blocks an SM wide (64 requests of
-// up to 4,096 tokens, 32 / 8 heads of 64, integers: 39 us, 4.3 TB/s; the loads alone take 33, the arithmetic alone 34).  8 requests behind
-// 2,100 tokens 10.5 us, 1 behind 300 4.2 us.  Codes through a ring in shared memory (cp.async, 2 to 4 stages) took 43 to 48 us for the 64 requests
+// up to 4,096 tokens, 32 / 8 heads of 64, integers: 39.5 us, 4.3 TB/s; the loads alone take 33, the arithmetic alone 34).  8 requests behind
+// 2,100 tokens 10.0 us, 1 behind 300 4.2 us.  Codes through a ring in shared memory (cp.async, 2 to 4 stages) took 43 to 48 us for the 64 requests
 // (more work for the load and store unit), groups of 16 keys or of 64 were slower with heads of 64, conversions cost nothing that could be seen.
 #define DC_WARPS 4
 #define DC_THREADS (DC_WARPS * 32)
@@ -511,7 +511,7 @@ attn_decode_q8_kernel(const DcArgs a) {
 // all of them.  64-key tiles: the codes of the next tile are requested into registers while this one is computed, then written to shared
 // memory as float16 (two stages, one barrier a tile); scores, weights and sums as for single tokens, 16 rows a warp.
 // For the heads that attention_q8_sm100.cu does not take, and what it refuses.  Bound by `mma.sync` and its ldmatrix loads (2,048 tokens, 32 / 8
-// heads of 64: 91 us, there 41; 512 behind 32,768 1,313 and 178).
+// heads of 64: 97 us, there 42; 512 behind 32,768 496 and 180).
 #define PF_WARPS 8
 #define PF_THREADS (PF_WARPS * 32)
 #define PF_ROWS (PF_WARPS * 16)

@@ -23,10 +23,10 @@
 // (so 42 and 180).  The same two over a cache of such values: 0.9 and 4.7 ms.
 // Every mbarrier wait is bounded; a waiter that gives up sets a status bit and the block runs to its end.
 //
-// Bound by the softmax warps' instructions and by the handshakes of a tile (tensor pipe 28 %, exponential unit 57 %, issue slots 61 %
+// Bound by the softmax warps' instructions and by the handshakes of a tile (tensor pipe 28 %, exponential unit 56 %, issue slots 60 %
 // busy): 0.93 us for 64 keys of 256 rows, and about 7 us for a block's start and end.  512 tokens behind 32,768 (24 / 8 heads of 64)
-// 178 us = 582 TFLOP/s; 2,048 tokens, 32 / 8 heads of 64: 41 us; 6 requests of up to 611 tokens, 16 / 4 heads of 128, 65 us.  One row tile a block, two blocks an SM
-// 221 us instead of 178; one stream a row tile 214; registers moved from loaders to softmax warps, exponentials of two streams in turn, two
+// 180 us = 577 TFLOP/s; 2,048 tokens, 32 / 8 heads of 64: 42 us; 6 requests of up to 611 tokens, 16 / 4 heads of 128, 65 us.  One row tile a block, two blocks an SM
+// 221 us where this was 178; one stream a row tile 214; registers moved from loaders to softmax warps, exponentials of two streams in turn, two
 // issuers, scores of 128 keys at once, 6 or 8 stages: no gain or slower.
 #include <cstddef>
 #include <type_traits>

@@ -5,6 +5,10 @@ stream to the C launcher, and raises on a refused size.  There is no CPU path: a
 that is not on a CUDA device is an error, and so is a missing compiler or library.
 Shapes in the docstrings use N = rows (tokens) of the step, R = entries (requests) of the
 step, H = model width.
+
+Kernels are launched so that they begin while those in front of them on the stream end, and many read the description of the step (block
+tables, row_entry, cu_q, ctx_before, positions) before those have ended.  The step function fills it by a copy from the host, which is
+complete by then; a caller whose own kernel writes it has to let that kernel end first.
 """
 from __future__ import annotations
 
